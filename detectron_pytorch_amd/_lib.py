@@ -11,13 +11,17 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmi_detectron_ops.so")
 
 MI_OK = 0
-ABI_VERSION = 8  # MI_ABI_VERSION of include/mi_detectron_ops.h this binding was written against
+ABI_VERSION = 9  # MI_ABI_VERSION of include/mi_detectron_ops.h this binding was written against
 LAYOUT_NCHW, LAYOUT_NHWC = 0, 1
 ROI_ALIGN_CAFFE2, ROI_ALIGN_LEGACY = 0, 1
 NMS_GE_ORIG_ASC, NMS_GT_SORTED_POS = 0, 1
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+REDUCTION_NONE, REDUCTION_MEAN, REDUCTION_SUM = 0, 1, 2
+PASS_FORWARD, PASS_FORWARD_PRED, PASS_BACKWARD = 0, 1, 2
 ROI_ALIGN_RECORDS_READY, ROI_ALIGN_OVERWRITE = 1, 2
 
 _c_int, _c_float, _c_void_p, _c_size_t = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
+_c_longlong = ctypes.c_longlong
 
 # name -> (restype, argtypes); mirrors include/mi_detectron_ops.h declaration by declaration
 SIGNATURES = {
@@ -81,6 +85,18 @@ SIGNATURES = {
     "mi_mask_paste_rle": (_c_int, [_c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_void_p,
                                   _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p]),
     "mi_keypoint_decode": (_c_int, [_c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p]),
+    "mi_linear_cross_entropy_saved_bytes": (_c_size_t, [_c_int] * 4 + [_c_void_p, _c_longlong]),
+    "mi_linear_cross_entropy_workspace_bytes": (_c_size_t, [_c_int] * 5),
+    "mi_linear_cross_entropy_forward": (_c_int, [_c_void_p, _c_longlong, _c_void_p, _c_longlong, _c_void_p, _c_void_p]
+                                        + [_c_int] * 5 + [_c_longlong, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_size_t,
+                                                          _c_void_p, _c_size_t, _c_void_p]),
+    "mi_linear_cross_entropy_backward": (_c_int, [_c_void_p, _c_void_p, _c_longlong, _c_void_p] + [_c_int] * 5
+                                         + [_c_void_p] * 4 + [_c_size_t, _c_void_p, _c_size_t, _c_void_p]),
+    "mi_orthogonalize_workspace_bytes": (_c_size_t, [_c_int, _c_void_p, _c_void_p]),
+    "mi_orthogonalize": (_c_int, [_c_int] + [_c_void_p] * 4 + [_c_int, _c_int, _c_void_p, _c_float, _c_void_p, _c_size_t,
+                                                             _c_void_p]),
+    "mi_muon_step": (_c_int, [_c_int] + [_c_void_p] * 5 + [_c_int, _c_float, _c_float, _c_int, _c_float, _c_int, _c_void_p,
+                                                         _c_float, _c_void_p, _c_size_t, _c_void_p]),
     "mi_dbg_roi_align_timeline": (None, [_c_void_p]),
     "mi_dbg_reload_tuning": (None, []),
     "mi_dbg_copy_float4": (_c_int, [_c_void_p, _c_void_p, _c_size_t, _c_void_p]),

@@ -21,13 +21,17 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB_NAME = "libmi_detectron_ops.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
-SOURCES = ["abi.hip", "roi_align.hip", "roi_align_records.hip", "roi_align_nhwc.hip", "roi_pool.hip", "roi_crop.hip", "nms.hip", "soft_nms.hip", "proposals.hip", "affine_channel.hip", "topk.hip", "results.hip", "box_voting.hip", "mask_targets.hip"]
+SOURCES = ["abi.hip", "roi_align.hip", "roi_align_records.hip", "roi_align_nhwc.hip", "roi_pool.hip", "roi_crop.hip", "nms.hip", "soft_nms.hip", "proposals.hip", "affine_channel.hip", "topk.hip", "results.hip", "box_voting.hip", "mask_targets.hip",
+           "linear_cross_entropy.hip", "orthogonalize.hip"]
 ARCH = "gfx950"
 # Per-unit flags.  roi_align_records.hip: the leading scalar / pointer kernel arguments arrive preloaded in SGPRs (gfx950
 # kernarg preload) -- the records-free RoIAlign forward starts with a chain of dependent fetches (arguments -> the RoI's five
 # floats -> geometry -> window), and this takes the first link out of it.
 UNIT_FLAGS = {"roi_align_records.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=14"],
-              "roi_align_nhwc.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=14"]}
+              "roi_align_nhwc.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=14"],
+              # scalar FP32 arithmetic only: some packed forms have given wrong results on this hardware
+              "linear_cross_entropy.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"],
+              "orthogonalize.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]}
 
 
 def hipcc():

@@ -1,0 +1,818 @@
+// linear_cross_entropy.hip -- softmax cross entropy of a linear classifier, forward and backward, without the logits in memory.
+//
+// Mathematics, for rows x_i (features), classes w_v with bias b_v, and labels y_i:
+//   z_iv = x_i . w_v + b_v,   lse_i = log sum_v exp z_iv,   l_i = lse_i - z_i,y_i
+//   q_iv = exp(z_iv - lse_i) - [v = y_i],   dx_i = g_i sum_v q_iv w_v,   dw_v = sum_i g_i q_iv x_i,   db_v = sum_i g_i q_iv
+// The [rows, classes] logits are formed tile by tile on the matrix cores (tile_product.h) and die in registers: the forward
+// keeps, per row and strip of columns, the running maximum and the sum of exponentials, and a second kernel joins the
+// strips.  The backward forms the same tiles again, piece of the vocabulary by piece, turns them into q (16 bits, bounded
+// workspace) and multiplies q by the weights and by the features.
+//
+// Work: 2 R V D operations forward, 6 R V D backward (one third of it the logits' second time).  Bound by the matrix cores
+// wherever R and V fill the chip; by launches and the latency of a K loop where they do not.
+//
+// Types.  16-bit features and weights are multiplied as they are, in place.  float32 ones are laid out as hi + lo fp16 under one
+// power-of-two scale per tensor (its largest finite magnitude lands in [2^14, 2^15), so hi + lo carry 22 bits for
+// everything within 2^18 of it and lose one bit per halving below).  Maximum, sum, lse, loss and all accumulators are float32;
+// the sum over rows is fp64.  q is rounded once, to the features' type: |q| <= 1 and the error of a gradient element
+// is that of a sum of such roundings, below the rounding of the gradient itself; for float32 q is hi + lo again.
+//
+// Rows with the ignored label are laid out as zeros, whatever they hold, and get q = 0.  A label that is neither ignored nor
+// a class makes its row's loss and gradient NaN.
+#include "common.h"
+#include "tile_product.h"
+
+#include <cmath>
+
+namespace mi {
+namespace {
+
+constexpr int kPad = 64;              // rows and classes of the operands' k axes are padded to this
+constexpr int kMaxParts = 1024;       // workgroups of the maximum's pass
+constexpr float kQScale = 16384.f;    // q is stored times 2^14: fp16 keeps probabilities down to 2^-38
+constexpr int kIgnored = -1, kOutside = -2;
+constexpr size_t kPieceBytes = size_t(256) << 20;  // q of one piece of the vocabulary
+
+__device__ __forceinline__ float to_float(uint16_t v, bool bf16) {
+  return bf16 ? __uint_as_float((unsigned)v << 16) : (float)__builtin_bit_cast(_Float16, v);
+}
+template <int T>
+__device__ __forceinline__ float load_as_float(const void* p, long long i) {
+  if constexpr (T == MI_TYPE_F32)
+    return static_cast<const float*>(p)[i];
+  else
+    return to_float(static_cast<const uint16_t*>(p)[i], T == MI_TYPE_BF16);
+}
+__device__ __forceinline__ uint16_t half_bits(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
+__device__ __forceinline__ uint16_t bf16_bits(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
+template <int T>
+__device__ __forceinline__ uint16_t round16(float v) {
+  if constexpr (T == MI_TYPE_BF16)
+    return bf16_bits(v);
+  else
+    return half_bits(v);
+}
+template <int T>
+__device__ __forceinline__ void store_from_float(void* p, long long i, float v) {
+  if constexpr (T == MI_TYPE_F32)
+    static_cast<float*>(p)[i] = v;
+  else
+    static_cast<uint16_t*>(p)[i] = round16<T>(v);
+}
+
+// What a forward keeps for its backward and what both work with, all inside the caller's two buffers.
+struct Plan {
+  int rows, dim, classes;
+  int rows_p, dim_p;        // padded to kPad
+  bool split, copy_w;       // float32; weights laid out anew (float32, or 16-bit ones that the product cannot take in place)
+  long long ld;             // words between rows of a laid-out operand
+  size_t x_at, w_at, lab_at, lse_at, scalars_at, saved_bytes;
+};
+
+size_t up(size_t v) { return (v + 255) & ~size_t(255); }
+
+Plan make_plan(int rows, int dim, int classes, int dtype, bool w_in_place) {
+  Plan p;
+  p.rows = rows, p.dim = dim, p.classes = classes;
+  p.rows_p = (rows + kPad - 1) / kPad * kPad;
+  p.dim_p = (dim + kPad - 1) / kPad * kPad;
+  p.split = dtype == MI_TYPE_F32;
+  p.copy_w = p.split || !w_in_place;
+  p.ld = (long long)p.dim_p * (p.split ? 2 : 1);
+  size_t at = 0;
+  p.x_at = at, at = up(at + (size_t)p.rows_p * p.ld * 2);
+  p.w_at = at, at = up(at + (p.copy_w ? (size_t)classes * p.ld * 2 : 0));
+  p.lab_at = at, at = up(at + (size_t)p.rows_p * 4);
+  p.lse_at = at, at = up(at + (size_t)p.rows_p * 4);
+  p.scalars_at = at, at = up(at + 64);
+  p.saved_bytes = at;
+  return p;
+}
+
+struct Scalars {      // at scalars_at
+  float scale_x, scale_w;  // powers of two
+  float inv_x, inv_w;
+  float count;             // rows that count, at least 1
+};
+
+// ---- laying out --------------------------------------------------------------------------------------------------------
+
+// 2^(14 - floor(log2 m)); 1 for zero and for what is no number
+__device__ __forceinline__ float scale_of(float m) {
+  if (!(m > 0.f) || m > 3.402823466e38f) return 1.f;
+  int e = 14 - ilogbf(m);
+  return ldexpf(1.f, min(max(e, -120), 120));
+}
+
+template <class LABEL>
+__device__ __forceinline__ bool ignored_row(const LABEL* labels, int row, long long ignore) {
+  return (long long)labels[row] == ignore;
+}
+
+// Largest finite magnitude of the features (blocks below `x_blocks`) and of the weights (the others): one value per block.
+template <class LABEL>
+__global__ __launch_bounds__(256) void largest(const float* x, long long x_stride, const float* w, long long w_stride,
+                                               const LABEL* labels, long long ignore, int rows, int classes, int dim,
+                                               int x_blocks, float* parts) {
+  const bool is_x = (int)blockIdx.x < x_blocks;
+  const float* src = is_x ? x : w;
+  const long long stride = is_x ? x_stride : w_stride;
+  const int n = is_x ? rows : classes, blocks = is_x ? x_blocks : gridDim.x - x_blocks;
+  const int b = is_x ? blockIdx.x : blockIdx.x - x_blocks;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  float m = 0.f;
+  for (int r = b * 4 + wave; r < n; r += blocks * 4) {
+    if (is_x && ignored_row(labels, r, ignore)) continue;
+    const float* p = src + (long long)r * stride;
+    for (int c = lane; c < dim; c += 64) {
+      const float v = fabsf(p[c]);
+      if (v <= 3.402823466e38f) m = fmaxf(m, v);
+    }
+  }
+  for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+  __shared__ float s[4];
+  if (lane == 0) s[wave] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) parts[blockIdx.x] = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+}
+
+// Features (rows_p rows; ignored ones and the padding are zeros), weights and labels in the product's form.  A wave takes one
+// row at a time, a lane eight elements of it.
+template <int T, class LABEL>
+__global__ __launch_bounds__(256) void lay_out(const void* x, long long x_stride, const void* w, long long w_stride,
+                                               const LABEL* labels, long long ignore, int rows, int rows_p, int classes,
+                                               int dim, int dim_p, uint16_t* xo, uint16_t* wo, int* lab, const float* parts,
+                                               int x_parts, int w_parts, Scalars* sc) {
+  constexpr bool split = T == MI_TYPE_F32;
+  __shared__ float scales[2];
+  if constexpr (split) {
+    __shared__ float s[2][4];
+    float mx = 0.f, mw = 0.f;
+    for (int i = threadIdx.x; i < x_parts; i += 256) mx = fmaxf(mx, parts[i]);
+    for (int i = threadIdx.x; i < w_parts; i += 256) mw = fmaxf(mw, parts[x_parts + i]);
+    for (int d = 32; d; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d)), mw = fmaxf(mw, __shfl_xor(mw, d));
+    if ((threadIdx.x & 63) == 0) s[0][threadIdx.x >> 6] = mx, s[1][threadIdx.x >> 6] = mw;
+    __syncthreads();
+    if (threadIdx.x < 2) {
+      const float* v = s[threadIdx.x];
+      scales[threadIdx.x] = scale_of(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
+    }
+    __syncthreads();
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    sc->scale_x = split ? scales[0] : 1.f, sc->scale_w = split ? scales[1] : 1.f;
+    sc->inv_x = 1.f / sc->scale_x, sc->inv_w = 1.f / sc->scale_w;
+  }
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < rows_p; i += gridDim.x * 256) {
+    const long long y = i < rows ? (long long)labels[i] : ignore;
+    lab[i] = y == ignore ? kIgnored : (y >= 0 && y < classes) ? (int)y : kOutside;
+  }
+  const int total = rows_p + (wo != nullptr ? classes : 0);
+  const int lane = threadIdx.x & 63;
+  for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < total; r += gridDim.x * 4) {
+    const bool is_x = r < rows_p;
+    const int row = is_x ? r : r - rows_p;
+    const bool zero = is_x && (row >= rows || ignored_row(labels, row, ignore));
+    const void* src = is_x ? x : w;
+    const long long from = (long long)row * (is_x ? x_stride : w_stride);
+    uint16_t* to = (is_x ? xo : wo) + (long long)row * dim_p * (split ? 2 : 1);
+    const float scale = split ? scales[is_x ? 0 : 1] : 1.f;
+    for (int c = lane * 8; c < dim_p; c += 512) {
+      s16x8 hi = {0, 0, 0, 0, 0, 0, 0, 0}, lo = hi;
+      if (!zero) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < dim) {
+            if constexpr (split) {
+              const float v = static_cast<const float*>(src)[from + c + e] * scale;
+              const _Float16 h = (_Float16)v;
+              hi[e] = __builtin_bit_cast(short, h);
+              lo[e] = (short)half_bits(v - (float)h);
+            } else {
+              hi[e] = static_cast<const short*>(src)[from + c + e];
+            }
+          }
+      }
+      if constexpr (split) {
+        uint16_t* at = to + (c >> 5) * 64 + (c & 31);
+        *reinterpret_cast<s16x8*>(at) = hi;
+        *reinterpret_cast<s16x8*>(at + 32) = lo;
+      } else {
+        *reinterpret_cast<s16x8*>(to + c) = hi;
+      }
+    }
+  }
+}
+
+// ---- forward -------------------------------------------------------------------------------------------------------------
+
+struct Best {  // largest logit of a row and its lowest class; a NaN is the largest of all
+  float v;
+  int at;
+};
+__device__ __forceinline__ bool beats(float v, int at, const Best& b) {
+  const bool nv = v != v, nb = b.v != b.v;
+  if (nv != nb) return nv;
+  if (nv || v == b.v) return at < b.at;
+  return v > b.v;
+}
+
+// One tile of logits -> per row and strip of columns (one strip per wave column) the maximum and the sum of exp(z - max).
+template <class P, int T, bool PRED>
+__global__ __launch_bounds__(P::kThreads) void logits_forward(Operand x, Operand w, const void* bias, const int* lab,
+                                                              const Scalars* sc, int rows, int rows_p, int classes,
+                                                              int tiles_m, int tiles_n, int steps, float2* part, Best* best,
+                                                              float* target) {
+  extern __shared__ char smem[];
+  int tm, tn;
+  tile_of(blockIdx.x, tiles_m, tiles_n, 4, tm, tn);
+  f32x4 acc[P::FM][P::FN];
+  P::run(acc, x, w, tm * P::BM, tn * P::BN, 0, steps, (lds_bytes)smem);
+  const int row0 = tm * P::BM + P::lane_row(), col0 = tn * P::BN + P::lane_col();
+  const float ix = P::SPLIT ? sc->inv_x : 1.f, iw = P::SPLIT ? sc->inv_w : 1.f;
+  float b[P::FN][4];
+#pragma unroll
+  for (int j = 0; j < P::FN; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int col = col0 + j * 16 + r;
+      b[j][r] = (bias != nullptr && col < classes) ? load_as_float<T>(bias, col) : 0.f;
+    }
+  const int strip = tn * P::WC + uniform((int)(threadIdx.x >> 6)) % P::WC;
+#pragma unroll
+  for (int i = 0; i < P::FM; ++i) {
+    const int row = row0 + i * 16;
+    const int y = row < rows ? lab[row] : kIgnored;
+    float m = -INFINITY;
+    Best best_here = {-INFINITY, 0x7fffffff};
+#pragma unroll
+    for (int j = 0; j < P::FN; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int col = col0 + j * 16 + r;
+        const float z = col < classes ? (P::SPLIT ? acc[i][j][r] * ix * iw : acc[i][j][r]) + b[j][r] : -INFINITY;
+        acc[i][j][r] = z;
+        m = fmaxf(m, z);
+        if (col == y) target[row] = z;
+        if (PRED && col < classes && beats(z, col, best_here)) best_here = {z, col};
+      }
+    m = fmaxf(m, __shfl_xor(m, 16));
+    m = fmaxf(m, __shfl_xor(m, 32));
+    const float from = m == -INFINITY ? 0.f : m;  // a strip of classes that are all masked sums to zero
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < P::FN; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s += __expf(acc[i][j][r] - from);
+    s += __shfl_xor(s, 16);
+    s += __shfl_xor(s, 32);
+    if constexpr (PRED) {
+#pragma unroll
+      for (int d = 16; d <= 32; d <<= 1) {
+        const Best o = {__shfl_xor(best_here.v, d), __shfl_xor(best_here.at, d)};
+        if (beats(o.v, o.at, best_here)) best_here = o;
+      }
+    }
+    if (row < rows && (threadIdx.x & 48) == 0) {
+      part[(long long)strip * rows_p + row] = make_float2(m, s);
+      if constexpr (PRED) best[(long long)strip * rows_p + row] = best_here;
+    }
+  }
+}
+
+// Joins the strips of 16 rows: 16 threads a row.
+__global__ __launch_bounds__(256) void join_strips(const float2* part, const Best* best, int strips, const int* lab, int rows,
+                                                   int rows_p, const float* target, float* lse, float* losses, int64_t* pred) {
+  __shared__ float2 s[16][17];
+  __shared__ Best sb[16][17];
+  const int r = threadIdx.x & 15, p0 = threadIdx.x >> 4, row = blockIdx.x * 16 + r;
+  float m = -INFINITY, sum = 0.f;
+  Best b = {-INFINITY, 0x7fffffff};
+  if (row < rows) {
+    for (int p = p0; p < strips; p += 16) {
+      const float2 v = part[(long long)p * rows_p + row];
+      const float n = fmaxf(m, v.x), from = n == -INFINITY ? 0.f : n;
+      sum = sum * __expf(m - from) + v.y * __expf(v.x - from);
+      m = n;
+      if (best != nullptr) {
+        const Best o = best[(long long)p * rows_p + row];
+        if (beats(o.v, o.at, b)) b = o;
+      }
+    }
+  }
+  s[p0][r] = make_float2(m, sum);
+  sb[p0][r] = b;
+  __syncthreads();
+  if (p0 != 0 || row >= rows_p) return;
+  for (int p = 1; p < 16; ++p) {
+    const float2 v = s[p][r];
+    const float n = fmaxf(m, v.x), from = n == -INFINITY ? 0.f : n;
+    sum = sum * __expf(m - from) + v.y * __expf(v.x - from);
+    m = n;
+    if (best != nullptr && beats(sb[p][r].v, sb[p][r].at, b)) b = sb[p][r];
+  }
+  const int y = lab[row];
+  float l = m + logf(sum);
+  if (y == kOutside) l = NAN;
+  lse[row] = y == kIgnored ? 0.f : l;
+  if (row >= rows) return;
+  losses[row] = y == kIgnored ? 0.f : y == kOutside ? NAN : l - target[row];
+  if (pred != nullptr) pred[row] = y == kIgnored ? -1 : b.at;
+}
+
+// Sum and count of the rows; the mean divides by the count, at least 1.
+__global__ __launch_bounds__(1024) void sum_rows(const float* losses, const int* lab, int rows, int mean, float* loss,
+                                                 Scalars* sc) {
+  double sum = 0;
+  int n = 0;
+  for (int i = threadIdx.x; i < rows; i += 1024) sum += (double)losses[i], n += lab[i] != kIgnored;
+  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d), n += __shfl_xor(n, d);
+  __shared__ double ss[16];
+  __shared__ int sn[16];
+  if ((threadIdx.x & 63) == 0) ss[threadIdx.x >> 6] = sum, sn[threadIdx.x >> 6] = n;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int i = 1; i < 16; ++i) sum += ss[i], n += sn[i];
+  const float count = (float)max(n, 1);
+  sc->count = count;
+  *loss = (float)(mean ? sum / (double)max(n, 1) : sum);
+}
+
+// ---- backward ------------------------------------------------------------------------------------------------------------
+
+// What multiplies each row's q before it is rounded, and (behind the rows) what the finished sums are multiplied with.  A common gradient stays out
+// of q; gradients of single rows go into it, scaled by a power of two so that the largest of them fills the type.
+__global__ __launch_bounds__(1024) void row_factors(const float* grad, int reduction, const int* lab, int rows, int rows_p,
+                                                    float* factors, const Scalars* sc) {
+  float s = kQScale, f;
+  if (reduction == MI_REDUCTION_NONE) {
+    float m = 0.f;
+    for (int i = threadIdx.x; i < rows; i += 1024) {
+      const float v = fabsf(grad[i]);
+      if (lab[i] != kIgnored && v <= 3.402823466e38f) m = fmaxf(m, v);
+    }
+    for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    __shared__ float sm[16];
+    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
+    __syncthreads();
+    for (int i = 0; i < 16; ++i) m = fmaxf(m, sm[i]);
+    s = scale_of(m) * 0.5f;
+    f = 1.f / s;
+  } else {
+    f = (reduction == MI_REDUCTION_MEAN ? grad[0] / sc->count : grad[0]) * (1.f / kQScale);
+  }
+  for (int i = threadIdx.x; i < rows_p; i += 1024)
+    factors[i] = (i >= rows || lab[i] == kIgnored) ? 0.f : reduction == MI_REDUCTION_NONE ? grad[i] * s : s;
+  if (threadIdx.x == 0) factors[rows_p] = f;
+}
+
+// One tile of logits, again -> q times its row's factor; column sums for the bias gradient, one strip per wave row.
+template <class P, int T>
+__global__ __launch_bounds__(P::kThreads) void logits_backward(Operand x, Operand w, const void* bias, const int* lab,
+                                                               const float* lse, const float* factors, const Scalars* sc,
+                                                               int rows_p, int class0, int classes, int classes_p,
+                                                               int tiles_m, int tiles_n, int steps, uint16_t* q, float* sums) {
+  extern __shared__ char smem[];
+  int tm, tn;
+  tile_of(blockIdx.x, tiles_m, tiles_n, 4, tm, tn);
+  f32x4 acc[P::FM][P::FN];
+  P::run(acc, x, w, tm * P::BM, tn * P::BN, 0, steps, (lds_bytes)smem);
+  const int row0 = tm * P::BM + P::lane_row(), col0 = tn * P::BN + P::lane_col();
+  const float ix = P::SPLIT ? sc->inv_x : 1.f, iw = P::SPLIT ? sc->inv_w : 1.f;
+  const long long ld = (long long)classes_p * (P::SPLIT ? 2 : 1);
+  float b[P::FN][4], sum[P::FN][4];
+#pragma unroll
+  for (int j = 0; j < P::FN; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int col = col0 + j * 16 + r;
+      b[j][r] = (bias != nullptr && col < classes) ? load_as_float<T>(bias, class0 + col) : 0.f;
+      sum[j][r] = 0.f;
+    }
+#pragma unroll
+  for (int i = 0; i < P::FM; ++i) {
+    const int row = row0 + i * 16;
+    const bool in = row < rows_p;
+    const int y = in ? lab[row] : kIgnored;
+    const float l = in ? lse[row] : 0.f, f = in ? factors[row] : 0.f;
+#pragma unroll
+    for (int j = 0; j < P::FN; ++j) {
+      const int col = col0 + j * 16;
+      s16x4 hi, lo;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float z = (P::SPLIT ? acc[i][j][r] * ix * iw : acc[i][j][r]) + b[j][r];
+        float v = 0.f;
+        if (y != kIgnored && col + r < classes) v = (__expf(z - l) - (class0 + col + r == y ? 1.f : 0.f)) * f;
+        sum[j][r] += v;
+        if constexpr (P::SPLIT) {
+          const _Float16 h = (_Float16)v;
+          hi[r] = __builtin_bit_cast(short, h);
+          lo[r] = (short)half_bits(v - (float)h);
+        } else {
+          hi[r] = (short)round16<T>(v);
+        }
+      }
+      if (in && col < classes_p) {
+        if constexpr (P::SPLIT) {
+          uint16_t* at = q + row * ld + (col >> 5) * 64 + (col & 31);
+          *reinterpret_cast<s16x4*>(at) = hi;
+          *reinterpret_cast<s16x4*>(at + 32) = lo;
+        } else {
+          *reinterpret_cast<s16x4*>(q + row * ld + col) = hi;
+        }
+      }
+    }
+  }
+  if (sums == nullptr) return;
+  const int strip = tm * P::WR + uniform((int)(threadIdx.x >> 6)) / P::WC;
+#pragma unroll
+  for (int j = 0; j < P::FN; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float v = sum[j][r];
+      for (int d = 1; d < 16; d <<= 1) v += __shfl_xor(v, d);
+      const int col = col0 + j * 16 + r;
+      if ((threadIdx.x & 15) == 0 && col < classes) sums[(long long)strip * classes_p + col] = v;
+    }
+}
+
+template <int T>
+__global__ __launch_bounds__(256) void bias_gradient(const float* sums, int strips, int classes, int classes_p, const float* factor,
+                                                     void* out, int class0) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= classes) return;
+  float v = 0.f;
+  for (int s = 0; s < strips; ++s) v += sums[(long long)s * classes_p + c];
+  store_from_float<T>(out, class0 + c, v * *factor);
+}
+
+// A gradient's tile: slice blockIdx.y of the k axis.  With one slice and one piece the result goes out rounded; otherwise
+// the slices' float32 sums are kept (and added to those of the pieces before) and joined by join_slices in their order.
+template <class P, int T, bool OF_WEIGHT>
+__global__ __launch_bounds__(P::kThreads) void gradient_product(Operand a, Operand b, int rows, int cols, int tiles_m,
+                                                                int tiles_n, int steps, int per_slice, const Scalars* sc,
+                                                                const float* factor, void* out, long long out_ld,
+                                                                float* slices, int add) {
+  extern __shared__ char smem[];
+  int tm, tn;
+  tile_of(blockIdx.x, tiles_m, tiles_n, 4, tm, tn);
+  f32x4 acc[P::FM][P::FN];
+  const int step0 = blockIdx.y * per_slice, n = min(per_slice, steps - step0);
+  P::run(acc, a, b, tm * P::BM, tn * P::BN, step0, n, (lds_bytes)smem);
+  const int row0 = tm * P::BM + P::lane_row(), col0 = tn * P::BN + P::lane_col();
+  const float f = *factor * (P::SPLIT ? (OF_WEIGHT ? sc->inv_x : sc->inv_w) : 1.f);
+#pragma unroll
+  for (int i = 0; i < P::FM; ++i) {
+    const int row = row0 + i * 16;
+    if (row >= rows) continue;
+#pragma unroll
+    for (int j = 0; j < P::FN; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int col = col0 + j * 16 + r;
+        if (col >= cols) continue;
+        if (slices != nullptr) {
+          float* at = slices + ((long long)blockIdx.y * rows + row) * cols + col;
+          *at = add ? *at + acc[i][j][r] : acc[i][j][r];
+        } else {
+          store_from_float<T>(out, (long long)row * out_ld + col, acc[i][j][r] * f);
+        }
+      }
+  }
+}
+
+template <int T, bool OF_WEIGHT>
+__global__ __launch_bounds__(256) void join_slices(const float* slices, int n, long long count, const Scalars* sc,
+                                                   const float* factor, void* out) {
+  const float f = *factor * (T == MI_TYPE_F32 ? (OF_WEIGHT ? sc->inv_x : sc->inv_w) : 1.f);
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < count; i += gridDim.x * 256LL) {
+    float v = 0.f;
+    for (int s = 0; s < n; ++s) v += slices[s * count + i];
+    store_from_float<T>(out, i, v * f);
+  }
+}
+
+// ---- launching -----------------------------------------------------------------------------------------------------------
+
+// Tiles of 128 x 128 where they give every compute unit one (two fit a unit and hide each other's waits), else 64 x 64 with
+// a deeper pipeline: 1024 x 1204 x 1024 in float32 takes 20 us with the small tiles and 30 us with the large ones,
+// 8192 x 8192 x 4096 2.5 ms and 1.3 ms.
+bool large_tiles(long long m, long long n, int slices) {
+  return (long long)ceil_div(m, 128) * ceil_div(n, 128) * slices >= compute_units();
+}
+
+template <bool SPLIT, bool BF16, bool AKM, bool BKM>
+using Large = TileProduct<128, 128, 2, 2, 2, SPLIT, BF16, AKM, BKM>;
+template <bool SPLIT, bool BF16, bool AKM, bool BKM>
+using Small = TileProduct<64, 64, 2, 2, 4, SPLIT, BF16, AKM, BKM>;
+
+// Slices of a gradient's k axis: as many as give every compute unit a small tile or two, each at least 8 stages long.
+int slices_of(long long m, long long n, long long steps) {
+  const long long tiles = (long long)ceil_div(m, 64) * ceil_div(n, 64);
+  long long s = tiles >= compute_units() ? 1 : 2LL * compute_units() / tiles;
+  if (s > steps / 8) s = steps / 8;
+  return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+
+struct Pieces {
+  int n, width;  // of the vocabulary; width is a multiple of kPad
+  int x_slices, w_slices;
+  size_t q_at, sums_at, factors_at, slices_at, bytes;
+};
+
+Pieces make_pieces(const Plan& p) {
+  Pieces c;
+  const size_t words = p.split ? 2 : 1;
+  long long most = (long long)(kPieceBytes / ((size_t)p.rows_p * words * 2)) / kPad * kPad;
+  if (most < kPad) most = kPad;
+  c.n = ceil_div(p.classes, most);
+  c.width = ceil_div(ceil_div(p.classes, c.n), kPad) * kPad;
+  c.n = ceil_div(p.classes, c.width);
+  const int step = p.split ? 32 : 64;
+  c.x_slices = slices_of(p.rows, p.dim, c.width / step);
+  c.w_slices = slices_of(c.width, p.dim, p.rows_p / step);
+  size_t at = 0;
+  c.q_at = at, at = up(at + (size_t)p.rows_p * c.width * words * 2);
+  c.sums_at = at, at = up(at + (size_t)(ceil_div(p.rows_p, 64) * 2) * c.width * 4);
+  c.factors_at = at, at = up(at + (size_t)(p.rows_p + 1) * 4);
+  const size_t xs = c.n > 1 || c.x_slices > 1 ? (size_t)c.x_slices * p.rows * p.dim * 4 : 0;
+  const size_t ws = c.w_slices > 1 ? (size_t)c.w_slices * c.width * p.dim * 4 : 0;
+  c.slices_at = at, at = up(at + xs) + up(ws);
+  c.bytes = at;
+  return c;
+}
+
+struct ForwardRoom {
+  size_t parts_at, best_at, target_at, losses_at, max_at, bytes;
+};
+ForwardRoom make_room(const Plan& p, bool with_pred) {
+  ForwardRoom f;
+  const size_t strips = (size_t)ceil_div(p.classes, large_tiles(p.rows, p.classes, 1) ? 128 : 64) * 2;
+  size_t at = 0;
+  f.parts_at = at, at = up(at + strips * p.rows_p * sizeof(float2));
+  f.best_at = at, at = up(at + (with_pred ? strips * p.rows_p * sizeof(Best) : 0));
+  f.target_at = at, at = up(at + (size_t)p.rows_p * 4);
+  f.losses_at = at, at = up(at + (size_t)p.rows_p * 4);
+  f.max_at = at, at = up(at + (size_t)2 * kMaxParts * 4);
+  f.bytes = at;
+  return f;
+}
+
+template <class K>
+void allow_lds(K kernel, unsigned bytes) {
+  if (bytes > 65536)
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
+struct Call {
+  const void *x, *weight, *bias, *labels;
+  long long x_stride, w_stride, ignore;
+  int labels_64, reduction;
+  char *saved, *room;
+  hipStream_t stream;
+};
+
+uint16_t* weights_of(const Plan& p, const Call& c) {
+  return p.copy_w ? reinterpret_cast<uint16_t*>(c.saved + p.w_at)
+                  : const_cast<uint16_t*>(static_cast<const uint16_t*>(c.weight));
+}
+long long weights_ld(const Plan& p, const Call& c) { return p.copy_w ? p.ld : c.w_stride; }
+
+template <int T, class LABEL>
+void lay_out_all(const Plan& p, const Call& c, float* maxima) {
+  const LABEL* labels = static_cast<const LABEL*>(c.labels);
+  int xb = 0, wb = 0;
+  if constexpr (T == MI_TYPE_F32) {
+    xb = ceil_div(p.rows, 16), wb = ceil_div(p.classes, 16);
+    xb = xb > kMaxParts ? kMaxParts : xb, wb = wb > kMaxParts ? kMaxParts : wb;
+    largest<LABEL><<<xb + wb, 256, 0, c.stream>>>(static_cast<const float*>(c.x), c.x_stride,
+                                                  static_cast<const float*>(c.weight), c.w_stride, labels, c.ignore, p.rows,
+                                                  p.classes, p.dim, xb, maxima);
+  }
+  const int rows = p.rows_p + (p.copy_w ? p.classes : 0);
+  const int grid = ceil_div(rows, 4) < 4 * compute_units() ? ceil_div(rows, 4) : 4 * compute_units();
+  lay_out<T, LABEL><<<grid, 256, 0, c.stream>>>(
+      c.x, c.x_stride, c.weight, c.w_stride, labels, c.ignore, p.rows, p.rows_p, p.classes, p.dim, p.dim_p,
+      reinterpret_cast<uint16_t*>(c.saved + p.x_at), p.copy_w ? reinterpret_cast<uint16_t*>(c.saved + p.w_at) : nullptr,
+      reinterpret_cast<int*>(c.saved + p.lab_at), maxima, xb, wb, reinterpret_cast<Scalars*>(c.saved + p.scalars_at));
+}
+
+template <class P, int T, bool PRED>
+int launch_logits(const Plan& p, const Call& c, const ForwardRoom& f) {
+  const Operand x = {reinterpret_cast<uint16_t*>(c.saved + p.x_at), p.ld, p.rows_p, p.dim_p};
+  const Operand w = {weights_of(p, c), weights_ld(p, c), p.classes, p.dim_p};
+  const int tm = ceil_div(p.rows, P::BM), tn = ceil_div(p.classes, P::BN);
+  allow_lds(logits_forward<P, T, PRED>, P::kLds);
+  logits_forward<P, T, PRED><<<tm * tn, P::kThreads, P::kLds, c.stream>>>(
+      x, w, c.bias, reinterpret_cast<const int*>(c.saved + p.lab_at), reinterpret_cast<const Scalars*>(c.saved + p.scalars_at),
+      p.rows, p.rows_p, p.classes, tm, tn, p.dim_p / P::kStep, reinterpret_cast<float2*>(c.room + f.parts_at),
+      reinterpret_cast<Best*>(c.room + f.best_at), reinterpret_cast<float*>(c.room + f.target_at));
+  return tn * P::WC;
+}
+
+template <int T>
+int forward(const Plan& p, const Call& c, float* loss, float* losses, int64_t* pred) {
+  constexpr bool split = T == MI_TYPE_F32, bf16 = T == MI_TYPE_BF16;
+  const ForwardRoom f = make_room(p, pred != nullptr);
+  float* maxima = reinterpret_cast<float*>(c.room + f.max_at);
+  if (c.labels_64)
+    lay_out_all<T, int64_t>(p, c, maxima);
+  else
+    lay_out_all<T, int32_t>(p, c, maxima);
+  int strips;
+  if (large_tiles(p.rows, p.classes, 1))
+    strips = pred ? launch_logits<Large<split, bf16, false, false>, T, true>(p, c, f)
+                  : launch_logits<Large<split, bf16, false, false>, T, false>(p, c, f);
+  else
+    strips = pred ? launch_logits<Small<split, bf16, false, false>, T, true>(p, c, f)
+                  : launch_logits<Small<split, bf16, false, false>, T, false>(p, c, f);
+  float* per_row = losses != nullptr ? losses : reinterpret_cast<float*>(c.room + f.losses_at);
+  const int* lab = reinterpret_cast<const int*>(c.saved + p.lab_at);
+  join_strips<<<ceil_div(p.rows_p, 16), 256, 0, c.stream>>>(
+      reinterpret_cast<const float2*>(c.room + f.parts_at), pred ? reinterpret_cast<const Best*>(c.room + f.best_at) : nullptr,
+      strips, lab, p.rows, p.rows_p, reinterpret_cast<const float*>(c.room + f.target_at),
+      reinterpret_cast<float*>(c.saved + p.lse_at), per_row, pred);
+  if (c.reduction != MI_REDUCTION_NONE)
+    sum_rows<<<1, 1024, 0, c.stream>>>(per_row, lab, p.rows, c.reduction == MI_REDUCTION_MEAN, loss,
+                                     reinterpret_cast<Scalars*>(c.saved + p.scalars_at));
+  return check_launch("mi_linear_cross_entropy_forward");
+}
+
+template <class P, int T>
+int launch_q(const Plan& p, const Call& c, const Pieces& s, int class0, int classes, int classes_p, bool want_bias) {
+  const Operand x = {reinterpret_cast<uint16_t*>(c.saved + p.x_at), p.ld, p.rows_p, p.dim_p};
+  const long long ld = weights_ld(p, c);
+  const Operand w = {weights_of(p, c) + (long long)class0 * ld, ld, classes, p.dim_p};
+  const int tm = ceil_div(p.rows_p, P::BM), tn = ceil_div(classes_p, P::BN);
+  allow_lds(logits_backward<P, T>, P::kLds);
+  logits_backward<P, T><<<tm * tn, P::kThreads, P::kLds, c.stream>>>(
+      x, w, c.bias, reinterpret_cast<const int*>(c.saved + p.lab_at), reinterpret_cast<const float*>(c.saved + p.lse_at),
+      reinterpret_cast<const float*>(c.room + s.factors_at), reinterpret_cast<const Scalars*>(c.saved + p.scalars_at), p.rows_p,
+      class0, classes, classes_p, tm, tn, p.dim_p / P::kStep, reinterpret_cast<uint16_t*>(c.room + s.q_at),
+      want_bias ? reinterpret_cast<float*>(c.room + s.sums_at) : nullptr);
+  return tm * P::WR;
+}
+
+template <class P, int T, bool OF_WEIGHT>
+void launch_gradient(const Operand& a, const Operand& b, int rows, int cols, int steps, int slices, const Scalars* sc,
+                     const float* factor, void* out, long long out_ld, float* room, int add, hipStream_t stream) {
+  const int tm = ceil_div(rows, P::BM), tn = ceil_div(cols, P::BN), per = ceil_div(steps, slices);
+  allow_lds(gradient_product<P, T, OF_WEIGHT>, P::kLds);
+  gradient_product<P, T, OF_WEIGHT><<<dim3(tm * tn, slices), P::kThreads, P::kLds, stream>>>(
+      a, b, rows, cols, tm, tn, steps, per, sc, factor, out, out_ld, room, add);
+}
+
+template <int T>
+int backward(const Plan& p, const Call& c, const float* grad, void* grad_x, void* grad_w, void* grad_b) {
+  constexpr bool split = T == MI_TYPE_F32, bf16 = T == MI_TYPE_BF16;
+  constexpr int words = split ? 2 : 1, step = split ? 32 : 64, out_bytes = T == MI_TYPE_F32 ? 4 : 2;
+  const Pieces s = make_pieces(p);
+  const Scalars* sc = reinterpret_cast<const Scalars*>(c.saved + p.scalars_at);
+  float* factors = reinterpret_cast<float*>(c.room + s.factors_at);
+  const float* factor = factors + p.rows_p;
+  row_factors<<<1, 1024, 0, c.stream>>>(grad, c.reduction, reinterpret_cast<const int*>(c.saved + p.lab_at), p.rows, p.rows_p,
+                                        factors, sc);
+  const uint16_t* q = reinterpret_cast<const uint16_t*>(c.room + s.q_at);
+  const long long ldw = weights_ld(p, c);
+  const bool x_joined = s.n > 1 || s.x_slices > 1;
+  float* x_room = reinterpret_cast<float*>(c.room + s.slices_at);
+  float* w_room = reinterpret_cast<float*>(c.room + s.slices_at + (x_joined ? up((size_t)s.x_slices * p.rows * p.dim * 4) : 0));
+  for (int k = 0; k < s.n; ++k) {
+    const int class0 = k * s.width, classes = p.classes - class0 < s.width ? p.classes - class0 : s.width;
+    const int classes_p = ceil_div(classes, kPad) * kPad;
+    const int strips = large_tiles(p.rows_p, classes_p, 1)
+                           ? launch_q<Large<split, bf16, false, false>, T>(p, c, s, class0, classes, classes_p, grad_b != nullptr)
+                           : launch_q<Small<split, bf16, false, false>, T>(p, c, s, class0, classes, classes_p, grad_b != nullptr);
+    if (grad_b != nullptr)
+      bias_gradient<T><<<ceil_div(classes, 256), 256, 0, c.stream>>>(reinterpret_cast<const float*>(c.room + s.sums_at), strips,
+                                                                   classes, classes_p, factor, grad_b, class0);
+    if (grad_x != nullptr) {
+      const Operand a = {q, (long long)classes_p * words, p.rows_p, classes_p};
+      const Operand b = {weights_of(p, c) + class0 * ldw, ldw, p.dim, classes};
+      // every piece has the same slices: a last, shorter piece leaves some of them empty
+      const int steps = classes_p / step;
+      if (large_tiles(p.rows, p.dim, s.x_slices))
+        launch_gradient<Large<split, bf16, false, true>, T, false>(a, b, p.rows, p.dim, steps, s.x_slices, sc, factor, grad_x, p.dim,
+                                                                   x_joined ? x_room : nullptr, k > 0, c.stream);
+      else
+        launch_gradient<Small<split, bf16, false, true>, T, false>(a, b, p.rows, p.dim, steps, s.x_slices, sc, factor, grad_x, p.dim,
+                                                                   x_joined ? x_room : nullptr, k > 0, c.stream);
+    }
+    if (grad_w != nullptr) {
+      const Operand a = {q, (long long)classes_p * words, classes_p, p.rows_p};
+      const Operand b = {reinterpret_cast<uint16_t*>(c.saved + p.x_at), p.ld, p.dim, p.rows_p};
+      void* out = static_cast<char*>(grad_w) + (size_t)class0 * p.dim * out_bytes;
+      float* room = s.w_slices > 1 ? w_room : nullptr;
+      if (large_tiles(classes, p.dim, s.w_slices))
+        launch_gradient<Large<split, bf16, true, true>, T, true>(a, b, classes, p.dim, p.rows_p / step, s.w_slices, sc, factor, out,
+                                                                 p.dim, room, 0, c.stream);
+      else
+        launch_gradient<Small<split, bf16, true, true>, T, true>(a, b, classes, p.dim, p.rows_p / step, s.w_slices, sc, factor, out,
+                                                                 p.dim, room, 0, c.stream);
+      if (room != nullptr) {
+        const long long n = (long long)classes * p.dim;
+        join_slices<T, true><<<grid_for(n, 256), 256, 0, c.stream>>>(room, s.w_slices, n, sc, factor, out);
+      }
+    }
+  }
+  if (grad_x != nullptr && x_joined) {
+    const long long n = (long long)p.rows * p.dim;
+    join_slices<T, false><<<grid_for(n, 256), 256, 0, c.stream>>>(x_room, s.x_slices, n, sc, factor, grad_x);
+  }
+  return check_launch("mi_linear_cross_entropy_backward");
+}
+
+// 16-bit weights are multiplied where they lie if k needs no padding and their rows start on 16 bytes.
+bool in_place(const void* weight, long long stride, int dim, int dtype) {
+  return dtype != MI_TYPE_F32 && dim % kPad == 0 && stride % 8 == 0 && reinterpret_cast<uintptr_t>(weight) % 16 == 0;
+}
+
+int check_sizes(int rows, int dim, int classes, int dtype) {
+  MI_REQUIRE(rows >= 1 && rows <= (1 << 24), "linear_cross_entropy: %d rows, 1 to 2^24 are taken", rows);
+  MI_REQUIRE(dim >= 1 && dim <= (1 << 20), "linear_cross_entropy: %d features, 1 to 2^20 are taken", dim);
+  MI_REQUIRE(classes >= 1 && classes <= (1 << 24), "linear_cross_entropy: %d classes, 1 to 2^24 are taken", classes);
+  MI_REQUIRE(dtype == MI_TYPE_F32 || dtype == MI_TYPE_F16 || dtype == MI_TYPE_BF16, "linear_cross_entropy: dtype %d", dtype);
+  return MI_OK;
+}
+
+}  // namespace
+}  // namespace mi
+
+using namespace mi;
+
+extern "C" {
+
+size_t mi_linear_cross_entropy_saved_bytes(int rows, int dim, int classes, int dtype, const void* weight,
+                                           long long weight_stride) {
+  if (check_sizes(rows, dim, classes, dtype) != MI_OK) return 0;
+  return make_plan(rows, dim, classes, dtype, in_place(weight, weight_stride, dim, dtype)).saved_bytes;
+}
+
+size_t mi_linear_cross_entropy_workspace_bytes(int rows, int dim, int classes, int dtype, int pass) {
+  if (check_sizes(rows, dim, classes, dtype) != MI_OK) return 0;
+  const Plan p = make_plan(rows, dim, classes, dtype, true);
+  return pass == MI_PASS_BACKWARD ? make_pieces(p).bytes : make_room(p, pass == MI_PASS_FORWARD_PRED).bytes;
+}
+
+static int check_call(const void* x, long long x_stride, const void* weight, long long weight_stride, const void* labels, int rows,
+                      int dim, int classes, int dtype, int reduction, const void* saved, size_t saved_bytes,
+                      const void* workspace, size_t workspace_bytes, size_t needed, Plan* plan) {
+  if (const int rc = check_sizes(rows, dim, classes, dtype)) return rc;
+  MI_REQUIRE(x != nullptr && weight != nullptr && labels != nullptr && saved != nullptr && workspace != nullptr,
+             "linear_cross_entropy: null pointer");
+  MI_REQUIRE(x_stride >= dim && weight_stride >= dim && weight_stride <= (1 << 22),
+             "linear_cross_entropy: row strides %lld and %lld for %d features", x_stride, weight_stride, dim);
+  MI_REQUIRE(reduction >= MI_REDUCTION_NONE && reduction <= MI_REDUCTION_SUM, "linear_cross_entropy: reduction %d", reduction);
+  MI_REQUIRE(reinterpret_cast<uintptr_t>(saved) % 256 == 0 && reinterpret_cast<uintptr_t>(workspace) % 256 == 0,
+             "linear_cross_entropy: buffers start on 256 bytes");
+  *plan = make_plan(rows, dim, classes, dtype, in_place(weight, weight_stride, dim, dtype));
+  if (saved_bytes < plan->saved_bytes || workspace_bytes < needed) {
+    set_error("linear_cross_entropy: %zu bytes to keep and %zu of workspace are needed, %zu and %zu given", plan->saved_bytes,
+              needed, saved_bytes, workspace_bytes);
+    return MI_ERR_WORKSPACE;
+  }
+  return MI_OK;
+}
+
+int mi_linear_cross_entropy_forward(const void* x, long long x_stride, const void* weight, long long weight_stride,
+                                    const void* bias, const void* labels, int labels_64, int rows, int dim, int classes, int dtype,
+                                    long long ignore_index, int reduction, float* loss, int64_t* pred, void* saved,
+                                    size_t saved_bytes, void* workspace, size_t workspace_bytes, mi_stream_t stream) {
+  Plan p;
+  if (const int rc = check_call(x, x_stride, weight, weight_stride, labels, rows, dim, classes, dtype, reduction, saved,
+                                saved_bytes, workspace, workspace_bytes,
+                                mi_linear_cross_entropy_workspace_bytes(rows, dim, classes, dtype,
+                                                                        pred != nullptr ? MI_PASS_FORWARD_PRED : MI_PASS_FORWARD),
+                                &p))
+    return rc;
+  MI_REQUIRE(loss != nullptr, "linear_cross_entropy: null pointer");
+  begin_call();
+  const Call c = {x, weight, bias, labels, x_stride, weight_stride, ignore_index, labels_64, reduction,
+                  static_cast<char*>(saved), static_cast<char*>(workspace), as_stream(stream)};
+  float* total = reduction == MI_REDUCTION_NONE ? nullptr : loss;
+  float* each = reduction == MI_REDUCTION_NONE ? loss : nullptr;
+  if (dtype == MI_TYPE_F32) return forward<MI_TYPE_F32>(p, c, total, each, pred);
+  if (dtype == MI_TYPE_F16) return forward<MI_TYPE_F16>(p, c, total, each, pred);
+  return forward<MI_TYPE_BF16>(p, c, total, each, pred);
+}
+
+int mi_linear_cross_entropy_backward(const float* grad_loss, const void* weight, long long weight_stride, const void* bias,
+                                     int rows, int dim, int classes, int dtype, int reduction, void* grad_x, void* grad_weight,
+                                     void* grad_bias, void* saved, size_t saved_bytes, void* workspace, size_t workspace_bytes,
+                                     mi_stream_t stream) {
+  Plan p;
+  if (const int rc = check_call(saved, dim, weight, weight_stride, saved, rows, dim, classes, dtype, reduction, saved, saved_bytes,
+                                workspace, workspace_bytes,
+                                mi_linear_cross_entropy_workspace_bytes(rows, dim, classes, dtype, MI_PASS_BACKWARD), &p))
+    return rc;
+  MI_REQUIRE(grad_loss != nullptr, "linear_cross_entropy: null pointer");
+  begin_call();
+  const Call c = {nullptr, weight, bias, nullptr, dim, weight_stride, 0, 0, reduction,
+                  static_cast<char*>(saved), static_cast<char*>(workspace), as_stream(stream)};
+  if (dtype == MI_TYPE_F32) return backward<MI_TYPE_F32>(p, c, grad_loss, grad_x, grad_weight, grad_bias);
+  if (dtype == MI_TYPE_F16) return backward<MI_TYPE_F16>(p, c, grad_loss, grad_x, grad_weight, grad_bias);
+  return backward<MI_TYPE_BF16>(p, c, grad_loss, grad_x, grad_weight, grad_bias);
+}
+
+}  // extern "C"

@@ -1,0 +1,126 @@
+"""Optimiser with momentum and orthogonalised updates for weight matrices -- host side of mi_muon_step.
+
+    muon_step_(params, grads, momenta, lr=...)   one step of a list of matrices, in place
+    Muon(params, lr=...)                         the torch.optim.Optimizer around it (rcnn.train.make_optimizer: SOLVER.TYPE)
+
+Per matrix:  M <- mu M + G,  U = G + mu M (nesterov) or M,
+             W <- (1 - lr weight_decay) W - lr sqrt(max(1, rows / cols)) orthogonalize(U).
+A convolution's weight [out, in, kh, kw] is the matrix [out, in kh kw].  What is no matrix (biases) takes the momentum SGD step
+of torch.optim.SGD, with its own learning rate.
+"""
+import ctypes
+
+import torch
+
+from . import _lib
+from .orthogonalize import COEFFICIENTS, EPS, STEPS, check_matrices, host_arrays, pointers, workspace_for
+
+
+@torch.no_grad()
+def muon_step_(params, grads, momenta, lr, momentum=0.95, weight_decay=0.0, nesterov=True, steps=STEPS,
+               coefficients=COEFFICIENTS, eps=EPS):
+    """One step of contiguous matrices `params` (float32, float16 or bfloat16) with `grads` of their type and shapes and
+    float32 `momenta`, which are updated too.  Asynchronous on the current stream; capturable (the numbers are the
+    captured ones)."""
+    params, grads, momenta = list(params), list(grads), list(momenta)
+    if not len(params) == len(grads) == len(momenta):
+        raise ValueError("muon_step_ takes as many gradients and momenta as parameters")
+    if not params:
+        return
+    dev, dtype = check_matrices(params, "params")
+    for p, g, m in zip(params, grads, momenta):
+        _lib.require_cuda(g, "grads")
+        _lib.require_cuda(m, "momenta")
+        if g.shape != p.shape or m.shape != p.shape or g.dtype != p.dtype or m.dtype != torch.float32:
+            raise ValueError("a gradient has its parameter's shape and type, a momentum its shape in float32")
+        if g.device != dev or m.device != dev:
+            raise ValueError("muon_step_ takes tensors on one device")
+        if not (p.is_contiguous() and m.is_contiguous()):
+            raise ValueError("parameters and momenta are updated in place: they must be contiguous")
+    written = [t.data_ptr() for t in params + momenta if t.numel()]
+    if len(set(written)) != len(written):
+        raise ValueError("a parameter or momentum appears twice")
+    full = [(p, g.contiguous(), m) for p, g, m in zip(params, grads, momenta) if p.numel()]
+    if not full:
+        return
+    ps, gs, ms = zip(*full)
+    count, rows, cols = host_arrays(ps)
+    with torch.cuda.device(dev):
+        workspace = workspace_for(count, rows, cols, dev)
+        rc = _lib.lib().mi_muon_step(count, pointers(ps), pointers(gs), pointers(ms), rows, cols, dtype, float(lr),
+                                     float(momentum), int(nesterov), float(weight_decay), int(steps),
+                                     (ctypes.c_float * 3)(*coefficients), float(eps), workspace.data_ptr(), workspace.numel(),
+                                     _lib.current_stream_handle(dev))
+    _lib.check(rc, "mi_muon_step")
+
+
+def as_matrix(t):
+    """A dense parameter of two or more dimensions as a contiguous matrix [out, rest] over the same memory, None for other
+    layouts.  A channels-last weight is the matrix with its columns in memory order: orthogonalisation does not depend on the
+    order of columns."""
+    if t.is_contiguous():
+        return t.view(t.size(0), -1)
+    if t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last):
+        return t.permute(0, 2, 3, 1).reshape(t.size(0), -1)
+    return None
+
+
+class Muon(torch.optim.Optimizer):
+    """Parameters of two or more dimensions take the orthogonalised step with `lr`, the others momentum SGD with `sgd_lr`
+    (lr when None) and `sgd_momentum`.  Per group as usual: {"params": ..., "lr": ..., "sgd_lr": ..., "weight_decay": ...};
+    "orthogonalize": False keeps a group's matrices on SGD too."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, sgd_lr=None, sgd_momentum=0.9,
+                 steps=STEPS, coefficients=COEFFICIENTS, eps=EPS, orthogonalize=True):
+        if lr < 0 or (sgd_lr is not None and sgd_lr < 0) or weight_decay < 0 or not 0 <= momentum < 1 or not 0 <= sgd_momentum < 1:
+            raise ValueError("learning rates and weight decay are at least 0, momenta in [0, 1)")
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, sgd_lr=sgd_lr,
+                                      sgd_momentum=sgd_momentum, steps=steps, coefficients=tuple(coefficients), eps=eps,
+                                      orthogonalize=orthogonalize))
+
+    def _momentum(self, p):
+        state = self.state[p]
+        if "momentum_buffer" not in state:
+            state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+        return state["momentum_buffer"]
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            by_kind = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise ValueError("Muon does not take sparse gradients")
+                if group["orthogonalize"] and p.dim() >= 2:
+                    m = as_matrix(p)
+                    if m is None:
+                        raise ValueError("Muon updates dense parameters (contiguous or channels-last), got strides %s"
+                                         % (p.stride(),))
+                    buf = self._momentum(p)
+                    grad = p.grad if p.grad.stride() == p.stride() else torch.empty_like(p).copy_(p.grad)
+                    mats = by_kind.setdefault((p.device, p.dtype), ([], [], []))
+                    for to, t in zip(mats, (p, grad, buf)):
+                        to.append(as_matrix(t))
+                else:
+                    self._sgd(p, group)
+            for params, grads, momenta in by_kind.values():
+                muon_step_(params, grads, momenta, lr=group["lr"], momentum=group["momentum"],
+                           weight_decay=group["weight_decay"], nesterov=group["nesterov"], steps=group["steps"],
+                           coefficients=group["coefficients"], eps=group["eps"])
+        return loss
+
+    def _sgd(self, p, group):
+        """torch.optim.SGD's momentum step (coupled weight decay, no dampening)."""
+        lr = group["lr"] if group["sgd_lr"] is None else group["sgd_lr"]
+        buf = self._momentum(p)
+        g = p.grad.float()
+        if group["weight_decay"]:
+            g = g + group["weight_decay"] * p.float()
+        buf.mul_(group["sgd_momentum"]).add_(g)
+        p.sub_((lr * buf).to(p.dtype))

@@ -49,8 +49,9 @@ extern "C" {
  * overwrites, no atomics).  8 (round 6): no new entry point -- a forward whose workspace has no room for a backward (smaller
  * than mi_roi_align_backward_workspace_bytes), and the forward without a workspace, run the records-free NCHW kernel
  * (roi_align_fwd_slab: ONE launch, nothing written to the workspace); mi_roi_align_forward_writes_records speaks of a
- * backward-sized workspace. */
-#define MI_ABI_VERSION 8
+ * backward-sized workspace.  9: mi_linear_cross_entropy_*,
+ * mi_orthogonalize, mi_muon_step. */
+#define MI_ABI_VERSION 9
 
 typedef void* mi_stream_t; /* hipStream_t */
 
@@ -61,6 +62,11 @@ enum mi_status {
   MI_ERR_WORKSPACE = 3,     /* workspace smaller than mi_*_workspace_bytes()            */
   MI_ERR_UNSUPPORTED = 4    /* shape outside what the kernels implement (see message)  */
 };
+
+enum mi_type { MI_TYPE_F32 = 0, MI_TYPE_F16 = 1, MI_TYPE_BF16 = 2 };
+enum mi_reduction { MI_REDUCTION_NONE = 0, MI_REDUCTION_MEAN = 1, MI_REDUCTION_SUM = 2 };
+/* whose workspace is asked for: a forward, a forward that also writes the predicted classes, a backward */
+enum mi_pass { MI_PASS_FORWARD = 0, MI_PASS_FORWARD_PRED = 1, MI_PASS_BACKWARD = 2 };
 
 enum mi_layout { MI_LAYOUT_NCHW = 0, MI_LAYOUT_NHWC = 1 };
 
@@ -479,6 +485,51 @@ int mi_keypoint_decode(const float* heatmaps, const float* rois, int num_rois, i
  * visiting order, *num_keep their number.  num_keypoints must be 17 (the reference's sigma table), num_rois <= 512. */
 int mi_keypoint_nms_oks(const float* xy_preds, const float* rois, int num_rois, int num_keypoints, double thresh,
                         int64_t* keep, int32_t* num_keep, mi_stream_t stream);
+
+/* ---- softmax cross entropy of a linear classifier, without keeping its logits (no reference counterpart) ------------
+ * z = x weight^T + bias over [rows, dim] x [classes, dim], loss_i = log sum_v exp z_iv - z_i,labels_i: what
+ * fast_rcnn_heads.py:39,57 computes as nn.Linear and F.cross_entropy with [rows, classes] logits in memory.  The logits are formed
+ * tile by tile, twice (forward, backward), and never stored; the backward works in pieces of the vocabulary.
+ *   dtype         of x, weight, bias and their gradients: MI_TYPE_*.  float32 products carry 22 bits and accumulate in float32.
+ *   x, weight     rows of `dim` contiguous elements, `x_stride` / `weight_stride` elements apart; bias [classes] or NULL
+ *   labels        [rows] int32 or int64 (labels_64 != 0).  Rows whose label is ignore_index count nowhere, whatever x holds
+ *                 there; a label that is no class either makes the row's loss and gradients NaN
+ *   reduction     MI_REDUCTION_MEAN over the rows that count (0 when none does), _SUM: loss float32 [1]; _NONE: [rows], 0 for
+ *                 ignored rows
+ *   pred          int64 [rows] or NULL: the lowest class of the largest logit, -1 for ignored rows; a NaN logit is the largest
+ *   saved         kept by the caller from the forward to the backward; nothing but the forward writes it, so
+ *                 several backward passes may follow, each with a workspace of its own
+ * The backward takes grad_loss float32 ([1], or [rows] for MI_REDUCTION_NONE) and writes dense gradients [rows, dim],
+ * [classes, dim], [classes]; each of the three may be NULL.  `weight` must be the forward's, unchanged.  Results do not depend on the
+ * order of execution (no atomics).  `saved` and `workspace` start on 256 bytes. */
+size_t mi_linear_cross_entropy_saved_bytes(int rows, int dim, int classes, int dtype, const void* weight,
+                                           long long weight_stride);
+size_t mi_linear_cross_entropy_workspace_bytes(int rows, int dim, int classes, int dtype, int pass);
+int mi_linear_cross_entropy_forward(const void* x, long long x_stride, const void* weight, long long weight_stride,
+                                    const void* bias, const void* labels, int labels_64, int rows, int dim, int classes, int dtype,
+                                    long long ignore_index, int reduction, float* loss, int64_t* pred, void* saved,
+                                    size_t saved_bytes, void* workspace, size_t workspace_bytes, mi_stream_t stream);
+int mi_linear_cross_entropy_backward(const float* grad_loss, const void* weight, long long weight_stride, const void* bias,
+                                     int rows, int dim, int classes, int dtype, int reduction, void* grad_x, void* grad_weight,
+                                     void* grad_bias, void* saved, size_t saved_bytes, void* workspace, size_t workspace_bytes,
+                                     mi_stream_t stream);
+
+/* ---- orthogonalised updates of weight matrices (no reference counterpart) -------------------------------------------
+ * mi_orthogonalize: Newton-Schulz iteration.  For each matrix G (turned when it has more rows than columns)
+ *   X = G / max(|G|_F, eps);   `steps` times  A = X X^T, X = a X + (b A + c A A) X   with coefficients = (a, b, c)
+ * dense row-major matrices of one dtype (MI_TYPE_*); `in`, `out`, rows, cols and coefficients are HOST arrays, out[i] may be
+ * in[i].  Products carry 22 bits and accumulate in float32.  All matrices go through the stages together.
+ * Coefficients that let the iteration leave [-15, 15] from |X| <= 1 are refused (MI_ERR_UNSUPPORTED).
+ * mi_muon_step: the optimiser step around it, per matrix (momenta float32, params and grads of `dtype`):
+ *   M = momentum M + G;  U = G + momentum M (nesterov) or M;
+ *   W = (1 - lr weight_decay) W - lr sqrt(max(1, rows / cols)) orthogonalize(U)
+ * The same matrix may not appear twice.  The workspace starts on 256 bytes. */
+size_t mi_orthogonalize_workspace_bytes(int count, const int* rows, const int* cols);
+int mi_orthogonalize(int count, const void* const* in, void* const* out, const int* rows, const int* cols, int dtype, int steps,
+                     const float* coefficients, float eps, void* workspace, size_t workspace_bytes, mi_stream_t stream);
+int mi_muon_step(int count, void* const* params, const void* const* grads, float* const* momenta, const int* rows, const int* cols,
+                 int dtype, float lr, float momentum, int nesterov, float weight_decay, int steps, const float* coefficients,
+                 float eps, void* workspace, size_t workspace_bytes, mi_stream_t stream);
 
 /* ---- diagnostics (no reference counterpart) ---------------------------------------------------
  * Tuning aid used by tools/timeline_records.py / timeline_nhwc.py / timeline_bwd.py: while a non-NULL device buffer of 8 int64 per forward workgroup is set,

@@ -1,0 +1,361 @@
+"""The classifier's loss in pieces of the vocabulary against the formulas in 64 bits, element by element.
+
+Tolerances count roundings.  u is half a step of the type (bf16 2^-8, fp16 2^-11, fp32 2^-24).  n float32 additions are off by at
+most 8 sqrt(n) 2^-24 of the sum of magnitudes (a random walk, eight standard deviations).  A float32 product carries 22 bits of
+each factor (2^-20 of it in all) and 2^-39 of the tensor's largest value below that.  exp(t) is off by (2 + |t|) 2^-21.
+"""
+import numpy as np
+import pytest
+import torch
+
+from detectron_pytorch_amd.linear_cross_entropy import linear_cross_entropy
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+FLOOR = {torch.float32: 2.0 ** -126, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -126}   # smallest steps of the type
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def formulas(x, weight, bias, labels, ignore_index=-1, reduction="mean", grad=None):
+    """loss, pred, (dx, dw, db) in float64 and the bounds of their errors, as (value, bound) pairs."""
+    u, dtype = HALF_STEP[x.dtype], x.dtype
+    keep = labels.long() != ignore_index
+    x = torch.where(keep[:, None], x.detach().double(), 0.0)
+    w = weight.detach().double()
+    b = torch.zeros(w.size(0), dtype=torch.float64, device=w.device) if bias is None else bias.detach().double()
+    (rows, dim), classes = x.shape, w.size(0)
+    y = labels.long().clamp(0, classes - 1)
+    z = x @ w.t() + b
+    size = x.abs() @ w.abs().t() + torch.where(torch.isfinite(b), b.abs(), 0.0)
+    ez = (8 * dim ** 0.5 + 4) * 2.0 ** -24 * size
+    if dtype == torch.float32:
+        ez = ez + 2.0 ** -20 * size + dim * 2.0 ** -38 * x.abs().max() * w.abs().max()
+    ez = ez.max(dim=1, keepdim=True)[0]
+    lse = torch.logsumexp(z, dim=1, keepdim=True)
+    t = z - lse
+    p = t.exp()
+    rel = 2 * ez + (2 + t.abs().clamp_max(104.0)) * 2.0 ** -21 + 8 * (32 + classes / 64) ** 0.5 * 2.0 ** -24
+    zy = z.gather(1, y[:, None])
+    losses = torch.where(keep, (lse - zy)[:, 0], 0.0)
+    e_losses = torch.where(keep, (2 * ez + rel.min(dim=1, keepdim=True)[0] + 2.0 ** -22 * (lse.abs() + zy.abs() + 1))[:, 0], 0.0)
+    n = max(1, int(keep.sum()))
+    pred = torch.where(keep, z.argmax(dim=1), -1)
+    if reduction == "none":
+        loss, e_loss, g = losses, e_losses, grad.double()
+    else:
+        k = 1.0 / n if reduction == "mean" else 1.0
+        loss, e_loss = losses.sum() * k, e_losses.sum() * k + 2.0 ** -23 * (losses.sum() * k).abs()
+        g = torch.full((rows,), k * (1.0 if grad is None else float(grad)), dtype=torch.float64, device=x.device)
+    g = torch.where(keep, g, 0.0)[:, None]
+    q = (p - torch.nn.functional.one_hot(y, classes)) * g
+    u_q = 2.0 ** -21 if dtype == torch.float32 else u
+    eq = g.abs() * (p * rel + 2.0 ** -23) + (u_q + 2.0 ** -22) * q.abs() + 2.0 ** -38 * g.abs().max()
+    eq = torch.where(keep[:, None], eq, 0.0)
+    carried = 2.0 ** -20 if dtype == torch.float32 else 0.0
+
+    def product(a, ea, c, terms):
+        v = a @ c
+        mag = a.abs() @ c.abs()
+        small = 2.0 ** -38 * c.abs().max() * a.abs().sum(dim=1, keepdim=True) if dtype == torch.float32 else 0.0
+        return v, ea @ c.abs() + (8 * terms ** 0.5 * 2.0 ** -24 + carried) * mag + small + 1.01 * u * v.abs() + FLOOR[dtype]
+
+    db, e_db = q.sum(dim=0), eq.sum(dim=0) + 8 * rows ** 0.5 * 2.0 ** -24 * q.abs().sum(dim=0)
+    db = (db, e_db + 1.01 * u * db.abs() + FLOOR[dtype])
+    return (loss, e_loss), pred, product(q, eq, w, classes), product(q.t(), eq.t(), x, rows), db, keep
+
+
+def close(got, want, what):
+    value, bound = want
+    assert torch.isfinite(got).all(), what
+    off = (got.double() - value).abs()
+    assert bool((off <= bound).all()), "%s: off by %.3g where %.3g is allowed" % (
+        what, float((off - bound).max() + bound.flatten()[(off - bound).argmax()]), float(bound.flatten()[(off - bound).argmax()]))
+
+
+def make(rows, dim, classes, dtype, seed=0, ignored=0.2, bias=True, labels=torch.int64, ignore_index=-1):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed + rows * 7 + dim * 3 + classes)
+    x = torch.randn(rows, dim, generator=g, device=DEV).to(dtype).requires_grad_(True)
+    w = (2 * torch.randn(classes, dim, generator=g, device=DEV) / dim ** 0.5).to(dtype).requires_grad_(True)
+    b = torch.randn(classes, generator=g, device=DEV).to(dtype).requires_grad_(True) if bias else None
+    y = torch.randint(0, classes, (rows,), generator=g, device=DEV)
+    y = torch.where(torch.rand(rows, generator=g, device=DEV) < ignored, ignore_index, y).to(labels)
+    return x, w, b, y
+
+
+def check(x, w, b, y, ignore_index=-1, reduction="mean", grad=None):
+    want = formulas(x, w, b, y, ignore_index, reduction, grad)
+    loss, pred = linear_cross_entropy(x, w, b, y, ignore_index=ignore_index, reduction=reduction, with_pred=True)
+    leaves = [x, w] + ([b] if b is not None else [])
+    got = torch.autograd.grad(loss, leaves, grad)
+    assert loss.dtype == torch.float32 and [t.dtype for t in got] == [t.dtype for t in leaves]
+    close(loss, want[0], "loss")
+    assert torch.equal(pred, want[1])
+    for t, v, name in zip(got, want[2:5], ("dx", "dw", "db")):
+        close(t, v, name)
+    assert bool((got[0][~want[5]] == 0).all()), "an ignored row has a gradient"
+    assert torch.equal(linear_cross_entropy(x, w, b, y, ignore_index=ignore_index, reduction=reduction), loss)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim,classes", [(1, 1, 1), (1, 1, 2), (1, 64, 81), (2, 3, 5), (63, 65, 64), (64, 64, 129),
+                                              (65, 128, 257), (300, 200, 130), (513, 77, 1204), (1024, 256, 81)])
+def test_against_the_formulas(rows, dim, classes, dtype):
+    check(*make(rows, dim, classes, dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim,classes", [(2500, 96, 3001), (129, 64, 40001), (9000, 40, 600)])
+def test_large_tiles_and_slices(rows, dim, classes, dtype):
+    check(*make(rows, dim, classes, dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("reduction", ["none", "sum"])
+def test_reductions(reduction, dtype):
+    x, w, b, y = make(130, 72, 300, dtype)
+    grad = None
+    if reduction == "none":   # gradients of very different rows, one of them zero
+        grad = torch.randn(130, device=DEV) * torch.logspace(-6, 3, 130, device=DEV)
+        grad[7] = 0.0
+    check(x, w, b, y, reduction=reduction, grad=grad)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_without_bias_and_with_32_bit_labels(dtype):
+    check(*make(70, 33, 90, dtype, bias=False, labels=torch.int32))
+
+
+@pytest.mark.parametrize("ignore_index", [0, 17, -100, 10 ** 12])
+def test_other_ignored_labels(ignore_index):
+    check(*make(70, 64, 90, torch.float32, ignore_index=ignore_index), ignore_index=ignore_index)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_vocabulary_in_several_pieces(dtype):
+    # 16384 rows x 10000 classes are more than one piece's workspace in every type
+    check(*make(16384, 64, 10000, dtype, ignored=0.05))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides_and_alignment(dtype):
+    x, w, b, y = make(100, 64, 150, dtype)
+    wide_x = torch.randn(100, 200, device=DEV).to(dtype)
+    wide_w = torch.randn(150, 201, device=DEV).to(dtype)
+    for x_at, w_at in ((0, 0), (3, 1), (8, 16)):
+        wide_x[:, x_at:x_at + 64], wide_w[:, w_at:w_at + 64] = x.detach(), w.detach()
+        xs = wide_x[:, x_at:x_at + 64].requires_grad_(True)
+        ws = wide_w[:, w_at:w_at + 64].requires_grad_(True)
+        check(xs, ws, b, y)
+        wide_x, wide_w = wide_x.detach().clone(), wide_w.detach().clone()
+    even = torch.randn(150, 208, device=DEV).to(dtype)        # rows that start on 16 bytes: multiplied in place
+    even[:, 8:72] = w.detach()
+    check(x, even[:, 8:72].requires_grad_(True), b, y)
+    check(x.detach().t().contiguous().t().requires_grad_(True), w.detach().t().contiguous().t().requires_grad_(True), b, y)
+    check(x[:1].detach().expand(100, 64).requires_grad_(True), w, b, y)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_ignored_rows_may_hold_anything(dtype):
+    x, w, b, y = make(90, 64, 70, dtype, ignored=0.4)
+    loss = linear_cross_entropy(x, w, b, y)
+    want = torch.autograd.grad(loss, (x, w, b))
+    bad = x.detach().clone()
+    rows = torch.nonzero(y == -1)[:, 0]
+    bad[rows[0::3]], bad[rows[1::3]] = float("nan"), float("inf")
+    bad[rows[2::3]] = torch.finfo(dtype).max
+    bad.requires_grad_(True)
+    got_loss, pred = linear_cross_entropy(bad, w, b, y, with_pred=True)
+    got = torch.autograd.grad(got_loss, (bad, w, b))
+    assert torch.equal(got_loss, loss) and bool((pred[rows] == -1).all())
+    for a, c in zip(got, want):
+        assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_no_row_counts(dtype):
+    x, w, b, y = make(70, 64, 50, dtype, ignored=2.0)
+    for reduction in ("mean", "sum", "none"):
+        loss, pred = linear_cross_entropy(x, w, b, y, reduction=reduction, with_pred=True)
+        grads = torch.autograd.grad(loss.sum(), (x, w, b))
+        assert bool((loss == 0).all()) and bool((pred == -1).all()) and all(bool((t == 0).all()) for t in grads)
+
+
+def test_no_rows():
+    w = torch.randn(5, 8, device=DEV, requires_grad=True)
+    x = torch.empty(0, 8, device=DEV, requires_grad=True)
+    y = torch.empty(0, dtype=torch.int64, device=DEV)
+    loss, pred = linear_cross_entropy(x, w, None, y, with_pred=True)
+    gx, gw = torch.autograd.grad(loss, (x, w))
+    assert float(loss) == 0 and pred.shape == (0,) and gx.shape == (0, 8) and bool((gw == 0).all())
+    assert linear_cross_entropy(x, w, None, y, reduction="none").shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_masked_classes(dtype):
+    """Classes whose bias is -inf or the type's lowest value take no part; a row's own class stays open."""
+    x, w, b, y = make(80, 64, 700, dtype, ignored=0.0)
+    masked = torch.arange(700, device=DEV) >= 10        # all of several tiles
+    y = y % 10
+    open_rows = linear_cross_entropy(x, w[:10], b[:10], y)
+    want = torch.autograd.grad(open_rows, (x, w, b))
+    for value in (float("-inf"), torch.finfo(dtype).min):
+        m = torch.where(masked, torch.full_like(b, value), b).detach().requires_grad_(True)
+        loss, pred = linear_cross_entropy(x, w, m, y, with_pred=True)
+        got = torch.autograd.grad(loss, (x, w, m))
+        assert int(pred.max()) < 10
+        assert abs(float(loss) - float(open_rows)) <= 2.0 ** -21 * (1 + abs(float(open_rows)))
+        u = 4 * HALF_STEP[dtype] + 2.0 ** -19
+        for a, c in zip(got, want):
+            assert torch.isfinite(a).all()
+            assert float((a.double() - c.double()).abs().max()) <= u * float(c.double().abs().max())
+        assert bool((got[1][10:] == 0).all()) and bool((got[2][10:] == 0).all())
+
+
+def test_not_a_number_and_infinity_reach_the_loss():
+    for value in (float("nan"), float("inf")):
+        for dtype in TYPES:
+            x, w, b, y = make(70, 64, 90, dtype, ignored=0.0)
+            x = x.detach().clone()
+            x[3, 5] = value
+            losses, pred = linear_cross_entropy(x, w, b, y, reduction="none", with_pred=True)
+            good = torch.ones(70, dtype=torch.bool, device=DEV)
+            good[3] = False
+            assert bool(torch.isnan(losses[3])) and bool(torch.isfinite(losses[good]).all())
+            assert bool(((pred >= 0) & (pred < 90)).all())
+            assert bool(torch.isnan(linear_cross_entropy(x, w, b, y)))
+
+
+def test_a_label_that_is_no_class_is_loud():
+    x, w, b, y = make(70, 64, 90, torch.float32, ignored=0.0)
+    for bad in (90, -2, 2 ** 40):
+        z = y.clone()
+        z[11] = bad
+        losses = linear_cross_entropy(x, w, b, z, reduction="none")
+        assert bool(torch.isnan(losses[11])) and int(torch.isnan(losses).sum()) == 1
+        loss = linear_cross_entropy(x, w, b, z)
+        gx, gw = torch.autograd.grad(loss, (x, w))
+        assert bool(torch.isnan(loss)) and bool(torch.isnan(gx[11]).all()) and bool(torch.isnan(gw).any())
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-6, 1e6])
+def test_float32_of_any_scale(scale):
+    x, w, b, y = make(130, 70, 200, torch.float32)
+    x = (x.detach() * scale).requires_grad_(True)
+    w = (w.detach() / scale).requires_grad_(True)
+    check(x, w, b, y)
+
+
+def test_float32_rows_of_different_scales():
+    x, w, b, y = make(130, 70, 200, torch.float32)
+    x = (x.detach() * torch.logspace(0, -6, 130, device=DEV)[:, None]).requires_grad_(True)
+    check(x, w, b, y)
+
+
+def test_lowest_class_of_equal_logits():
+    for dtype in TYPES:
+        x, w, _, y = make(50, 64, 1000, dtype, ignored=0.0)
+        w = w.detach()
+        w[700:] = w[:300]                                  # every logit of the first 300 classes comes twice
+        for best in (5, 299):
+            x = w[best].expand(50, 64).contiguous() * 4
+            _, pred = linear_cross_entropy(x, w, None, y, with_pred=True)
+            z = (x.double() @ w.double().t())
+            assert torch.equal(pred, torch.where(z == z.max(dim=1, keepdim=True)[0], torch.arange(1000, device=DEV), 1000).min(dim=1)[0])
+
+
+@pytest.mark.parametrize("wanted", [(True, False, False), (False, True, False), (False, False, True), (True, False, True)])
+def test_only_some_gradients(wanted):
+    leaves = make(70, 64, 90, torch.bfloat16)
+    full = torch.autograd.grad(linear_cross_entropy(*leaves), leaves[:3])
+    some = [t.detach().requires_grad_(f) for t, f in zip(leaves[:3], wanted)]
+    got = torch.autograd.grad(linear_cross_entropy(*some, leaves[3]), [t for t, f in zip(some, wanted) if f])
+    for a, c in zip(got, [t for t, f in zip(full, wanted) if f]):
+        assert torch.equal(a, c)
+
+
+def test_gradients_against_differences():
+    """Central differences of the float32 loss along random directions.  With |t''| <= 2 of the curvature the difference is off by
+    h^2 and by 2 e / h of the loss' own rounding e."""
+    x, w, b, y = make(40, 16, 30, torch.float32)
+    grads = torch.autograd.grad(linear_cross_entropy(x, w, b, y), (x, w, b))
+    h, e = 2.0 ** -6, 2.0 ** -20
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(3)
+    for k in range(3):
+        d = torch.randn(grads[k].shape, generator=gen, device=DEV)
+        d = d / d.norm()
+
+        def at(step):
+            leaves = [t.detach() for t in (x, w, b)]
+            leaves[k] = leaves[k] + step * d
+            return float(linear_cross_entropy(*leaves, y))
+
+        slope = (at(h) - at(-h)) / (2 * h)
+        assert abs(slope - float((grads[k] * d).sum())) <= 4 * h * h + 2 * e * 8 / h
+
+
+def test_backward_twice_and_results_do_not_change():
+    leaves = make(1500, 64, 2000, torch.float32)
+    loss = linear_cross_entropy(*leaves)
+    first = torch.autograd.grad(loss, leaves[:3], retain_graph=True)
+    second = torch.autograd.grad(loss, leaves[:3], grad_outputs=torch.tensor(2.0, device=DEV), retain_graph=True)
+    third = torch.autograd.grad(loss, leaves[:3])
+    for a, c, t in zip(first, second, third):
+        assert torch.equal(a, t) and torch.equal(2 * a, c)
+
+
+def test_second_derivatives_are_refused():
+    x, w, b, y = make(10, 8, 9, torch.float32)
+    (gx,) = torch.autograd.grad(linear_cross_entropy(x, w, b, y), (x,), create_graph=True)
+    with pytest.raises(RuntimeError):
+        gx.sum().backward()
+
+
+def test_on_another_stream():
+    leaves = make(300, 64, 900, torch.bfloat16)
+    want = torch.autograd.grad(linear_cross_entropy(*leaves), leaves[:3])
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = torch.autograd.grad(linear_cross_entropy(*leaves), leaves[:3])
+    torch.cuda.current_stream().wait_stream(stream)
+    for a, c in zip(got, want):
+        assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_captured_and_replayed(dtype):
+    """Forward and backward in one graph; every replay with new inputs equals the eager call on them."""
+    cases = [make(200, 64, 300, dtype, seed=s) for s in range(4)]
+    held = [t.detach().clone().requires_grad_(t.is_floating_point()) for t in cases[0]]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        torch.autograd.grad(linear_cross_entropy(*held), held[:3])
+    torch.cuda.current_stream().wait_stream(stream)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = linear_cross_entropy(*held)
+        grads = torch.autograd.grad(loss, held[:3])
+    for case in cases:
+        with torch.no_grad():
+            for to, t in zip(held, case):
+                to.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = linear_cross_entropy(*case)
+        want = torch.autograd.grad(eager, case[:3])
+        assert torch.equal(loss.detach(), eager.detach())
+        for a, c in zip(grads, want):
+            assert torch.equal(a, c)
+
+
+def test_inputs_are_left_alone():
+    leaves = make(70, 65, 90, torch.float16)
+    before = [t.detach().clone() for t in leaves]
+    torch.autograd.grad(linear_cross_entropy(*leaves), leaves[:3])
+    for a, c in zip(leaves, before):
+        assert torch.equal(a.detach(), c)
