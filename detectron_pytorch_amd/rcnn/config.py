@@ -46,11 +46,17 @@ def _defaults():
         FASTER_RCNN=False, MASK_ON=False, KEYPOINTS_ON=False, RPN_ONLY=False, SHARE_RES5=False,
         LOAD_IMAGENET_PRETRAINED_WEIGHTS=False)
     c.SOLVER = Node(                                          # config.py:520-610
-        BASE_LR=0.001, MOMENTUM=0.9, WEIGHT_DECAY=0.0005, WEIGHT_DECAY_GN=0.0, BIAS_DOUBLE_LR=True,
-        BIAS_WEIGHT_DECAY=False)
+        TYPE="SGD", BASE_LR=0.001, MOMENTUM=0.9, WEIGHT_DECAY=0.0005, WEIGHT_DECAY_GN=0.0, BIAS_DOUBLE_LR=True,
+        BIAS_WEIGHT_DECAY=False,
+        # TYPE "MUON" (not the reference's): weights of two or more dimensions take orthogonalised updates with this rate and
+        # momentum (muon.Muon), biases the SGD step with BASE_LR and MOMENTUM
+        MUON=Node(LR=0.02, MOMENTUM=0.95, NESTEROV=True, STEPS=5))
     c.FAST_RCNN = Node(                                       # config.py:615-650
         ROI_BOX_HEAD="", MLP_HEAD_DIM=1024, ROI_XFORM_METHOD="RoIPoolF", ROI_XFORM_SAMPLING_RATIO=0,
-        ROI_XFORM_RESOLUTION=14)
+        ROI_XFORM_RESOLUTION=14,
+        # not the reference's: the classification loss without its [rows, classes] logits (linear_cross_entropy), for long
+        # lists of classes
+        CLS_LOSS_IN_PIECES=False)
     c.RPN = Node(RPN_ON=False, CLS_ACTIVATION="sigmoid")      # config.py:655-675
     c.FPN = Node(                                             # config.py:680-726
         FPN_ON=False, DIM=256, ZERO_INIT_LATERAL=False, COARSEST_STRIDE=32, MULTILEVEL_ROIS=False,

@@ -12,6 +12,7 @@ import torch.nn.functional as F
 import torch.nn.init as init
 
 from ..affine_channel import conv_bias_act
+from ..linear_cross_entropy import linear_cross_entropy
 from .layers import BilinearInterpolation2d, msra_fill, smooth_l1_loss, xavier_fill
 
 
@@ -72,6 +73,25 @@ def fast_rcnn_losses(cls_score, bbox_pred, labels, bbox_targets, bbox_inside_wei
     loss_cls = F.cross_entropy(cls_score, labels, ignore_index=-1)
     loss_bbox = smooth_l1_loss(bbox_pred, bbox_targets, bbox_inside_weights, bbox_outside_weights, num_rows=num_rows)
     preds = cls_score.max(dim=1)[1]
+    accuracy = ((preds == labels) & real).float().sum() / num_rows
+    return loss_cls, loss_bbox, accuracy
+
+
+def fast_rcnn_losses_in_pieces(box_outs, x, labels, bbox_targets, bbox_inside_weights, bbox_outside_weights):
+    """`fast_rcnn_losses` of `box_outs(x)` without the class scores in memory (cfg.FAST_RCNN.CLS_LOSS_IN_PIECES): the score
+    layer and its cross entropy are one operator on the GPU.  Under autocast the score layer's product runs in the autocast
+    type, as nn.Linear's would.  A minibatch without a real row has loss 0 (cross_entropy: NaN)."""
+    if x.dim() == 4:
+        x = x.squeeze(3).squeeze(2)
+    weight, bias, feat = box_outs.cls_score.weight, box_outs.cls_score.bias, x
+    if torch.is_autocast_enabled():
+        dtype = torch.get_autocast_dtype("cuda")
+        weight, bias, feat = weight.to(dtype), bias.to(dtype), feat.to(dtype)
+    loss_cls, preds = linear_cross_entropy(feat, weight, bias, labels, ignore_index=-1, with_pred=True)
+    real = (labels >= 0)
+    num_rows = real.sum().clamp_min(1).float()
+    loss_bbox = smooth_l1_loss(box_outs.bbox_pred(x).float(), bbox_targets, bbox_inside_weights, bbox_outside_weights,
+                               num_rows=num_rows)
     accuracy = ((preds == labels) & real).float().sum() / num_rows
     return loss_cls, loss_bbox, accuracy
 

@@ -173,15 +173,20 @@ class GeneralizedRCNN(nn.Module):
                                             gt_polygons=roidb.get("gt_polygons"), rasterize_fn=self.rasterize_fn)
         self._mark("proposals_labelling")
         box_feat = self.Box_Head(roi_blobs, blobs)
-        cls_score, bbox_pred = self.Box_Outs(box_feat)
+        in_pieces = cfg.FAST_RCNN.CLS_LOSS_IN_PIECES
+        if not in_pieces:
+            cls_score, bbox_pred = self.Box_Outs(box_feat)
         losses, metrics = {}, {}
         loss_rpn_cls, loss_rpn_bbox = fpn_mod.fpn_rpn_losses(cfg, rpn_ret, rpn_targets)
         for i, lvl in enumerate(range(cfg.FPN.RPN_MIN_LEVEL, cfg.FPN.RPN_MAX_LEVEL + 1)):
             losses["loss_rpn_cls_fpn%d" % lvl] = loss_rpn_cls[i]
             losses["loss_rpn_bbox_fpn%d" % lvl] = loss_rpn_bbox[i]
-        loss_cls, loss_bbox, accuracy = heads.fast_rcnn_losses(
-            cls_score.float(), bbox_pred.float(), blobs["labels_int32"], blobs["bbox_targets"],
-            blobs["bbox_inside_weights"], blobs["bbox_outside_weights"])
+        targets_of_boxes = (blobs["labels_int32"], blobs["bbox_targets"], blobs["bbox_inside_weights"],
+                            blobs["bbox_outside_weights"])
+        if in_pieces:
+            loss_cls, loss_bbox, accuracy = heads.fast_rcnn_losses_in_pieces(self.Box_Outs, box_feat, *targets_of_boxes)
+        else:
+            loss_cls, loss_bbox, accuracy = heads.fast_rcnn_losses(cls_score.float(), bbox_pred.float(), *targets_of_boxes)
         losses["loss_cls"], losses["loss_bbox"] = loss_cls, loss_bbox
         metrics["accuracy_cls"] = accuracy
         self._mark("box_head_losses")

@@ -10,6 +10,7 @@ still runs.
 """
 import torch
 
+from ..muon import Muon
 from .model import total_loss
 
 
@@ -26,10 +27,18 @@ def parameter_groups(model, cfg):
 
 
 def make_optimizer(model, cfg, lr=None, fused=None):
+    """The optimiser of cfg.SOLVER.TYPE: "SGD" (the reference's), or "MUON": orthogonalised updates of the weight matrices with
+    SOLVER.MUON's rate and momentum, SGD for the biases.  `lr` takes the place of BASE_LR."""
     groups = parameter_groups(model, cfg)
+    if cfg.SOLVER.TYPE not in ("SGD", "MUON"):
+        raise NotImplementedError("SOLVER.TYPE %r" % (cfg.SOLVER.TYPE,))
     if lr is not None:
         groups[0]["lr"] = lr
         groups[1]["lr"] = lr * (cfg.SOLVER.BIAS_DOUBLE_LR + 1)
+    if cfg.SOLVER.TYPE == "MUON":
+        m = cfg.SOLVER.MUON
+        groups = [dict(g, lr=m.LR, sgd_lr=g["lr"]) for g in groups]
+        return Muon(groups, momentum=m.MOMENTUM, nesterov=m.NESTEROV, steps=m.STEPS, sgd_momentum=cfg.SOLVER.MOMENTUM)
     # device parameters: the single-pass update (weight decay, momentum and step in one kernel over the parameter list) instead
     # of three multi-tensor passes -- 40.17 against 40.47 ms per step on the bench's model (A/B, one box); same expressions
     if fused is None:
