@@ -217,63 +217,61 @@ __device__ __forceinline__ bool beats(float v, int at, const Best& b) {
   return v > b.v;
 }
 
+// A lane's e-th of the 16 columns of a fragment
+__device__ __forceinline__ constexpr int column(int e) { return (e >> 2) * 8 + (e & 3); }
+
 // One tile of logits -> per row and strip of columns (one strip per wave column) the maximum and the sum of exp(z - max).
 template <class P, int T, bool PRED>
-__global__ __launch_bounds__(P::kThreads) void logits_forward(Operand x, Operand w, const void* bias, const int* lab,
+__global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_forward(Operand x, Operand w, const void* bias, const int* lab,
                                                               const Scalars* sc, int rows, int rows_p, int classes,
                                                               int tiles_m, int tiles_n, int steps, float2* part, Best* best,
                                                               float* target) {
   extern __shared__ char smem[];
   int tm, tn;
   tile_of(blockIdx.x, tiles_m, tiles_n, 4, tm, tn);
-  f32x4 acc[P::FM][P::FN];
+  f32x16 acc[P::FM][P::FN];
   P::run(acc, x, w, tm * P::BM, tn * P::BN, 0, steps, (lds_bytes)smem);
   const int row0 = tm * P::BM + P::lane_row(), col0 = tn * P::BN + P::lane_col();
   const float ix = P::SPLIT ? sc->inv_x : 1.f, iw = P::SPLIT ? sc->inv_w : 1.f;
-  float b[P::FN][4];
+  float b[P::FN][16];
 #pragma unroll
   for (int j = 0; j < P::FN; ++j)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int col = col0 + j * 16 + r;
+    for (int r = 0; r < 16; ++r) {
+      const int col = col0 + j * 32 + column(r);
       b[j][r] = (bias != nullptr && col < classes) ? load_as_float<T>(bias, col) : 0.f;
     }
   const int strip = tn * P::WC + uniform((int)(threadIdx.x >> 6)) % P::WC;
 #pragma unroll
   for (int i = 0; i < P::FM; ++i) {
-    const int row = row0 + i * 16;
+    const int row = row0 + i * 32;
     const int y = row < rows ? lab[row] : kIgnored;
     float m = -INFINITY;
     Best best_here = {-INFINITY, 0x7fffffff};
 #pragma unroll
     for (int j = 0; j < P::FN; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int col = col0 + j * 16 + r;
+      for (int r = 0; r < 16; ++r) {
+        const int col = col0 + j * 32 + column(r);
         const float z = col < classes ? (P::SPLIT ? acc[i][j][r] * ix * iw : acc[i][j][r]) + b[j][r] : -INFINITY;
         acc[i][j][r] = z;
         m = fmaxf(m, z);
         if (col == y) target[row] = z;
         if (PRED && col < classes && beats(z, col, best_here)) best_here = {z, col};
       }
-    m = fmaxf(m, __shfl_xor(m, 16));
     m = fmaxf(m, __shfl_xor(m, 32));
     const float from = m == -INFINITY ? 0.f : m;  // a strip of classes that are all masked sums to zero
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < P::FN; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s += __expf(acc[i][j][r] - from);
-    s += __shfl_xor(s, 16);
+      for (int r = 0; r < 16; ++r) s += __expf(acc[i][j][r] - from);
     s += __shfl_xor(s, 32);
     if constexpr (PRED) {
-#pragma unroll
-      for (int d = 16; d <= 32; d <<= 1) {
-        const Best o = {__shfl_xor(best_here.v, d), __shfl_xor(best_here.at, d)};
-        if (beats(o.v, o.at, best_here)) best_here = o;
-      }
+      const Best o = {__shfl_xor(best_here.v, 32), __shfl_xor(best_here.at, 32)};
+      if (beats(o.v, o.at, best_here)) best_here = o;
     }
-    if (row < rows && (threadIdx.x & 48) == 0) {
+    if (row < rows && (threadIdx.x & 32) == 0) {
       part[(long long)strip * rows_p + row] = make_float2(m, s);
       if constexpr (PRED) best[(long long)strip * rows_p + row] = best_here;
     }
@@ -368,72 +366,75 @@ __global__ __launch_bounds__(1024) void row_factors(const float* grad, int reduc
 
 // One tile of logits, again -> q times its row's factor; column sums for the bias gradient, one strip per wave row.
 template <class P, int T>
-__global__ __launch_bounds__(P::kThreads) void logits_backward(Operand x, Operand w, const void* bias, const int* lab,
+__global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_backward(Operand x, Operand w, const void* bias, const int* lab,
                                                                const float* lse, const float* factors, const Scalars* sc,
                                                                int rows_p, int class0, int classes, int classes_p,
                                                                int tiles_m, int tiles_n, int steps, uint16_t* q, float* sums) {
   extern __shared__ char smem[];
   int tm, tn;
   tile_of(blockIdx.x, tiles_m, tiles_n, 4, tm, tn);
-  f32x4 acc[P::FM][P::FN];
+  f32x16 acc[P::FM][P::FN];
   P::run(acc, x, w, tm * P::BM, tn * P::BN, 0, steps, (lds_bytes)smem);
   const int row0 = tm * P::BM + P::lane_row(), col0 = tn * P::BN + P::lane_col();
   const float ix = P::SPLIT ? sc->inv_x : 1.f, iw = P::SPLIT ? sc->inv_w : 1.f;
   const long long ld = (long long)classes_p * (P::SPLIT ? 2 : 1);
-  float b[P::FN][4], sum[P::FN][4];
+  float b[P::FN][16], sum[P::FN][16];
 #pragma unroll
   for (int j = 0; j < P::FN; ++j)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int col = col0 + j * 16 + r;
+    for (int r = 0; r < 16; ++r) {
+      const int col = col0 + j * 32 + column(r);
       b[j][r] = (bias != nullptr && col < classes) ? load_as_float<T>(bias, class0 + col) : 0.f;
       sum[j][r] = 0.f;
     }
 #pragma unroll
   for (int i = 0; i < P::FM; ++i) {
-    const int row = row0 + i * 16;
+    const int row = row0 + i * 32;
     const bool in = row < rows_p;
     const int y = in ? lab[row] : kIgnored;
     const float l = in ? lse[row] : 0.f, f = in ? factors[row] : 0.f;
 #pragma unroll
-    for (int j = 0; j < P::FN; ++j) {
-      const int col = col0 + j * 16;
-      s16x4 hi, lo;
+    for (int j = 0; j < P::FN; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float z = (P::SPLIT ? acc[i][j][r] * ix * iw : acc[i][j][r]) + b[j][r];
-        float v = 0.f;
-        if (y != kIgnored && col + r < classes) v = (__expf(z - l) - (class0 + col + r == y ? 1.f : 0.f)) * f;
-        sum[j][r] += v;
-        if constexpr (P::SPLIT) {
-          const _Float16 h = (_Float16)v;
-          hi[r] = __builtin_bit_cast(short, h);
-          lo[r] = (short)half_bits(v - (float)h);
-        } else {
-          hi[r] = (short)round16<T>(v);
+      for (int g = 0; g < 4; ++g) {
+        const int col = col0 + j * 32 + g * 8;
+        s16x4 hi, lo;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int e = g * 4 + r;
+          const float z = (P::SPLIT ? acc[i][j][e] * ix * iw : acc[i][j][e]) + b[j][e];
+          float v = 0.f;
+          if (y != kIgnored && col + r < classes) v = (__expf(z - l) - (class0 + col + r == y ? 1.f : 0.f)) * f;
+          sum[j][e] += v;
+          if constexpr (P::SPLIT) {
+            const _Float16 h = (_Float16)v;
+            hi[r] = __builtin_bit_cast(short, h);
+            lo[r] = (short)half_bits(v - (float)h);
+          } else {
+            hi[r] = (short)round16<T>(v);
+          }
+        }
+        if (in && col < classes_p) {
+          if constexpr (P::SPLIT) {
+            uint16_t* at = q + row * ld + (col >> 5) * 64 + (col & 31);
+            *reinterpret_cast<s16x4*>(at) = hi;
+            *reinterpret_cast<s16x4*>(at + 32) = lo;
+          } else {
+            *reinterpret_cast<s16x4*>(q + row * ld + col) = hi;
+          }
         }
       }
-      if (in && col < classes_p) {
-        if constexpr (P::SPLIT) {
-          uint16_t* at = q + row * ld + (col >> 5) * 64 + (col & 31);
-          *reinterpret_cast<s16x4*>(at) = hi;
-          *reinterpret_cast<s16x4*>(at + 32) = lo;
-        } else {
-          *reinterpret_cast<s16x4*>(q + row * ld + col) = hi;
-        }
-      }
-    }
   }
   if (sums == nullptr) return;
   const int strip = tm * P::WR + uniform((int)(threadIdx.x >> 6)) / P::WC;
 #pragma unroll
   for (int j = 0; j < P::FN; ++j)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
+    for (int r = 0; r < 16; ++r) {
       float v = sum[j][r];
-      for (int d = 1; d < 16; d <<= 1) v += __shfl_xor(v, d);
-      const int col = col0 + j * 16 + r;
-      if ((threadIdx.x & 15) == 0 && col < classes) sums[(long long)strip * classes_p + col] = v;
+      for (int d = 1; d < 32; d <<= 1) v += __shfl_xor(v, d);
+      const int col = col0 + j * 32 + column(r);
+      if ((threadIdx.x & 31) == 0 && col < classes) sums[(long long)strip * classes_p + col] = v;
     }
 }
 
@@ -450,33 +451,51 @@ __global__ __launch_bounds__(256) void bias_gradient(const float* sums, int stri
 // A gradient's tile: slice blockIdx.y of the k axis.  With one slice and one piece the result goes out rounded; otherwise
 // the slices' float32 sums are kept (and added to those of the pieces before) and joined by join_slices in their order.
 template <class P, int T, bool OF_WEIGHT>
-__global__ __launch_bounds__(P::kThreads) void gradient_product(Operand a, Operand b, int rows, int cols, int tiles_m,
+__global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void gradient_product(Operand a, Operand b, int rows, int cols, int tiles_m,
                                                                 int tiles_n, int steps, int per_slice, const Scalars* sc,
-                                                                const float* factor, void* out, long long out_ld,
-                                                                float* slices, int add) {
+                                                                const float* factor, void* out, float* slices, int add) {
   extern __shared__ char smem[];
   int tm, tn;
   tile_of(blockIdx.x, tiles_m, tiles_n, 4, tm, tn);
-  f32x4 acc[P::FM][P::FN];
+  f32x16 acc[P::FM][P::FN];
   const int step0 = blockIdx.y * per_slice, n = min(per_slice, steps - step0);
   P::run(acc, a, b, tm * P::BM, tn * P::BN, step0, n, (lds_bytes)smem);
   const int row0 = tm * P::BM + P::lane_row(), col0 = tn * P::BN + P::lane_col();
   const float f = *factor * (P::SPLIT ? (OF_WEIGHT ? sc->inv_x : sc->inv_w) : 1.f);
+  const bool whole = (cols & 3) == 0;  // then every four columns of a lane are inside or outside together, and aligned
 #pragma unroll
   for (int i = 0; i < P::FM; ++i) {
-    const int row = row0 + i * 16;
+    const int row = row0 + i * 32;
     if (row >= rows) continue;
 #pragma unroll
     for (int j = 0; j < P::FN; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int col = col0 + j * 16 + r;
+      for (int g = 0; g < 4; ++g) {
+        const int col = col0 + j * 32 + g * 8;
         if (col >= cols) continue;
+        f32x4 v = P::quad(acc[i][j], g);
         if (slices != nullptr) {
           float* at = slices + ((long long)blockIdx.y * rows + row) * cols + col;
-          *at = add ? *at + acc[i][j][r] : acc[i][j][r];
+          if (whole) {
+            if (add) v += *reinterpret_cast<const f32x4*>(at);
+            *reinterpret_cast<f32x4*>(at) = v;
+          } else {
+            for (int r = 0; r < 4; ++r)
+              if (col + r < cols) at[r] = add ? at[r] + v[r] : v[r];
+          }
         } else {
-          store_from_float<T>(out, (long long)row * out_ld + col, acc[i][j][r] * f);
+          v *= f;
+          const long long at = (long long)row * cols + col;
+          if (whole && T == MI_TYPE_F32) {
+            *reinterpret_cast<f32x4*>(static_cast<float*>(out) + at) = v;
+          } else if (whole) {
+            s16x4 h;
+            for (int r = 0; r < 4; ++r) h[r] = (short)round16<T>(v[r]);
+            *reinterpret_cast<s16x4*>(static_cast<uint16_t*>(out) + at) = h;
+          } else {
+            for (int r = 0; r < 4; ++r)
+              if (col + r < cols) store_from_float<T>(out, at + r, v[r]);
+          }
         }
       }
   }
@@ -495,29 +514,33 @@ __global__ __launch_bounds__(256) void join_slices(const float* slices, int n, l
 
 // ---- launching -----------------------------------------------------------------------------------------------------------
 
-// Tiles of 128 x 128 where they give every compute unit one (two fit a unit and hide each other's waits), else 64 x 64 with
-// a deeper pipeline: 1024 x 1204 x 1024 in float32 takes 20 us with the small tiles and 30 us with the large ones,
-// 8192 x 8192 x 4096 2.5 ms and 1.3 ms.
-bool large_tiles(long long m, long long n, int slices) {
-  return (long long)ceil_div(m, 128) * ceil_div(n, 128) * slices >= compute_units();
+// The tile of a product whose k axis stays whole.
+int tile_for(long long m, long long n, bool split) {
+  const auto tiles = [&](int t) { return (long long)ceil_div(m, t) * ceil_div(n, t); };
+  return choose_tile(tiles(256), tiles(128), tiles(64), split);
 }
 
-template <bool SPLIT, bool BF16, bool AKM, bool BKM>
-using Large = TileProduct<128, 128, 2, 2, 2, SPLIT, BF16, AKM, BKM>;
-template <bool SPLIT, bool BF16, bool AKM, bool BKM>
-using Small = TileProduct<64, 64, 2, 2, 4, SPLIT, BF16, AKM, BKM>;
-
-// Slices of a gradient's k axis: as many as give every compute unit a small tile or two, each at least 8 stages long.
-int slices_of(long long m, long long n, long long steps) {
-  const long long tiles = (long long)ceil_div(m, 64) * ceil_div(n, 64);
-  long long s = tiles >= compute_units() ? 1 : 2LL * compute_units() / tiles;
-  if (s > steps / 8) s = steps / 8;
-  return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+// Tile and number of k slices of a gradient: the least estimated time, a join costing a launch and the slices' way to memory and
+// back.  A slice is at least 8 stages long.
+struct Cut {
+  int tile, slices;
+};
+Cut cut_for(long long m, long long n, long long steps, bool split, bool must_join) {
+  Cut best = {64, 1};
+  float least = INFINITY;
+  for (int tile : {256, 128, 64})
+    for (long long s = 1; s == 1 || (s <= 64 && steps / s >= 8); s *= 2) {
+      const long long tiles = (long long)ceil_div(m, tile) * ceil_div(n, tile) * s;
+      const bool join = s > 1 || must_join;
+      const float us = stage_us(tile, split, tiles) * ceil_div(steps, s) + (join ? 3.f + 8e-6f * m * n * (s + 1) / 4 : 0.f);
+      if (us < least) least = us, best = {tile, (int)s};
+    }
+  return best;
 }
 
 struct Pieces {
   int n, width;  // of the vocabulary; width is a multiple of kPad
-  int x_slices, w_slices;
+  Cut x, w;
   size_t q_at, sums_at, factors_at, slices_at, bytes;
 };
 
@@ -530,14 +553,14 @@ Pieces make_pieces(const Plan& p) {
   c.width = ceil_div(ceil_div(p.classes, c.n), kPad) * kPad;
   c.n = ceil_div(p.classes, c.width);
   const int step = p.split ? 32 : 64;
-  c.x_slices = slices_of(p.rows, p.dim, c.width / step);
-  c.w_slices = slices_of(c.width, p.dim, p.rows_p / step);
+  c.x = cut_for(p.rows, p.dim, c.width / step, p.split, c.n > 1);
+  c.w = cut_for(c.width, p.dim, p.rows_p / step, p.split, false);
   size_t at = 0;
   c.q_at = at, at = up(at + (size_t)p.rows_p * c.width * words * 2);
   c.sums_at = at, at = up(at + (size_t)(ceil_div(p.rows_p, 64) * 2) * c.width * 4);
   c.factors_at = at, at = up(at + (size_t)(p.rows_p + 1) * 4);
-  const size_t xs = c.n > 1 || c.x_slices > 1 ? (size_t)c.x_slices * p.rows * p.dim * 4 : 0;
-  const size_t ws = c.w_slices > 1 ? (size_t)c.w_slices * c.width * p.dim * 4 : 0;
+  const size_t xs = c.n > 1 || c.x.slices > 1 ? (size_t)c.x.slices * p.rows * p.dim * 4 : 0;
+  const size_t ws = c.w.slices > 1 ? (size_t)c.w.slices * c.width * p.dim * 4 : 0;
   c.slices_at = at, at = up(at + xs) + up(ws);
   c.bytes = at;
   return c;
@@ -548,7 +571,7 @@ struct ForwardRoom {
 };
 ForwardRoom make_room(const Plan& p, bool with_pred) {
   ForwardRoom f;
-  const size_t strips = (size_t)ceil_div(p.classes, large_tiles(p.rows, p.classes, 1) ? 128 : 64) * 2;
+  const size_t strips = (size_t)ceil_div(p.classes, tile_for(p.rows, p.classes, p.split)) * 2;
   size_t at = 0;
   f.parts_at = at, at = up(at + strips * p.rows_p * sizeof(float2));
   f.best_at = at, at = up(at + (with_pred ? strips * p.rows_p * sizeof(Best) : 0));
@@ -598,13 +621,14 @@ void lay_out_all(const Plan& p, const Call& c, float* maxima) {
       reinterpret_cast<int*>(c.saved + p.lab_at), maxima, xb, wb, reinterpret_cast<Scalars*>(c.saved + p.scalars_at));
 }
 
-template <class P, int T, bool PRED>
-int launch_logits(const Plan& p, const Call& c, const ForwardRoom& f) {
+template <class P, int T>
+int launch_logits(const Plan& p, const Call& c, const ForwardRoom& f, bool with_pred) {
   const Operand x = {reinterpret_cast<uint16_t*>(c.saved + p.x_at), p.ld, p.rows_p, p.dim_p};
   const Operand w = {weights_of(p, c), weights_ld(p, c), p.classes, p.dim_p};
   const int tm = ceil_div(p.rows, P::BM), tn = ceil_div(p.classes, P::BN);
-  allow_lds(logits_forward<P, T, PRED>, P::kLds);
-  logits_forward<P, T, PRED><<<tm * tn, P::kThreads, P::kLds, c.stream>>>(
+  const auto kernel = with_pred ? logits_forward<P, T, true> : logits_forward<P, T, false>;
+  allow_lds(kernel, P::kLds);
+  kernel<<<tm * tn, P::kThreads, P::kLds, c.stream>>>(
       x, w, c.bias, reinterpret_cast<const int*>(c.saved + p.lab_at), reinterpret_cast<const Scalars*>(c.saved + p.scalars_at),
       p.rows, p.rows_p, p.classes, tm, tn, p.dim_p / P::kStep, reinterpret_cast<float2*>(c.room + f.parts_at),
       reinterpret_cast<Best*>(c.room + f.best_at), reinterpret_cast<float*>(c.room + f.target_at));
@@ -620,13 +644,10 @@ int forward(const Plan& p, const Call& c, float* loss, float* losses, int64_t* p
     lay_out_all<T, int64_t>(p, c, maxima);
   else
     lay_out_all<T, int32_t>(p, c, maxima);
-  int strips;
-  if (large_tiles(p.rows, p.classes, 1))
-    strips = pred ? launch_logits<Large<split, bf16, false, false>, T, true>(p, c, f)
-                  : launch_logits<Large<split, bf16, false, false>, T, false>(p, c, f);
-  else
-    strips = pred ? launch_logits<Small<split, bf16, false, false>, T, true>(p, c, f)
-                  : launch_logits<Small<split, bf16, false, false>, T, false>(p, c, f);
+  const int tile = tile_for(p.rows, p.classes, split);
+  const int strips = tile == 256   ? launch_logits<Tile256<split, bf16, false, false>, T>(p, c, f, pred != nullptr)
+                     : tile == 128 ? launch_logits<Tile128<split, bf16, false, false>, T>(p, c, f, pred != nullptr)
+                                   : launch_logits<Tile64<split, bf16, false, false>, T>(p, c, f, pred != nullptr);
   float* per_row = losses != nullptr ? losses : reinterpret_cast<float*>(c.room + f.losses_at);
   const int* lab = reinterpret_cast<const int*>(c.saved + p.lab_at);
   join_strips<<<ceil_div(p.rows_p, 16), 256, 0, c.stream>>>(
@@ -656,11 +677,11 @@ int launch_q(const Plan& p, const Call& c, const Pieces& s, int class0, int clas
 
 template <class P, int T, bool OF_WEIGHT>
 void launch_gradient(const Operand& a, const Operand& b, int rows, int cols, int steps, int slices, const Scalars* sc,
-                     const float* factor, void* out, long long out_ld, float* room, int add, hipStream_t stream) {
+                     const float* factor, void* out, float* room, int add, hipStream_t stream) {
   const int tm = ceil_div(rows, P::BM), tn = ceil_div(cols, P::BN), per = ceil_div(steps, slices);
   allow_lds(gradient_product<P, T, OF_WEIGHT>, P::kLds);
   gradient_product<P, T, OF_WEIGHT><<<dim3(tm * tn, slices), P::kThreads, P::kLds, stream>>>(
-      a, b, rows, cols, tm, tn, steps, per, sc, factor, out, out_ld, room, add);
+      a, b, rows, cols, tm, tn, steps, per, sc, factor, out, room, add);
 }
 
 template <int T>
@@ -675,15 +696,18 @@ int backward(const Plan& p, const Call& c, const float* grad, void* grad_x, void
                                         factors, sc);
   const uint16_t* q = reinterpret_cast<const uint16_t*>(c.room + s.q_at);
   const long long ldw = weights_ld(p, c);
-  const bool x_joined = s.n > 1 || s.x_slices > 1;
+  const bool x_joined = s.n > 1 || s.x.slices > 1;
   float* x_room = reinterpret_cast<float*>(c.room + s.slices_at);
-  float* w_room = reinterpret_cast<float*>(c.room + s.slices_at + (x_joined ? up((size_t)s.x_slices * p.rows * p.dim * 4) : 0));
+  float* w_room = reinterpret_cast<float*>(c.room + s.slices_at + (x_joined ? up((size_t)s.x.slices * p.rows * p.dim * 4) : 0));
   for (int k = 0; k < s.n; ++k) {
     const int class0 = k * s.width, classes = p.classes - class0 < s.width ? p.classes - class0 : s.width;
     const int classes_p = ceil_div(classes, kPad) * kPad;
-    const int strips = large_tiles(p.rows_p, classes_p, 1)
-                           ? launch_q<Large<split, bf16, false, false>, T>(p, c, s, class0, classes, classes_p, grad_b != nullptr)
-                           : launch_q<Small<split, bf16, false, false>, T>(p, c, s, class0, classes, classes_p, grad_b != nullptr);
+    const int tile = tile_for(p.rows_p, classes_p, split);
+    const bool want_b = grad_b != nullptr;
+    const int strips =
+        tile == 256   ? launch_q<Tile256<split, bf16, false, false>, T>(p, c, s, class0, classes, classes_p, want_b)
+        : tile == 128 ? launch_q<Tile128<split, bf16, false, false>, T>(p, c, s, class0, classes, classes_p, want_b)
+                      : launch_q<Tile64<split, bf16, false, false>, T>(p, c, s, class0, classes, classes_p, want_b);
     if (grad_b != nullptr)
       bias_gradient<T><<<ceil_div(classes, 256), 256, 0, c.stream>>>(reinterpret_cast<const float*>(c.room + s.sums_at), strips,
                                                                    classes, classes_p, factor, grad_b, class0);
@@ -692,33 +716,40 @@ int backward(const Plan& p, const Call& c, const float* grad, void* grad_x, void
       const Operand b = {weights_of(p, c) + class0 * ldw, ldw, p.dim, classes};
       // every piece has the same slices: a last, shorter piece leaves some of them empty
       const int steps = classes_p / step;
-      if (large_tiles(p.rows, p.dim, s.x_slices))
-        launch_gradient<Large<split, bf16, false, true>, T, false>(a, b, p.rows, p.dim, steps, s.x_slices, sc, factor, grad_x, p.dim,
-                                                                   x_joined ? x_room : nullptr, k > 0, c.stream);
+      float* room = x_joined ? x_room : nullptr;
+      if (s.x.tile == 256)
+        launch_gradient<Tile256<split, bf16, false, true>, T, false>(a, b, p.rows, p.dim, steps, s.x.slices, sc, factor, grad_x,
+                                                                     room, k > 0, c.stream);
+      else if (s.x.tile == 128)
+        launch_gradient<Tile128<split, bf16, false, true>, T, false>(a, b, p.rows, p.dim, steps, s.x.slices, sc, factor, grad_x,
+                                                                     room, k > 0, c.stream);
       else
-        launch_gradient<Small<split, bf16, false, true>, T, false>(a, b, p.rows, p.dim, steps, s.x_slices, sc, factor, grad_x, p.dim,
-                                                                   x_joined ? x_room : nullptr, k > 0, c.stream);
+        launch_gradient<Tile64<split, bf16, false, true>, T, false>(a, b, p.rows, p.dim, steps, s.x.slices, sc, factor, grad_x,
+                                                                    room, k > 0, c.stream);
     }
     if (grad_w != nullptr) {
       const Operand a = {q, (long long)classes_p * words, classes_p, p.rows_p};
       const Operand b = {reinterpret_cast<uint16_t*>(c.saved + p.x_at), p.ld, p.dim, p.rows_p};
       void* out = static_cast<char*>(grad_w) + (size_t)class0 * p.dim * out_bytes;
-      float* room = s.w_slices > 1 ? w_room : nullptr;
-      if (large_tiles(classes, p.dim, s.w_slices))
-        launch_gradient<Large<split, bf16, true, true>, T, true>(a, b, classes, p.dim, p.rows_p / step, s.w_slices, sc, factor, out,
-                                                                 p.dim, room, 0, c.stream);
+      float* room = s.w.slices > 1 ? w_room : nullptr;
+      if (s.w.tile == 256)
+        launch_gradient<Tile256<split, bf16, true, true>, T, true>(a, b, classes, p.dim, p.rows_p / step, s.w.slices, sc, factor,
+                                                                   out, room, 0, c.stream);
+      else if (s.w.tile == 128)
+        launch_gradient<Tile128<split, bf16, true, true>, T, true>(a, b, classes, p.dim, p.rows_p / step, s.w.slices, sc, factor,
+                                                                   out, room, 0, c.stream);
       else
-        launch_gradient<Small<split, bf16, true, true>, T, true>(a, b, classes, p.dim, p.rows_p / step, s.w_slices, sc, factor, out,
-                                                                 p.dim, room, 0, c.stream);
+        launch_gradient<Tile64<split, bf16, true, true>, T, true>(a, b, classes, p.dim, p.rows_p / step, s.w.slices, sc, factor,
+                                                                  out, room, 0, c.stream);
       if (room != nullptr) {
         const long long n = (long long)classes * p.dim;
-        join_slices<T, true><<<grid_for(n, 256), 256, 0, c.stream>>>(room, s.w_slices, n, sc, factor, out);
+        join_slices<T, true><<<grid_for(n, 256), 256, 0, c.stream>>>(room, s.w.slices, n, sc, factor, out);
       }
     }
   }
   if (grad_x != nullptr && x_joined) {
     const long long n = (long long)p.rows * p.dim;
-    join_slices<T, false><<<grid_for(n, 256), 256, 0, c.stream>>>(x_room, s.x_slices, n, sc, factor, grad_x);
+    join_slices<T, false><<<grid_for(n, 256), 256, 0, c.stream>>>(x_room, s.x.slices, n, sc, factor, grad_x);
   }
   return check_launch("mi_linear_cross_entropy_backward");
 }

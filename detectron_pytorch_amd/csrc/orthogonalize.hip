@@ -187,7 +187,7 @@ __host__ __device__ inline int triangle_tiles(int n) { return n * (n + 1) / 2; }
 
 // X X': one tile of the upper triangle and one slice of the sum over n, in float32.
 template <class P>
-__global__ __launch_bounds__(P::kThreads) void gram(Table t, Tiles tiles, char* ws, int flip) {
+__global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void gram(Table t, Tiles tiles, char* ws, int flip) {
   extern __shared__ char smem[];
   const int k = find(tiles, t.count, blockIdx.x);
   const Mat& q = t.m[k];
@@ -197,16 +197,18 @@ __global__ __launch_bounds__(P::kThreads) void gram(Table t, Tiles tiles, char* 
   triangle(id - slice * per, nt, ti, tj);
   const int ld = up32(q.n), steps = ld / 32, each = div_up(steps, q.slices), step0 = slice * each;
   const Operand x = {reinterpret_cast<const uint16_t*>(ws + (flip ? q.y_at : q.x_at)), (long long)ld * 2, q.m, ld};
-  f32x4 acc[P::FM][P::FN];
+  f32x16 acc[P::FM][P::FN];
   P::run(acc, x, x, ti * P::BM, tj * P::BN, step0, min(each, steps - step0), (lds_bytes)smem);
   float* c = reinterpret_cast<float*>(ws + q.c_at) + (long long)slice * q.m * up32(q.m);
   const int row0 = ti * P::BM + P::lane_row(), col0 = tj * P::BN + P::lane_col();
 #pragma unroll
   for (int i = 0; i < P::FM; ++i)
 #pragma unroll
-    for (int j = 0; j < P::FN; ++j) {
-      const int row = row0 + i * 16, col = col0 + j * 16;
-      if (row < q.m && col < up32(q.m)) *reinterpret_cast<f32x4*>(c + (long long)row * up32(q.m) + col) = acc[i][j];
+    for (int j = 0; j < P::FN; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+      const int row = row0 + i * 32, col = col0 + j * 32 + g * 8;
+      if (row < q.m && col < up32(q.m)) *reinterpret_cast<f32x4*>(c + (long long)row * up32(q.m) + col) = P::quad(acc[i][j], g);
     }
 }
 
@@ -240,7 +242,7 @@ __global__ __launch_bounds__(256) void join_gram(Table t, Tiles tiles, char* ws)
 
 // B = b A + c A A: one tile of the upper triangle, written on both sides (the padding of a row lies in its upper half).
 template <class P>
-__global__ __launch_bounds__(P::kThreads) void polynomial(Table t, Tiles tiles, Step s, char* ws) {
+__global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void polynomial(Table t, Tiles tiles, Step s, char* ws) {
   extern __shared__ char smem[];
   const int k = find(tiles, t.count, blockIdx.x);
   const Mat& q = t.m[k];
@@ -250,19 +252,21 @@ __global__ __launch_bounds__(P::kThreads) void polynomial(Table t, Tiles tiles, 
   const uint16_t* a = reinterpret_cast<const uint16_t*>(ws + q.a_at);
   uint16_t* b = reinterpret_cast<uint16_t*>(ws + q.b_at);
   const Operand o = {a, (long long)ld * 2, q.m, ld};
-  f32x4 acc[P::FM][P::FN];
+  f32x16 acc[P::FM][P::FN];
   P::run(acc, o, o, ti * P::BM, tj * P::BN, 0, ld / 32, (lds_bytes)smem);
   const int row0 = ti * P::BM + P::lane_row(), col0 = tj * P::BN + P::lane_col();
 #pragma unroll
   for (int i = 0; i < P::FM; ++i)
 #pragma unroll
-    for (int j = 0; j < P::FN; ++j) {
-      const int row = row0 + i * 16, col = col0 + j * 16;
+    for (int j = 0; j < P::FN; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+      const int row = row0 + i * 32, col = col0 + j * 32 + g * 8;
       if (row >= q.m || col >= ld) continue;
       const f32x4 here = get_split4(a + split_at(row, col, ld));
       f32x4 v;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = col + r < q.m ? s.b * here[r] + s.c * (acc[i][j][r] * (1.f / kScale)) : 0.f;
+      for (int r = 0; r < 4; ++r) v[r] = col + r < q.m ? s.b * here[r] + s.c * (acc[i][j][g * 4 + r] * (1.f / kScale)) : 0.f;
       put_split4(b + split_at(row, col, ld), v);
       if (ti != tj)
 #pragma unroll
@@ -273,7 +277,7 @@ __global__ __launch_bounds__(P::kThreads) void polynomial(Table t, Tiles tiles, 
 
 // X <- a X + B X, or in the last iteration the result itself.
 template <class P, int T, bool LAST>
-__global__ __launch_bounds__(P::kThreads) void apply(Table t, Tiles tiles, Step s, char* ws, int flip) {
+__global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void apply(Table t, Tiles tiles, Step s, char* ws, int flip) {
   extern __shared__ char smem[];
   const int k = find(tiles, t.count, blockIdx.x);
   const Mat& q = t.m[k];
@@ -284,19 +288,21 @@ __global__ __launch_bounds__(P::kThreads) void apply(Table t, Tiles tiles, Step 
   uint16_t* y = reinterpret_cast<uint16_t*>(ws + (flip ? q.x_at : q.y_at));
   const Operand b = {reinterpret_cast<const uint16_t*>(ws + q.b_at), (long long)ldm * 2, q.m, ldm};
   const Operand xo = {x, (long long)ld * 2, q.n, q.m};
-  f32x4 acc[P::FM][P::FN];
+  f32x16 acc[P::FM][P::FN];
   P::run(acc, b, xo, tm * P::BM, tn * P::BN, 0, ldm / 32, (lds_bytes)smem);
   const int row0 = tm * P::BM + P::lane_row(), col0 = tn * P::BN + P::lane_col();
 #pragma unroll
   for (int i = 0; i < P::FM; ++i)
 #pragma unroll
-    for (int j = 0; j < P::FN; ++j) {
-      const int row = row0 + i * 16, col = col0 + j * 16;
+    for (int j = 0; j < P::FN; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+      const int row = row0 + i * 32, col = col0 + j * 32 + g * 8;
       if (row >= q.m || col >= ld) continue;
       const f32x4 here = get_split4(x + split_at(row, col, ld));
       f32x4 v;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = s.a * here[r] + acc[i][j][r] * (1.f / kScale);
+      for (int r = 0; r < 4; ++r) v[r] = s.a * here[r] + acc[i][j][g * 4 + r] * (1.f / kScale);
       if constexpr (!LAST) {
         put_split4(y + split_at(row, col, ld), v);
       } else {
@@ -313,10 +319,14 @@ __global__ __launch_bounds__(P::kThreads) void apply(Table t, Tiles tiles, Step 
 
 // ---- launching -----------------------------------------------------------------------------------------------------------
 
-template <bool BKM>
-using Large = TileProduct<128, 128, 2, 2, 2, true, false, false, BKM>;
-template <bool BKM>
-using Small = TileProduct<64, 64, 2, 2, 4, true, false, false, BKM>;
+template <int SIDE, bool BKM>
+struct TileOf {
+  using type = TileProduct<SIDE, SIDE, 2, 2, SIDE == 64 ? 4 : 2, true, false, false, BKM>;
+};
+template <int SIDE>
+using Gram = typename TileOf<SIDE, false>::type;
+template <int SIDE>
+using Apply = typename TileOf<SIDE, true>::type;
 
 size_t up(size_t v) { return (v + 255) & ~size_t(255); }
 
@@ -375,8 +385,18 @@ void launch(K kernel, int blocks, hipStream_t stream, A... args) {
   kernel<<<blocks, P::kThreads, P::kLds, stream>>>(args...);
 }
 
-// Tiles of 128 x 128 where they give every compute unit one, else 64 x 64 (tile_product.h's pipeline is deeper there).
-bool large(const Tiles& d, const Table& t) { return d.first[t.count] >= compute_units(); }
+// One stage of the iteration over all matrices: the workgroups of each for tiles of 256, 128 and 64, and the side that is taken.
+struct Dealt {
+  Tiles tiles;
+  int side;
+};
+template <class F>
+Dealt choose(const Table& t, F tiles_of) {
+  const Tiles a = deal(t, [&](const Mat& q) { return tiles_of(q, 256); }), b = deal(t, [&](const Mat& q) { return tiles_of(q, 128); }),
+              c = deal(t, [&](const Mat& q) { return tiles_of(q, 64); });
+  const int side = choose_tile(a.first[t.count], b.first[t.count], c.first[t.count], true);
+  return {side == 256 ? a : side == 128 ? b : c, side};
+}
 
 template <int T>
 void iterate(const Table& t, const Step& s, int steps, char* ws, hipStream_t stream) {
@@ -387,35 +407,35 @@ void iterate(const Table& t, const Step& s, int steps, char* ws, hipStream_t str
   momentum_and_norm<T><<<norm.first[t.count], 256, 0, stream>>>(t, norm, s, ws);
   const Tiles squares = deal(t, [](const Mat& q) { return div_up(q.m, 64) * div_up(q.n, 64); });
   normalize<T><<<squares.first[t.count], 256, 0, stream>>>(t, squares, norm, s, ws);
-  const Tiles gram_l = deal(t, [](const Mat& q) { return triangle_tiles(div_up(q.m, 128)) * q.slices; });
-  const Tiles gram_s = deal(t, [](const Mat& q) { return triangle_tiles(div_up(q.m, 64)) * q.slices; });
-  const Tiles poly_l = deal(t, [](const Mat& q) { return triangle_tiles(div_up(q.m, 128)); });
-  const Tiles poly_s = deal(t, [](const Mat& q) { return triangle_tiles(div_up(q.m, 64)); });
-  const Tiles app_l = deal(t, [](const Mat& q) { return div_up(q.m, 128) * div_up(q.n, 128); });
-  const Tiles app_s = squares;
+  const Dealt g = choose(t, [](const Mat& q, int side) { return triangle_tiles(div_up(q.m, side)) * q.slices; });
+  const Dealt p = choose(t, [](const Mat& q, int side) { return triangle_tiles(div_up(q.m, side)); });
+  const Dealt f = choose(t, [](const Mat& q, int side) { return div_up(q.m, side) * div_up(q.n, side); });
+  const Tiles joined = deal(t, [](const Mat& q) { return triangle_tiles(div_up(q.m, 64)); });
   for (int i = 0; i < steps; ++i) {
     const int flip = i & 1;
-    if (large(gram_l, t))
-      launch<Large<false>>(gram<Large<false>>, gram_l.first[t.count], stream, t, gram_l, ws, flip);
+    if (g.side == 256)
+      launch<Gram<256>>(gram<Gram<256>>, g.tiles.first[t.count], stream, t, g.tiles, ws, flip);
+    else if (g.side == 128)
+      launch<Gram<128>>(gram<Gram<128>>, g.tiles.first[t.count], stream, t, g.tiles, ws, flip);
     else
-      launch<Small<false>>(gram<Small<false>>, gram_s.first[t.count], stream, t, gram_s, ws, flip);
-    join_gram<<<poly_s.first[t.count], 256, 0, stream>>>(t, poly_s, ws);
-    if (large(poly_l, t))
-      launch<Large<false>>(polynomial<Large<false>>, poly_l.first[t.count], stream, t, poly_l, s, ws);
+      launch<Gram<64>>(gram<Gram<64>>, g.tiles.first[t.count], stream, t, g.tiles, ws, flip);
+    join_gram<<<joined.first[t.count], 256, 0, stream>>>(t, joined, ws);
+    if (p.side == 256)
+      launch<Gram<256>>(polynomial<Gram<256>>, p.tiles.first[t.count], stream, t, p.tiles, s, ws);
+    else if (p.side == 128)
+      launch<Gram<128>>(polynomial<Gram<128>>, p.tiles.first[t.count], stream, t, p.tiles, s, ws);
     else
-      launch<Small<false>>(polynomial<Small<false>>, poly_s.first[t.count], stream, t, poly_s, s, ws);
+      launch<Gram<64>>(polynomial<Gram<64>>, p.tiles.first[t.count], stream, t, p.tiles, s, ws);
     const bool last = i + 1 == steps;
-    if (large(app_l, t)) {
-      if (last)
-        launch<Large<true>>(apply<Large<true>, T, true>, app_l.first[t.count], stream, t, app_l, s, ws, flip);
-      else
-        launch<Large<true>>(apply<Large<true>, T, false>, app_l.first[t.count], stream, t, app_l, s, ws, flip);
-    } else {
-      if (last)
-        launch<Small<true>>(apply<Small<true>, T, true>, app_s.first[t.count], stream, t, app_s, s, ws, flip);
-      else
-        launch<Small<true>>(apply<Small<true>, T, false>, app_s.first[t.count], stream, t, app_s, s, ws, flip);
-    }
+    if (f.side == 256)
+      launch<Apply<256>>(last ? apply<Apply<256>, T, true> : apply<Apply<256>, T, false>, f.tiles.first[t.count], stream, t, f.tiles,
+                         s, ws, flip);
+    else if (f.side == 128)
+      launch<Apply<128>>(last ? apply<Apply<128>, T, true> : apply<Apply<128>, T, false>, f.tiles.first[t.count], stream, t, f.tiles,
+                         s, ws, flip);
+    else
+      launch<Apply<64>>(last ? apply<Apply<64>, T, true> : apply<Apply<64>, T, false>, f.tiles.first[t.count], stream, t, f.tiles, s,
+                        ws, flip);
   }
 }
 

@@ -10,30 +10,35 @@
 // the fp32 matrix instruction, and the accuracy is that of a float32 product (the accumulators are float32 in both).
 //
 // Staging: 16 bytes per lane go from memory straight to LDS (buffer_load_dwordx4 ... lds) into STAGES buffers of
-// (BM + BN) * 128 bytes; the next STAGES - 1 stages are in flight while the waves multiply one, with one barrier per
-// stage.  The DMA writes lanes in order, so the swizzle that keeps fragment reads free of bank conflicts is applied to the lanes' source
+// (BM + BN) * 128 bytes (64 k a stage, split 32), with one barrier per stage.  Fragments are read half a stage ahead of their
+// products, so a stage's buffer is free, and the stage STAGES later on its way into it, while its second half is still being
+// multiplied.  The DMA writes lanes in order, so the swizzle that keeps fragment reads free of bank conflicts is applied to the lanes' source
 // addresses.  The buffer descriptor ends with the operand: what lies behind it reads as zero.
 // The caller pads k with zeros to kStep in rows-of-k operands; a k-major operand ends after its last k by the descriptor.
 #pragma once
 
+#include "common.h"
 #include "lds_dma.h"
 
 namespace mi {
 namespace {
 
 using f32x4 = __attribute__((ext_vector_type(4))) float;
+using f32x16 = __attribute__((ext_vector_type(16))) float;
 using s16x4 = __attribute__((ext_vector_type(4))) short;
 using s16x8 = __attribute__((ext_vector_type(8))) short;
 using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 using lds_bytes = __attribute__((address_space(3))) char*;
 
+// The 32 x 32 x 16 form: one wave per SIMD keeps the matrix cores busy with it (2.46 PFLOP/s over the chip on zeros), where the
+// 16 x 16 x 32 form reaches 1.45-1.58 with one wave per SIMD and 2.27 with two.
 template <bool BF16>
-__device__ __forceinline__ f32x4 mfma_16x16x32(s16x8 a, s16x8 b, f32x4 c) {
+__device__ __forceinline__ f32x16 mfma_32x32x16(s16x8 a, s16x8 b, f32x16 c) {
   if constexpr (BF16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   else
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
 // One operand as the product sees it.  `rows`: its extent in the tile's direction; `k`: its extent in k (padded to kStep for
@@ -50,17 +55,19 @@ struct Loader {
   static constexpr int kPer = kPieces / WAVES;
   static_assert(kPieces % WAVES == 0, "every wave issues the same number of pieces");
   static constexpr int kWords = SPLIT ? 2 : 1;
-  static constexpr int kStep = SPLIT ? 32 : 64;
+  static constexpr int kStep = 64 / kWords;
   static constexpr int kRowBytes = ROWS * kWords * 2;  // k-major: bytes of one k in LDS
   unsigned voff[kPer];
   uintptr_t at;      // stage's first byte
   long long left;    // bytes of the operand from `at` on
   long long advance;
 
+  // XOR of a row's chunks: the rows that a fragment read touches at once fall into all banks evenly
+  static __device__ __forceinline__ int shuffle(int row) { return (row >> 1) & 7; }
   // XOR of a k-major row's 32-byte units: the 16 rows that a fragment read touches at once fall into all banks evenly
   static __device__ __forceinline__ unsigned twist(unsigned k) {
-    if constexpr (kRowBytes == 128) return ((k >> 1) & 1) | (((k >> 3) & 1) << 1);
-    return (k & 3) | (((k >> 3) & 1) << 2);
+    if constexpr (kRowBytes == 128) return (((k >> 1) & 1) << 1) | ((k >> 3) & 1);
+    return ((k & 3) << 1) | ((k >> 3) & 1);
   }
 
   __device__ __forceinline__ void init(const Operand& o, int row0, int step0, int wave, int lane) {
@@ -69,7 +76,7 @@ struct Loader {
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
         const int row = (wave * kPer + j) * 8 + (lane >> 3);
-        voff[j] = (unsigned)min(row, last) * (unsigned)(o.ld * 2) + (unsigned)(((lane & 7) ^ (lane >> 3)) * 16);
+        voff[j] = (unsigned)min(row, last) * (unsigned)(o.ld * 2) + (unsigned)(((lane & 7) ^ shuffle(row)) * 16);
       }
       at = reinterpret_cast<uintptr_t>(o.base + (long long)row0 * o.ld);
       left = ((long long)last * o.ld + (long long)o.k * kWords) * 2;
@@ -91,42 +98,46 @@ struct Loader {
     left -= advance * step0;
   }
 
-  __device__ __forceinline__ void issue(unsigned lds, int wave) {
-    const long long l = left < 0 ? 0 : left;
+  // The descriptor of the stage that is due, empty for stages behind the last one: their pieces read nothing.
+  __device__ __forceinline__ srd_t begin(bool any) {
+    const long long l = !any || left < 0 ? 0 : left;
     const srd_t srd = make_srd(reinterpret_cast<const void*>(at), l > 0xffffffffLL ? 0xffffffffu : (unsigned)l);
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) dma_dwordx4(srd, lds + (unsigned)(wave * kPer + j) * 1024u, voff[j], 0u);
     at += advance;
     left -= advance;
+    return srd;
+  }
+  __device__ __forceinline__ void piece(const srd_t& srd, unsigned lds, int wave, int j) {
+    dma_dwordx4(srd, lds + (unsigned)(wave * kPer + j) * 1024u, voff[j], 0u);
   }
 };
 
-// WR x WC waves share the tile; each holds FM x FN fragments of 16 x 16.  acc[i][j][r] of lane l is the element
-// (row i * 16 + (l & 15), column j * 16 + (l >> 4) * 4 + r) of the wave's part: four consecutive columns per lane.
+// WR x WC waves share the tile; each holds FM x FN fragments of 32 x 32.  acc[i][j][4 g + r] of lane l is the element
+// (row i * 32 + (l & 31), column j * 32 + g * 8 + (l >> 5) * 4 + r) of the wave's part: four consecutive columns per lane and g.
 template <int BM_, int BN_, int WR_, int WC_, int STAGES_, bool SPLIT_, bool BF16_, bool AKM, bool BKM>
 struct TileProduct {
   static constexpr int BM = BM_, BN = BN_, WR = WR_, WC = WC_;
   static constexpr bool SPLIT = SPLIT_, BF16 = BF16_;
   static constexpr int kWaves = WR * WC, kThreads = kWaves * 64;
   static constexpr int kStep = SPLIT ? 32 : 64;
-  static constexpr int FM = BM / WR / 16, FN = BN / WC / 16;
+  static constexpr int FM = BM / WR / 32, FN = BN / WC / 32;
   static constexpr unsigned kABytes = BM * 128, kStage = (BM + BN) * 128;
   static constexpr int STAGES = STAGES_;
   static constexpr unsigned kLds = STAGES * kStage;
   using LoadA = Loader<BM, kWaves, SPLIT, AKM>;
   using LoadB = Loader<BN, kWaves, SPLIT, BKM>;
 
+  // rows row .. row + 31, k from 16 kk on (split: of the hi or the lo words); lane l holds row l & 31, k (l >> 5) * 8 .. + 7
   template <class L, bool KMAJOR>
   static __device__ __forceinline__ s16x8 fragment(lds_bytes tile, int row, int kk, int lo, int lane) {
     if constexpr (!KMAJOR) {
-      const int chunk = (SPLIT ? lo * 4 : kk * 4) + (lane >> 4);
+      const int chunk = lo * 4 + kk * 2 + (lane >> 5);
       return *reinterpret_cast<__attribute__((address_space(3))) const s16x8*>(
-          tile + (row + (lane & 15)) * 128 + ((chunk ^ (lane & 7)) << 4));
+          tile + (row + (lane & 31)) * 128 + ((chunk ^ L::shuffle(lane & 31)) << 4));
     } else {
-      const int i = lane & 15, k = kk * 32 + (lane >> 4) * 8 + (i >> 2);
-      const int unit = SPLIT ? (row >> 5) * 4 + lo * 2 + ((row >> 4) & 1) : row >> 4;
+      const int i = lane & 15, k = kk * 16 + (lane >> 5) * 8 + (i >> 2), col = row + (lane & 16);
+      const int unit = SPLIT ? (col >> 5) * 4 + lo * 2 + ((col >> 4) & 1) : col >> 4;
       lds_bytes p = tile + k * L::kRowBytes + ((unit ^ L::twist(k)) << 5) + (i & 3) * 8;
-      // rows k + 4 .. k + 7 of the same lane: the twist looks at bits 0, 1 (or 1) and 3 of k only; bit 2 is h
+      // rows k .. k + 3, then k + 4 .. k + 7 of the same lane: the twist does not look at bit 2 of k
       const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4*>(p));
       const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
           reinterpret_cast<__attribute__((address_space(3))) s16x4*>(p + 4 * L::kRowBytes));
@@ -134,93 +145,167 @@ struct TileProduct {
     }
   }
 
-  // the tile's sum over `steps` stages from stage `step0` on; ends with all waves past their last read of LDS
-  static __device__ __forceinline__ void run(f32x4 (&acc)[FM][FN], const Operand& a, const Operand& b, int row0, int col0,
+  // Fragments of a stage in two halves.  Plain: k 0..31 and k 32..63.  Split: the hi words, then the lo words.
+  struct Fragments {
+    s16x8 a[2][FM], b[2][FN];
+  };
+  static constexpr int kLoads = 2 * (FM + FN);                // fragments of a half
+  static constexpr int kProducts = 2 * FM * FN;               // matrix instructions of a half
+  static constexpr int kPieces = LoadA::kPer + LoadB::kPer;   // DMA pieces of a stage that a wave issues
+
+  struct Place {  // of this wave in the tile
+    int wm, wn, lane;
+  };
+  static __device__ __forceinline__ void load_a(Fragments& f, int k, int i, lds_bytes stage, int half, const Place& w) {
+    f.a[k][i] = fragment<LoadA, AKM>(stage, w.wm + i * 32, SPLIT ? k : half * 2 + k, SPLIT ? half : 0, w.lane);
+  }
+  static __device__ __forceinline__ void load_b(Fragments& f, int k, int j, lds_bytes stage, int half, const Place& w) {
+    f.b[k][j] = fragment<LoadB, BKM>(stage + kABytes, w.wn + j * 32, SPLIT ? k : half * 2 + k, SPLIT ? half : 0, w.lane);
+  }
+  // the half's n-th fragment, in the order in which products need them
+  static __device__ __forceinline__ void load(Fragments& f, int n, lds_bytes stage, int half, const Place& w) {
+    const int k = n / (FM + FN), m = n % (FM + FN);
+    if (m < FN)
+      load_b(f, k, m, stage, half, w);
+    else
+      load_a(f, k, m - FN, stage, half, w);
+  }
+
+  // One half's products; behind the n-th of them `between(n)` issues memory instructions.  A wave issues in order, and LDS reads and
+  // DMA pieces queue: in one bunch they would hold up the products behind them (64 KB of pieces take as long to issue
+  // as half a stage's products), one at a time they pass beside them.
+  template <class F>
+  static __device__ __forceinline__ void multiply(f32x16 (&acc)[FM][FN], const s16x8 (&a)[2][FM], const s16x8 (&b)[2][FN],
+                                                  F between) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+          acc[i][j] = mfma_32x32x16<BF16>(b[k][j], a[k][i], acc[i][j]);
+          between((k * FN + j) * FM + i);
+        }
+  }
+  static __device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0); }
+
+  // Behind product n, its share of LOADS fragment loads and PIECES DMA pieces, one of each in turn.
+  template <int LOADS, int PIECES, class L, class S>
+  static __device__ __forceinline__ void deal(int n, L load_one, S piece_one) {
+    constexpr int ops = LOADS + PIECES, each = (ops + kProducts - 1) / kProducts, both = LOADS < PIECES ? LOADS : PIECES;
+#pragma unroll
+    for (int e = 0; e < each; ++e) {
+      const int op = n * each + e;
+      if (op >= ops) continue;
+      if (op < 2 * both) {
+        if (op % 2 == 0)
+          piece_one(op / 2);
+        else
+          load_one(op / 2);
+      } else if (PIECES > LOADS) {
+        piece_one(op - both);
+      } else {
+        load_one(op - both);
+      }
+    }
+    if (n * each < ops) pin();
+  }
+
+  // the tile's sum over `steps` stages from stage `step0` on
+  static __device__ __forceinline__ void run(f32x16 (&acc)[FM][FN], const Operand& a, const Operand& b, int row0, int col0,
                                              int step0, int steps, lds_bytes lds) {
     const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
     const unsigned base = (unsigned)(uintptr_t)lds;
+    const Place w = {wave / WC * (BM / WR), wave % WC * (BN / WC), lane};
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j] = f32x16{};
     LoadA la;
     LoadB lb;
     la.init(a, row0, step0, wave, lane);
     lb.init(b, col0, step0, wave, lane);
-    const int wm = wave / WC * (BM / WR), wn = wave % WC * (BN / WC);
 #pragma unroll
-    for (int i = 0; i < FM; ++i)
+    for (int s = 0; s < STAGES; ++s) {
+      const srd_t sa = la.begin(s < steps), sb = lb.begin(s < steps);
 #pragma unroll
-      for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    constexpr int kAhead = (STAGES - 2) * (LoadA::kPer + LoadB::kPer);  // DMA of younger stages that may stay in flight
+      for (int j = 0; j < LoadA::kPer; ++j) la.piece(sa, base + s * kStage, wave, j);
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s)
-      if (s < steps) {
-        la.issue(base + s * kStage, wave);
-        lb.issue(base + s * kStage + kABytes, wave);
-      }
+      for (int j = 0; j < LoadB::kPer; ++j) lb.piece(sb, base + s * kStage + kABytes, wave, j);
+    }
+    Fragments now, rest;
+    wait_for_stage<(STAGES - 1) * kPieces>();
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) load(now, n, lds, 0, w);
     int slot = 0;
     for (int s = 0; s < steps; ++s) {
-      // this stage has landed, and this wave's reads of the last one have returned: its LDS may be overwritten
-      if (kAhead > 0 && s + STAGES - 2 < steps)
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kAhead) : "memory");
-      else
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      if (s + STAGES - 1 < steps) {
-        const unsigned next = base + (unsigned)(slot == 0 ? STAGES - 1 : slot - 1) * kStage;
-        la.issue(next, wave);
-        lb.issue(next + kABytes, wave);
-      }
-      const lds_bytes ta = lds + slot * kStage, tb = ta + kABytes;
+      const lds_bytes here = lds + slot * kStage;
+      const unsigned freed = base + slot * kStage;
       slot = slot == STAGES - 1 ? 0 : slot + 1;
-      if constexpr (SPLIT) {
-        s16x8 ah[FM], al[FM], bh[FN], bl[FN];
+      const lds_bytes next = lds + slot * kStage;  // behind the last stage: a buffer that is read and not used
+      asm volatile("" ::: "memory");
+      multiply(acc, now.a, now.b, [&](int n) {  // under it, the other half's fragments
+        constexpr int every = kProducts / kLoads > 1 ? kProducts / kLoads : 1, each = (kLoads + kProducts - 1) / kProducts;
+        if (n % every == 0) {
 #pragma unroll
-        for (int i = 0; i < FM; ++i) ah[i] = fragment<LoadA, AKM>(ta, wm + i * 16, 0, 0, lane);
-#pragma unroll
-        for (int j = 0; j < FN; ++j) bh[j] = fragment<LoadB, BKM>(tb, wn + j * 16, 0, 0, lane);
-#pragma unroll
-        for (int j = 0; j < FN; ++j) bl[j] = fragment<LoadB, BKM>(tb, wn + j * 16, 0, 1, lane);
-#pragma unroll
-        for (int i = 0; i < FM; ++i) al[i] = fragment<LoadA, AKM>(ta, wm + i * 16, 0, 1, lane);
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-          for (int j = 0; j < FN; ++j) acc[i][j] = mfma_16x16x32<BF16>(bh[j], ah[i], acc[i][j]);
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-          for (int j = 0; j < FN; ++j) acc[i][j] = mfma_16x16x32<BF16>(bl[j], ah[i], acc[i][j]);
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-          for (int j = 0; j < FN; ++j) acc[i][j] = mfma_16x16x32<BF16>(bh[j], al[i], acc[i][j]);
-      } else {
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-          s16x8 af[FM], bf[FN];
-#pragma unroll
-          for (int i = 0; i < FM; ++i) af[i] = fragment<LoadA, AKM>(ta, wm + i * 16, kk, 0, lane);
-#pragma unroll
-          for (int j = 0; j < FN; ++j) bf[j] = fragment<LoadB, BKM>(tb, wn + j * 16, kk, 0, lane);
-#pragma unroll
-          for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int j = 0; j < FN; ++j) acc[i][j] = mfma_16x16x32<BF16>(bf[j], af[i], acc[i][j]);
+          for (int e = 0; e < each; ++e)
+            if (n / every * each + e < kLoads) load(rest, n / every * each + e, here, 1, w);
+          pin();
         }
+      });
+      // the next stage has landed, and every wave has this one's fragments in registers: its LDS may be overwritten
+      wait_for_stage<(STAGES - 2) * kPieces>();
+      const srd_t sa = la.begin(s + STAGES < steps), sb = lb.begin(s + STAGES < steps);
+      const auto stage = [&](int n) {  // the n-th DMA piece of the stage that takes this one's place
+        if (n < LoadA::kPer)
+          la.piece(sa, freed, wave, n);
+        else if (n < kPieces)
+          lb.piece(sb, freed + kABytes, wave, n - LoadA::kPer);
+      };
+      if constexpr (SPLIT) {
+        multiply(acc, now.a, rest.b, [&](int n) {
+          constexpr int each = (kPieces + kProducts - 1) / kProducts;
+#pragma unroll
+          for (int e = 0; e < each; ++e) stage(n * each + e);
+          if (n * each < kPieces) pin();
+        });
+        asm volatile("" ::: "memory");
+        multiply(acc, rest.a, now.b, [&](int n) {  // now.a is free, now.b[k][j] after its last product
+          const int k = n / (FM * FN), j = n / FM % FN, i = n % FM;
+          if (j == 0) load_a(now, k, i, next, 0, w);
+          if (i == FM - 1) load_b(now, k, j, next, 0, w);
+          pin();
+        });
+      } else {
+        multiply(acc, rest.a, rest.b, [&](int n) {
+          deal<kLoads, kPieces>(n, [&](int m) { load(now, m, next, 0, w); }, stage);
+        });
       }
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    // a workgroup may not end, nor its LDS be used otherwise, while pieces are in flight
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  }
+
+  // Waits until at most `YOUNGER` of this wave's DMA pieces are in flight and its LDS reads have returned, then for the other waves.
+  template <int YOUNGER>
+  static __device__ __forceinline__ void wait_for_stage() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(YOUNGER) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   }
 
+  // columns 8 g .. 8 g + 3 from the lane's column of fragment j on
+  static __device__ __forceinline__ f32x4 quad(const f32x16& v, int g) {
+    return f32x4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
+  }
   // this lane's first row and column inside the tile
   static __device__ __forceinline__ int lane_row() {
     const int wave = uniform((int)(threadIdx.x >> 6));
-    return wave / WC * (BM / WR) + (threadIdx.x & 15);
+    return wave / WC * (BM / WR) + (threadIdx.x & 31);
   }
   static __device__ __forceinline__ int lane_col() {
     const int wave = uniform((int)(threadIdx.x >> 6));
-    return wave % WC * (BN / WC) + ((threadIdx.x >> 4) & 3) * 4;
+    return wave % WC * (BN / WC) + ((threadIdx.x >> 5) & 1) * 4;
   }
 };
 
@@ -234,6 +319,37 @@ __device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int ba
   const int high = min(band, tiles_m - b * band);
   tn = in / high;
   tm = b * band + in - tn * high;
+}
+
+template <bool SPLIT, bool BF16, bool AKM, bool BKM>
+using Tile256 = TileProduct<256, 256, 2, 2, 2, SPLIT, BF16, AKM, BKM>;
+template <bool SPLIT, bool BF16, bool AKM, bool BKM>
+using Tile128 = TileProduct<128, 128, 2, 2, 2, SPLIT, BF16, AKM, BKM>;
+template <bool SPLIT, bool BF16, bool AKM, bool BKM>
+using Tile64 = TileProduct<64, 64, 2, 2, 4, SPLIT, BF16, AKM, BKM>;
+// waves per SIMD that a kernel with this tile is compiled for
+template <class P>
+constexpr int kWavesPerSimd = P::BM == 256 ? 1 : 2;
+
+// What a stage of a launch takes, in us: one 256 tile fits a compute unit, two of the others do.  Measured on products from one tile per
+// unit up to 8192 x 8192; `alone` is a launch that leaves every second place empty.  In float32 terms the large
+// tile reaches 450 TFLOP/s there and the others 420 and 280, in bf16 1190, 1060 and 570.
+struct StageTime {
+  float alone, full;
+};
+inline float stage_us(int tile, bool split, long long tiles) {
+  const StageTime t = tile == 256   ? (split ? StageTime{1.7f, 2.4f} : StageTime{1.1f, 1.8f})
+                      : tile == 128 ? (split ? StageTime{0.58f, 1.28f} : StageTime{0.61f, 1.09f})
+                                    : (split ? StageTime{0.31f, 0.51f} : StageTime{0.29f, 0.51f});
+  const long long cus = compute_units(), places = tile == 256 ? cus : 2 * cus;
+  if (tiles <= places / 2) return t.alone;
+  const long long rounds = tiles / places, rest = tiles % places;
+  return rounds * t.full + (rest == 0 ? 0.f : rest <= places / 2 && tile != 256 ? t.alone : t.full);
+}
+// The tile side with the least estimated time for a launch with that many tiles of 256, 128 and 64.
+inline int choose_tile(long long t256, long long t128, long long t64, bool split) {
+  const float a = stage_us(256, split, t256), b = stage_us(128, split, t128), c = stage_us(64, split, t64);
+  return a <= b && a <= c ? 256 : b <= c ? 128 : 64;
 }
 
 }  // namespace
