@@ -153,6 +153,9 @@ def check(rc, what):
 def current_stream_handle(device):
     import torch
 
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # the same handle without building a Stream object (2 us)
+    if raw is not None and device.index is not None:
+        return ctypes.c_void_p(raw(device.index))
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 

@@ -31,7 +31,10 @@ constexpr int kPad = 64;              // rows and classes of the operands' k axe
 constexpr int kMaxParts = 1024;       // workgroups of the maximum's pass
 constexpr float kQScale = 16384.f;    // q is stored times 2^14: fp16 keeps probabilities down to 2^-38
 constexpr int kIgnored = -1, kOutside = -2;
-constexpr size_t kPieceBytes = size_t(256) << 20;  // q of one piece of the vocabulary
+constexpr int kIsNaN = 1 << 30;       // mark of a predicted class whose logit is NaN
+constexpr int kNoClass = kIsNaN - 1;
+constexpr float kLargest = 3.402823466e38f;
+constexpr size_t kPieceBytes = size_t(1) << 30;  // q of one piece of the vocabulary
 
 __device__ __forceinline__ float to_float(uint16_t v, bool bf16) {
   return bf16 ? __uint_as_float((unsigned)v << 16) : (float)__builtin_bit_cast(_Float16, v);
@@ -89,27 +92,37 @@ Plan make_plan(int rows, int dim, int classes, int dtype, bool w_in_place) {
   return p;
 }
 
-struct Scalars {      // at scalars_at
-  float scale_x, scale_w;  // powers of two
-  float inv_x, inv_w;
-  float count;             // rows that count, at least 1
+struct Scalars {        // at scalars_at
+  float inv_x, inv_w;   // what undoes the scales of features and weights, powers of two
+  float count;          // rows that count, at least 1
+  int done;             // workgroups of the join that are through
+};
+struct Sum {
+  double loss;
+  int rows;
 };
 
 // ---- laying out --------------------------------------------------------------------------------------------------------
 
 // 2^(14 - floor(log2 m)); 1 for zero and for what is no number
 __device__ __forceinline__ float scale_of(float m) {
-  if (!(m > 0.f) || m > 3.402823466e38f) return 1.f;
-  int e = 14 - ilogbf(m);
+  if (!(m > 0.f) || m > kLargest) return 1.f;
+  const int e = 14 - ilogbf(m);
   return ldexpf(1.f, min(max(e, -120), 120));
 }
 
-template <class LABEL>
-__device__ __forceinline__ bool ignored_row(const LABEL* labels, int row, long long ignore) {
-  return (long long)labels[row] == ignore;
+// Four float32 from `p`: one load where the row starts on 16 bytes (`aligned`), else one each; zeros behind `left` elements.
+__device__ __forceinline__ f32x4 four(const float* p, int left, bool aligned) {
+  if (aligned && left >= 4) return *reinterpret_cast<const f32x4*>(p);
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < left) v[e] = p[e];
+  return v;
 }
 
-// Largest finite magnitude of the features (blocks below `x_blocks`) and of the weights (the others): one value per block.
+// Largest finite magnitude of the features that count (blocks below `x_blocks`) and of the weights (the others): one value per
+// block.  A wave takes a row at a time.
 template <class LABEL>
 __global__ __launch_bounds__(256) void largest(const float* x, long long x_stride, const float* w, long long w_stride,
                                                const LABEL* labels, long long ignore, int rows, int classes, int dim,
@@ -120,13 +133,19 @@ __global__ __launch_bounds__(256) void largest(const float* x, long long x_strid
   const int n = is_x ? rows : classes, blocks = is_x ? x_blocks : gridDim.x - x_blocks;
   const int b = is_x ? blockIdx.x : blockIdx.x - x_blocks;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const bool aligned = reinterpret_cast<uintptr_t>(src) % 16 == 0 && stride % 4 == 0;
   float m = 0.f;
   for (int r = b * 4 + wave; r < n; r += blocks * 4) {
-    if (is_x && ignored_row(labels, r, ignore)) continue;
+    if (is_x && (long long)labels[r] == ignore) continue;
     const float* p = src + (long long)r * stride;
-    for (int c = lane; c < dim; c += 64) {
-      const float v = fabsf(p[c]);
-      if (v <= 3.402823466e38f) m = fmaxf(m, v);
+#pragma unroll 4
+    for (int c = lane * 4; c < dim; c += 256) {
+      const f32x4 v = four(p + c, dim - c, aligned);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float a = fabsf(v[e]);
+        m = a <= kLargest ? fmaxf(m, a) : m;
+      }
     }
   }
   for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
@@ -160,44 +179,50 @@ __global__ __launch_bounds__(256) void lay_out(const void* x, long long x_stride
     __syncthreads();
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) {
-    sc->scale_x = split ? scales[0] : 1.f, sc->scale_w = split ? scales[1] : 1.f;
-    sc->inv_x = 1.f / sc->scale_x, sc->inv_w = 1.f / sc->scale_w;
+    sc->inv_x = split ? 1.f / scales[0] : 1.f, sc->inv_w = split ? 1.f / scales[1] : 1.f;
+    sc->done = 0;
   }
   for (int i = blockIdx.x * 256 + threadIdx.x; i < rows_p; i += gridDim.x * 256) {
     const long long y = i < rows ? (long long)labels[i] : ignore;
     lab[i] = y == ignore ? kIgnored : (y >= 0 && y < classes) ? (int)y : kOutside;
   }
   const int total = rows_p + (wo != nullptr ? classes : 0);
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, bytes = split ? 4 : 2;
   for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < total; r += gridDim.x * 4) {
     const bool is_x = r < rows_p;
     const int row = is_x ? r : r - rows_p;
-    const bool zero = is_x && (row >= rows || ignored_row(labels, row, ignore));
-    const void* src = is_x ? x : w;
-    const long long from = (long long)row * (is_x ? x_stride : w_stride);
+    const bool zero = is_x && (row >= rows || (long long)labels[row] == ignore);
+    const char* src = static_cast<const char*>(is_x ? x : w) + (long long)row * (is_x ? x_stride : w_stride) * bytes;
+    const bool aligned = reinterpret_cast<uintptr_t>(src) % 16 == 0;
     uint16_t* to = (is_x ? xo : wo) + (long long)row * dim_p * (split ? 2 : 1);
     const float scale = split ? scales[is_x ? 0 : 1] : 1.f;
+#pragma unroll 2
     for (int c = lane * 8; c < dim_p; c += 512) {
       s16x8 hi = {0, 0, 0, 0, 0, 0, 0, 0}, lo = hi;
-      if (!zero) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c + e < dim) {
-            if constexpr (split) {
-              const float v = static_cast<const float*>(src)[from + c + e] * scale;
-              const _Float16 h = (_Float16)v;
-              hi[e] = __builtin_bit_cast(short, h);
-              lo[e] = (short)half_bits(v - (float)h);
-            } else {
-              hi[e] = static_cast<const short*>(src)[from + c + e];
-            }
-          }
-      }
       if constexpr (split) {
+        if (!zero) {
+          const float* p = reinterpret_cast<const float*>(src) + c;
+          const f32x4 v0 = four(p, dim - c, aligned), v1 = four(p + 4, dim - c - 4, aligned);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float v = (e < 4 ? v0[e & 3] : v1[e & 3]) * scale;
+            const _Float16 h = (_Float16)v;
+            hi[e] = __builtin_bit_cast(short, h);
+            lo[e] = (short)half_bits(v - (float)h);
+          }
+        }
         uint16_t* at = to + (c >> 5) * 64 + (c & 31);
         *reinterpret_cast<s16x8*>(at) = hi;
         *reinterpret_cast<s16x8*>(at + 32) = lo;
       } else {
+        const short* p = reinterpret_cast<const short*>(src) + c;
+        if (!zero && aligned && c + 8 <= dim) {
+          hi = *reinterpret_cast<const s16x8*>(p);
+        } else if (!zero) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (c + e < dim) hi[e] = p[e];
+        }
         *reinterpret_cast<s16x8*>(to + c) = hi;
       }
     }
@@ -210,22 +235,34 @@ struct Best {  // largest logit of a row and its lowest class; a NaN is the larg
   float v;
   int at;
 };
-__device__ __forceinline__ bool beats(float v, int at, const Best& b) {
-  const bool nv = v != v, nb = b.v != b.v;
-  if (nv != nb) return nv;
-  if (nv || v == b.v) return at < b.at;
-  return v > b.v;
+__device__ __forceinline__ bool beats(const Best& a, const Best& b) {
+  const bool na = a.v != a.v, nb = b.v != b.v;
+  if (na != nb) return na;
+  if (na || a.v == b.v) return a.at < b.at;
+  return a.v > b.v;
 }
 
 // A lane's e-th of the 16 columns of a fragment
 __device__ __forceinline__ constexpr int column(int e) { return (e >> 2) * 8 + (e & 3); }
 
+// The lane's biases; columns behind the last class get -inf, which takes them out of maximum, sum and gradient.
+template <class P, int T>
+__device__ __forceinline__ void load_bias(float (&b)[P::FN][16], const void* bias, int class0, int col0, int classes) {
+#pragma unroll
+  for (int j = 0; j < P::FN; ++j)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int col = col0 + j * 32 + column(e);
+      b[j][e] = col >= classes ? -INFINITY : bias != nullptr ? load_as_float<T>(bias, class0 + col) : 0.f;
+    }
+}
+
 // One tile of logits -> per row and strip of columns (one strip per wave column) the maximum and the sum of exp(z - max).
 template <class P, int T, bool PRED>
-__global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_forward(Operand x, Operand w, const void* bias, const int* lab,
-                                                              const Scalars* sc, int rows, int rows_p, int classes,
-                                                              int tiles_m, int tiles_n, int steps, float2* part, Best* best,
-                                                              float* target) {
+__global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_forward(Operand x, Operand w, const void* bias,
+                                                                                const int* lab, const Scalars* sc, int rows,
+                                                                                int rows_p, int classes, int tiles_m, int tiles_n,
+                                                                                int steps, float2* part, int* best, float* target) {
   extern __shared__ char smem[];
   int tm, tn;
   tile_of(blockIdx.x, tiles_m, tiles_n, 4, tm, tn);
@@ -234,142 +271,177 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_forward(
   const int row0 = tm * P::BM + P::lane_row(), col0 = tn * P::BN + P::lane_col();
   const float ix = P::SPLIT ? sc->inv_x : 1.f, iw = P::SPLIT ? sc->inv_w : 1.f;
   float b[P::FN][16];
-#pragma unroll
-  for (int j = 0; j < P::FN; ++j)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int col = col0 + j * 32 + column(r);
-      b[j][r] = (bias != nullptr && col < classes) ? load_as_float<T>(bias, col) : 0.f;
-    }
+  load_bias<P, T>(b, bias, 0, col0, classes);
   const int strip = tn * P::WC + uniform((int)(threadIdx.x >> 6)) % P::WC;
 #pragma unroll
   for (int i = 0; i < P::FM; ++i) {
     const int row = row0 + i * 32;
     const int y = row < rows ? lab[row] : kIgnored;
     float m = -INFINITY;
-    Best best_here = {-INFINITY, 0x7fffffff};
 #pragma unroll
     for (int j = 0; j < P::FN; ++j)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int col = col0 + j * 32 + column(r);
-        const float z = col < classes ? (P::SPLIT ? acc[i][j][r] * ix * iw : acc[i][j][r]) + b[j][r] : -INFINITY;
-        acc[i][j][r] = z;
-        m = fmaxf(m, z);
-        if (col == y) target[row] = z;
-        if (PRED && col < classes && beats(z, col, best_here)) best_here = {z, col};
+      for (int e = 0; e < 16; ++e) {
+        acc[i][j][e] = (P::SPLIT ? acc[i][j][e] * ix * iw : acc[i][j][e]) + b[j][e];
+        m = fmaxf(m, acc[i][j][e]);
       }
+    const int in = y - col0;  // the label's class among the wave's columns, from the lane's first one on
+    if (__any(in >= 0 && in < P::FN * 32)) {
+#pragma unroll
+      for (int j = 0; j < P::FN; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (in == j * 32 + column(e)) target[row] = acc[i][j][e];
+    }
     m = fmaxf(m, __shfl_xor(m, 32));
     const float from = m == -INFINITY ? 0.f : m;  // a strip of classes that are all masked sums to zero
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < P::FN; ++j)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s += __expf(acc[i][j][r] - from);
+      for (int e = 0; e < 16; ++e) s += __expf(acc[i][j][e] - from);
     s += __shfl_xor(s, 32);
+    const bool writes = row < rows && (threadIdx.x & 32) == 0;
+    if (writes) part[(long long)strip * rows_p + row] = make_float2(m, s);
     if constexpr (PRED) {
-      const Best o = {__shfl_xor(best_here.v, 32), __shfl_xor(best_here.at, 32)};
-      if (beats(o.v, o.at, best_here)) best_here = o;
-    }
-    if (row < rows && (threadIdx.x & 32) == 0) {
-      part[(long long)strip * rows_p + row] = make_float2(m, s);
-      if constexpr (PRED) best[(long long)strip * rows_p + row] = best_here;
+      int at = kNoClass;
+#pragma unroll
+      for (int j = P::FN - 1; j >= 0; --j)
+#pragma unroll
+        for (int e = 15; e >= 0; --e) at = acc[i][j][e] == m ? col0 + j * 32 + column(e) : at;
+      if (__any(s != s)) {  // the first NaN, where the row has one
+        int first = kNoClass;
+#pragma unroll
+        for (int j = P::FN - 1; j >= 0; --j)
+#pragma unroll
+          for (int e = 15; e >= 0; --e) {
+            const int col = col0 + j * 32 + column(e);
+            first = col < classes && acc[i][j][e] != acc[i][j][e] ? col : first;
+          }
+        const int other = min(first, __shfl_xor(first, 32));
+        if (other != kNoClass) at = other | kIsNaN;
+      }
+      at = min(at, __shfl_xor(at, 32));
+      if (writes) best[(long long)strip * rows_p + row] = at;
     }
   }
 }
 
-// Joins the strips of 16 rows: 16 threads a row.
-__global__ __launch_bounds__(256) void join_strips(const float2* part, const Best* best, int strips, const int* lab, int rows,
-                                                   int rows_p, const float* target, float* lse, float* losses, int64_t* pred) {
+// Joins the strips of 16 rows, 16 threads a row; the workgroup that comes last sums the rows' losses in their order.
+__global__ __launch_bounds__(256) void join_strips(const float2* part, const int* best, int strips, const int* lab, int rows,
+                                                   int rows_p, const float* target, float* lse, float* losses, int64_t* pred,
+                                                   int mean, float* loss, Sum* sums, Scalars* sc) {
   __shared__ float2 s[16][17];
   __shared__ Best sb[16][17];
+  __shared__ Sum total[16];
+  __shared__ int last;
   const int r = threadIdx.x & 15, p0 = threadIdx.x >> 4, row = blockIdx.x * 16 + r;
-  float m = -INFINITY, sum = 0.f;
-  Best b = {-INFINITY, 0x7fffffff};
+  const auto merge = [](float2& a, float2 v) {
+    const float n = fmaxf(a.x, v.x), from = n == -INFINITY ? 0.f : n;
+    a = make_float2(n, a.y * __expf(a.x - from) + v.y * __expf(v.x - from));
+  };
+  float2 a = make_float2(-INFINITY, 0.f);
+  Best b = {-INFINITY, kNoClass};
   if (row < rows) {
+#pragma unroll 4
     for (int p = p0; p < strips; p += 16) {
       const float2 v = part[(long long)p * rows_p + row];
-      const float n = fmaxf(m, v.x), from = n == -INFINITY ? 0.f : n;
-      sum = sum * __expf(m - from) + v.y * __expf(v.x - from);
-      m = n;
+      merge(a, v);
       if (best != nullptr) {
-        const Best o = best[(long long)p * rows_p + row];
-        if (beats(o.v, o.at, b)) b = o;
+        const int at = best[(long long)p * rows_p + row];
+        const Best o = {at & kIsNaN ? NAN : v.x, at & ~kIsNaN};
+        if (beats(o, b)) b = o;
       }
     }
   }
-  s[p0][r] = make_float2(m, sum);
+  s[p0][r] = a;
   sb[p0][r] = b;
   __syncthreads();
-  if (p0 != 0 || row >= rows_p) return;
-  for (int p = 1; p < 16; ++p) {
-    const float2 v = s[p][r];
-    const float n = fmaxf(m, v.x), from = n == -INFINITY ? 0.f : n;
-    sum = sum * __expf(m - from) + v.y * __expf(v.x - from);
-    m = n;
-    if (best != nullptr && beats(sb[p][r].v, sb[p][r].at, b)) b = sb[p][r];
+  if (p0 == 0) {
+    for (int p = 1; p < 16; ++p) {
+      merge(a, s[p][r]);
+      if (best != nullptr && beats(sb[p][r], b)) b = sb[p][r];
+    }
+    float mine = 0.f;
+    int y = kIgnored;
+    if (row < rows_p) {
+      y = lab[row];
+      const float l = y == kOutside ? NAN : a.x + logf(a.y);
+      lse[row] = y == kIgnored ? INFINITY : l;  // exp(z - inf) = 0: an ignored row has no gradient
+      if (row < rows) {
+        if (y != kIgnored) mine = y == kOutside ? NAN : l - target[row];
+        if (losses != nullptr) losses[row] = mine;
+        if (pred != nullptr) pred[row] = y == kIgnored ? -1 : b.at;
+      }
+    }
+    total[r] = {(double)mine, y != kIgnored};
   }
-  const int y = lab[row];
-  float l = m + logf(sum);
-  if (y == kOutside) l = NAN;
-  lse[row] = y == kIgnored ? 0.f : l;
-  if (row >= rows) return;
-  losses[row] = y == kIgnored ? 0.f : y == kOutside ? NAN : l - target[row];
-  if (pred != nullptr) pred[row] = y == kIgnored ? -1 : b.at;
-}
-
-// Sum and count of the rows; the mean divides by the count, at least 1.
-__global__ __launch_bounds__(1024) void sum_rows(const float* losses, const int* lab, int rows, int mean, float* loss,
-                                                 Scalars* sc) {
-  double sum = 0;
-  int n = 0;
-  for (int i = threadIdx.x; i < rows; i += 1024) sum += (double)losses[i], n += lab[i] != kIgnored;
-  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d), n += __shfl_xor(n, d);
-  __shared__ double ss[16];
-  __shared__ int sn[16];
-  if ((threadIdx.x & 63) == 0) ss[threadIdx.x >> 6] = sum, sn[threadIdx.x >> 6] = n;
+  if (loss == nullptr) return;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    Sum t = total[0];
+    for (int i = 1; i < 16; ++i) t.loss += total[i].loss, t.rows += total[i].rows;
+    __hip_atomic_store(&sums[blockIdx.x].loss, t.loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(&sums[blockIdx.x].rows, t.rows, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    last = __hip_atomic_fetch_add(&sc->done, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  Sum t = {0.0, 0};
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += 256) {
+    t.loss += __hip_atomic_load(&sums[i].loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    t.rows += __hip_atomic_load(&sums[i].rows, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  for (int d = 32; d; d >>= 1) t.loss += __shfl_xor(t.loss, d), t.rows += __shfl_xor(t.rows, d);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) total[threadIdx.x >> 6] = t;
   __syncthreads();
   if (threadIdx.x != 0) return;
-  for (int i = 1; i < 16; ++i) sum += ss[i], n += sn[i];
-  const float count = (float)max(n, 1);
-  sc->count = count;
-  *loss = (float)(mean ? sum / (double)max(n, 1) : sum);
+  for (int i = 1; i < 4; ++i) t.loss += total[i].loss, t.rows += total[i].rows;
+  const int count = max(t.rows, 1);
+  sc->count = (float)count;
+  *loss = (float)(mean ? t.loss / (double)count : t.loss);
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------------
 
-// What multiplies each row's q before it is rounded, and (behind the rows) what the finished sums are multiplied with.  A common gradient stays out
-// of q; gradients of single rows go into it, scaled by a power of two so that the largest of them fills the type.
-__global__ __launch_bounds__(1024) void row_factors(const float* grad, int reduction, const int* lab, int rows, int rows_p,
-                                                    float* factors, const Scalars* sc) {
-  float s = kQScale, f;
-  if (reduction == MI_REDUCTION_NONE) {
-    float m = 0.f;
-    for (int i = threadIdx.x; i < rows; i += 1024) {
-      const float v = fabsf(grad[i]);
-      if (lab[i] != kIgnored && v <= 3.402823466e38f) m = fmaxf(m, v);
-    }
-    for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-    __shared__ float sm[16];
-    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
-    __syncthreads();
-    for (int i = 0; i < 16; ++i) m = fmaxf(m, sm[i]);
-    s = scale_of(m) * 0.5f;
-    f = 1.f / s;
-  } else {
-    f = (reduction == MI_REDUCTION_MEAN ? grad[0] / sc->count : grad[0]) * (1.f / kQScale);
+// What the finished sums are multiplied with.  A common gradient stays out of q; gradients of single rows are in it already.
+struct Factor {
+  const float* grad;  // of the loss; NULL: the rows' factors are in use
+  const Scalars* sc;
+  const float* scale;  // [1], behind the rows' factors
+  int mean;
+};
+__device__ __forceinline__ float value(const Factor& f) {
+  if (f.grad == nullptr) return *f.scale;
+  return (f.mean ? *f.grad / f.sc->count : *f.grad) * (1.f / kQScale);
+}
+
+// Gradients of single rows, times a power of two so that the largest of them fills the type.
+__global__ __launch_bounds__(1024) void row_factors(const float* grad, const int* lab, int rows, int rows_p, float* factors) {
+  float m = 0.f;
+  for (int i = threadIdx.x; i < rows; i += 1024) {
+    const float v = fabsf(grad[i]);
+    if (lab[i] != kIgnored && v <= kLargest) m = fmaxf(m, v);
   }
-  for (int i = threadIdx.x; i < rows_p; i += 1024)
-    factors[i] = (i >= rows || lab[i] == kIgnored) ? 0.f : reduction == MI_REDUCTION_NONE ? grad[i] * s : s;
-  if (threadIdx.x == 0) factors[rows_p] = f;
+  for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+  __shared__ float sm[16];
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
+  __syncthreads();
+  for (int i = 0; i < 16; ++i) m = fmaxf(m, sm[i]);
+  const float s = scale_of(m) * 0.5f;
+  for (int i = threadIdx.x; i < rows_p; i += 1024) factors[i] = (i >= rows || lab[i] == kIgnored) ? 0.f : grad[i] * s;
+  if (threadIdx.x == 0) factors[rows_p] = 1.f / s;
 }
 
 // One tile of logits, again -> q times its row's factor; column sums for the bias gradient, one strip per wave row.
 template <class P, int T>
-__global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_backward(Operand x, Operand w, const void* bias, const int* lab,
-                                                               const float* lse, const float* factors, const Scalars* sc,
-                                                               int rows_p, int class0, int classes, int classes_p,
-                                                               int tiles_m, int tiles_n, int steps, uint16_t* q, float* sums) {
+__global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_backward(Operand x, Operand w, const void* bias,
+                                                                                 const int* lab, const float* lse,
+                                                                                 const float* factors, const Scalars* sc,
+                                                                                 int rows_p, int class0, int classes, int classes_p,
+                                                                                 int tiles_m, int tiles_n, int steps, uint16_t* q,
+                                                                                 float* sums) {
   extern __shared__ char smem[];
   int tm, tn;
   tile_of(blockIdx.x, tiles_m, tiles_n, 4, tm, tn);
@@ -379,20 +451,29 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_backward
   const float ix = P::SPLIT ? sc->inv_x : 1.f, iw = P::SPLIT ? sc->inv_w : 1.f;
   const long long ld = (long long)classes_p * (P::SPLIT ? 2 : 1);
   float b[P::FN][16], sum[P::FN][16];
+  load_bias<P, T>(b, bias, class0, col0, classes);
 #pragma unroll
   for (int j = 0; j < P::FN; ++j)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int col = col0 + j * 32 + column(r);
-      b[j][r] = (bias != nullptr && col < classes) ? load_as_float<T>(bias, class0 + col) : 0.f;
-      sum[j][r] = 0.f;
-    }
+    for (int e = 0; e < 16; ++e) sum[j][e] = 0.f;
 #pragma unroll
   for (int i = 0; i < P::FM; ++i) {
     const int row = row0 + i * 32;
     const bool in = row < rows_p;
-    const int y = in ? lab[row] : kIgnored;
-    const float l = in ? lse[row] : 0.f, f = in ? factors[row] : 0.f;
+    const int y = (in ? lab[row] : kIgnored) - class0 - col0;
+    const float l = in ? lse[row] : INFINITY;
+    const float f = factors != nullptr ? (in ? factors[row] : 0.f) : kQScale;
+#pragma unroll
+    for (int j = 0; j < P::FN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        acc[i][j][e] = __expf((P::SPLIT ? acc[i][j][e] * ix * iw : acc[i][j][e]) + b[j][e] - l) * f;
+    if (__any(y >= 0 && y < P::FN * 32)) {
+#pragma unroll
+      for (int j = 0; j < P::FN; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] -= y == j * 32 + column(e) ? f : 0.f;
+    }
 #pragma unroll
     for (int j = 0; j < P::FN; ++j)
 #pragma unroll
@@ -401,11 +482,8 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_backward
         s16x4 hi, lo;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int e = g * 4 + r;
-          const float z = (P::SPLIT ? acc[i][j][e] * ix * iw : acc[i][j][e]) + b[j][e];
-          float v = 0.f;
-          if (y != kIgnored && col + r < classes) v = (__expf(z - l) - (class0 + col + r == y ? 1.f : 0.f)) * f;
-          sum[j][e] += v;
+          const float v = acc[i][j][g * 4 + r];
+          sum[j][g * 4 + r] += v;
           if constexpr (P::SPLIT) {
             const _Float16 h = (_Float16)v;
             hi[r] = __builtin_bit_cast(short, h);
@@ -430,118 +508,171 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_backward
 #pragma unroll
   for (int j = 0; j < P::FN; ++j)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      float v = sum[j][r];
+    for (int e = 0; e < 16; ++e) {
+      float v = sum[j][e];
       for (int d = 1; d < 32; d <<= 1) v += __shfl_xor(v, d);
-      const int col = col0 + j * 32 + column(r);
+      const int col = col0 + j * 32 + column(e);
       if ((threadIdx.x & 31) == 0 && col < classes) sums[(long long)strip * classes_p + col] = v;
     }
 }
 
-template <int T>
-__global__ __launch_bounds__(256) void bias_gradient(const float* sums, int strips, int classes, int classes_p, const float* factor,
-                                                     void* out, int class0) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= classes) return;
-  float v = 0.f;
-  for (int s = 0; s < strips; ++s) v += sums[(long long)s * classes_p + c];
-  store_from_float<T>(out, class0 + c, v * *factor);
-}
+// One of the two products q W and q' x.  With one slice of the k axis the result goes out rounded; otherwise the slices'
+// float32 sums are kept (and added to those of the pieces before) and joined by join_slices in their order.
+struct Gradient {
+  Operand a, b;
+  int rows, cols, tiles_m, tiles_n, steps, per_slice;
+  void* out;
+  float* slices;
+  int add;
+};
+struct BiasGradient {
+  const float* sums;
+  int strips, classes, classes_p;
+  void* out;
+};
 
-// A gradient's tile: slice blockIdx.y of the k axis.  With one slice and one piece the result goes out rounded; otherwise
-// the slices' float32 sums are kept (and added to those of the pieces before) and joined by join_slices in their order.
 template <class P, int T, bool OF_WEIGHT>
-__global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void gradient_product(Operand a, Operand b, int rows, int cols, int tiles_m,
-                                                                int tiles_n, int steps, int per_slice, const Scalars* sc,
-                                                                const float* factor, void* out, float* slices, int add) {
-  extern __shared__ char smem[];
+__device__ __forceinline__ void gradient_tile(const Gradient& g, int id, const Factor& factor, lds_bytes lds) {
+  const int tiles = g.tiles_m * g.tiles_n, slice = id / tiles;
   int tm, tn;
-  tile_of(blockIdx.x, tiles_m, tiles_n, 4, tm, tn);
+  tile_of(id - slice * tiles, g.tiles_m, g.tiles_n, 4, tm, tn);
   f32x16 acc[P::FM][P::FN];
-  const int step0 = blockIdx.y * per_slice, n = min(per_slice, steps - step0);
-  P::run(acc, a, b, tm * P::BM, tn * P::BN, step0, n, (lds_bytes)smem);
+  const int step0 = slice * g.per_slice;
+  P::run(acc, g.a, g.b, tm * P::BM, tn * P::BN, step0, min(g.per_slice, g.steps - step0), lds);
   const int row0 = tm * P::BM + P::lane_row(), col0 = tn * P::BN + P::lane_col();
-  const float f = *factor * (P::SPLIT ? (OF_WEIGHT ? sc->inv_x : sc->inv_w) : 1.f);
-  const bool whole = (cols & 3) == 0;  // then every four columns of a lane are inside or outside together, and aligned
+  const float f = value(factor) * (P::SPLIT ? (OF_WEIGHT ? factor.sc->inv_x : factor.sc->inv_w) : 1.f);
+  const bool whole = (g.cols & 3) == 0;  // then every four columns of a lane are inside or outside together, and aligned
 #pragma unroll
   for (int i = 0; i < P::FM; ++i) {
     const int row = row0 + i * 32;
-    if (row >= rows) continue;
+    if (row >= g.rows) continue;
 #pragma unroll
     for (int j = 0; j < P::FN; ++j)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int col = col0 + j * 32 + g * 8;
-        if (col >= cols) continue;
-        f32x4 v = P::quad(acc[i][j], g);
-        if (slices != nullptr) {
-          float* at = slices + ((long long)blockIdx.y * rows + row) * cols + col;
+      for (int k = 0; k < 4; ++k) {
+        const int col = col0 + j * 32 + k * 8;
+        if (col >= g.cols) continue;
+        f32x4 v = P::quad(acc[i][j], k);
+        if (g.slices != nullptr) {
+          float* at = g.slices + ((long long)slice * g.rows + row) * g.cols + col;
           if (whole) {
-            if (add) v += *reinterpret_cast<const f32x4*>(at);
+            if (g.add) v += *reinterpret_cast<const f32x4*>(at);
             *reinterpret_cast<f32x4*>(at) = v;
           } else {
             for (int r = 0; r < 4; ++r)
-              if (col + r < cols) at[r] = add ? at[r] + v[r] : v[r];
+              if (col + r < g.cols) at[r] = g.add ? at[r] + v[r] : v[r];
           }
         } else {
           v *= f;
-          const long long at = (long long)row * cols + col;
+          const long long at = (long long)row * g.cols + col;
           if (whole && T == MI_TYPE_F32) {
-            *reinterpret_cast<f32x4*>(static_cast<float*>(out) + at) = v;
+            *reinterpret_cast<f32x4*>(static_cast<float*>(g.out) + at) = v;
           } else if (whole) {
             s16x4 h;
             for (int r = 0; r < 4; ++r) h[r] = (short)round16<T>(v[r]);
-            *reinterpret_cast<s16x4*>(static_cast<uint16_t*>(out) + at) = h;
+            *reinterpret_cast<s16x4*>(static_cast<uint16_t*>(g.out) + at) = h;
           } else {
             for (int r = 0; r < 4; ++r)
-              if (col + r < cols) store_from_float<T>(out, at + r, v[r]);
+              if (col + r < g.cols) store_from_float<T>(g.out, at + r, v[r]);
           }
         }
       }
   }
 }
 
-template <int T, bool OF_WEIGHT>
-__global__ __launch_bounds__(256) void join_slices(const float* slices, int n, long long count, const Scalars* sc,
-                                                   const float* factor, void* out) {
-  const float f = *factor * (T == MI_TYPE_F32 ? (OF_WEIGHT ? sc->inv_x : sc->inv_w) : 1.f);
-  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < count; i += gridDim.x * 256LL) {
+// All gradients of a piece in one launch: the tiles of q W, those of q' x, and the bias' columns, 64 a workgroup.
+template <class PX, class PW, int T>
+__global__ __launch_bounds__(PX::kThreads, kWavesPerSimd<PX>) void gradients(Gradient x, Gradient w, BiasGradient bias, int x_blocks,
+                                                                             int w_blocks, Factor factor) {
+  extern __shared__ char smem[];
+  const int id = blockIdx.x;
+  if (id < x_blocks) {
+    gradient_tile<PX, T, false>(x, id, factor, (lds_bytes)smem);
+  } else if (id < x_blocks + w_blocks) {
+    gradient_tile<PW, T, true>(w, id - x_blocks, factor, (lds_bytes)smem);
+  } else {
+    float* part = reinterpret_cast<float*>(smem);
+    const int c = (id - x_blocks - w_blocks) * 64 + (threadIdx.x & 63), at = threadIdx.x >> 6;
     float v = 0.f;
-    for (int s = 0; s < n; ++s) v += slices[s * count + i];
-    store_from_float<T>(out, i, v * f);
+    if (c < bias.classes)
+#pragma unroll 8
+      for (int s = at; s < bias.strips; s += PX::kThreads / 64) v += bias.sums[(long long)s * bias.classes_p + c];
+    part[threadIdx.x] = v;
+    __syncthreads();
+    if (at != 0 || c >= bias.classes) return;
+    for (int s = 1; s < PX::kThreads / 64; ++s) v += part[s * 64 + threadIdx.x];
+    store_from_float<T>(bias.out, c, v * value(factor));
+  }
+}
+
+// Sums the slices of up to two gradients, four elements a thread.
+struct Joined {
+  const float* slices;
+  int n;
+  long long count;
+  void* out;
+};
+template <int T>
+__global__ __launch_bounds__(256) void join_slices(Joined x, Joined w, int x_blocks, Factor factor) {
+  const bool is_x = (int)blockIdx.x < x_blocks;
+  const Joined& j = is_x ? x : w;
+  const int block = is_x ? blockIdx.x : blockIdx.x - x_blocks, blocks = is_x ? x_blocks : gridDim.x - x_blocks;
+  const float f = value(factor) * (T == MI_TYPE_F32 ? (is_x ? factor.sc->inv_w : factor.sc->inv_x) : 1.f);
+  const bool whole = (j.count & 3) == 0;
+  for (long long i = (block * 256LL + threadIdx.x) * 4; i < j.count; i += blocks * 1024LL) {
+    const int left = j.count - i < 4 ? (int)(j.count - i) : 4;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < j.n; ++s) v += four(j.slices + s * j.count + i, left, whole);
+    for (int r = 0; r < left; ++r) store_from_float<T>(j.out, i + r, v[r] * f);
   }
 }
 
 // ---- launching -----------------------------------------------------------------------------------------------------------
 
 // The tile of a product whose k axis stays whole.
-int tile_for(long long m, long long n, bool split) {
+int tile_for(long long m, long long n, int k, bool split) {
   const auto tiles = [&](int t) { return (long long)ceil_div(m, t) * ceil_div(n, t); };
-  return choose_tile(tiles(256), tiles(128), tiles(64), split);
+  return choose_tile(tiles(256), tiles(128), tiles(64), (float)k / (split ? 32 : 64), split);
 }
 
-// Tile and number of k slices of a gradient: the least estimated time, a join costing a launch and the slices' way to memory and
-// back.  A slice is at least 8 stages long.
+// Tile of both gradients' products and the slices of their k axes: the least estimated time.  A slice is at least 8 stages long;
+// a join costs a launch and its slices' way to memory and back (8 bytes an element at 4 TB/s).
 struct Cut {
-  int tile, slices;
+  int tile, x, w;
 };
-Cut cut_for(long long m, long long n, long long steps, bool split, bool must_join) {
-  Cut best = {64, 1};
+Cut cut_for(const Plan& p, int width, bool x_joined) {
+  const int step = p.split ? 32 : 64;
+  const long long xs = width / step, ws = p.rows_p / step;
+  Cut best = {64, 1, 1};
   float least = INFINITY;
-  for (int tile : {256, 128, 64})
-    for (long long s = 1; s == 1 || (s <= 64 && steps / s >= 8); s *= 2) {
-      const long long tiles = (long long)ceil_div(m, tile) * ceil_div(n, tile) * s;
-      const bool join = s > 1 || must_join;
-      const float us = stage_us(tile, split, tiles) * ceil_div(steps, s) + (join ? 3.f + 8e-6f * m * n * (s + 1) / 4 : 0.f);
-      if (us < least) least = us, best = {tile, (int)s};
-    }
+  for (int tile : {256, 128, 64}) {
+    const long long xt = (long long)ceil_div(p.rows, tile) * ceil_div(p.dim, tile), wt = (long long)ceil_div(width, tile) * ceil_div(p.dim, tile);
+    const TileTime t = tile_time(tile, p.split);
+    const long long places = tile_places(tile);
+    for (long long a = 1; a == 1 || (a <= 64 && xs / a >= 8); a *= 2)
+      for (long long b = 1; b == 1 || (b <= 64 && ws / b >= 8); b *= 2) {
+        const long long blocks = xt * a + wt * b, longest = xs / a > ws / b ? xs / a : ws / b;
+        float us = t.around + longest * t.alone;
+        if (blocks > places / 2) {  // the longest tile may begin when the others are half through
+          const float busy = (float)(xt * xs + wt * ws) / places * t.full + (float)blocks / places * t.around + 0.5f * longest * t.full;
+          us = us > busy ? us : busy;
+        }
+        const bool xj = x_joined || a > 1, wj = b > 1;
+        if (xj || wj) us += 4.f;
+        if (xj) us += 2e-6f * p.rows * p.dim * (a + 1);
+        if (wj) us += 2e-6f * width * p.dim * (b + 1);
+        if (us < least) least = us, best = {tile, (int)a, (int)b};
+      }
+  }
   return best;
 }
 
 struct Pieces {
   int n, width;  // of the vocabulary; width is a multiple of kPad
-  Cut x, w;
-  size_t q_at, sums_at, factors_at, slices_at, bytes;
+  Cut cut;
+  bool x_joined;
+  size_t q_at, sums_at, factors_at, x_at, w_at, bytes;
 };
 
 Pieces make_pieces(const Plan& p) {
@@ -552,31 +683,29 @@ Pieces make_pieces(const Plan& p) {
   c.n = ceil_div(p.classes, most);
   c.width = ceil_div(ceil_div(p.classes, c.n), kPad) * kPad;
   c.n = ceil_div(p.classes, c.width);
-  const int step = p.split ? 32 : 64;
-  c.x = cut_for(p.rows, p.dim, c.width / step, p.split, c.n > 1);
-  c.w = cut_for(c.width, p.dim, p.rows_p / step, p.split, false);
+  c.cut = cut_for(p, c.width, c.n > 1);
+  c.x_joined = c.n > 1 || c.cut.x > 1;
   size_t at = 0;
   c.q_at = at, at = up(at + (size_t)p.rows_p * c.width * words * 2);
   c.sums_at = at, at = up(at + (size_t)(ceil_div(p.rows_p, 64) * 2) * c.width * 4);
   c.factors_at = at, at = up(at + (size_t)(p.rows_p + 1) * 4);
-  const size_t xs = c.n > 1 || c.x.slices > 1 ? (size_t)c.x.slices * p.rows * p.dim * 4 : 0;
-  const size_t ws = c.w.slices > 1 ? (size_t)c.w.slices * c.width * p.dim * 4 : 0;
-  c.slices_at = at, at = up(at + xs) + up(ws);
+  c.x_at = at, at = up(at + (c.x_joined ? (size_t)c.cut.x * p.rows * p.dim * 4 : 0));
+  c.w_at = at, at = up(at + (c.cut.w > 1 ? (size_t)c.cut.w * c.width * p.dim * 4 : 0));
   c.bytes = at;
   return c;
 }
 
 struct ForwardRoom {
-  size_t parts_at, best_at, target_at, losses_at, max_at, bytes;
+  size_t parts_at, best_at, target_at, sums_at, max_at, bytes;
 };
 ForwardRoom make_room(const Plan& p, bool with_pred) {
   ForwardRoom f;
-  const size_t strips = (size_t)ceil_div(p.classes, tile_for(p.rows, p.classes, p.split)) * 2;
+  const size_t strips = (size_t)ceil_div(p.classes, tile_for(p.rows, p.classes, p.dim_p, p.split)) * 2;
   size_t at = 0;
   f.parts_at = at, at = up(at + strips * p.rows_p * sizeof(float2));
-  f.best_at = at, at = up(at + (with_pred ? strips * p.rows_p * sizeof(Best) : 0));
+  f.best_at = at, at = up(at + (with_pred ? strips * p.rows_p * sizeof(int) : 0));
   f.target_at = at, at = up(at + (size_t)p.rows_p * 4);
-  f.losses_at = at, at = up(at + (size_t)p.rows_p * 4);
+  f.sums_at = at, at = up(at + (size_t)(p.rows_p / 16) * sizeof(Sum));
   f.max_at = at, at = up(at + (size_t)2 * kMaxParts * 4);
   f.bytes = at;
   return f;
@@ -607,14 +736,14 @@ void lay_out_all(const Plan& p, const Call& c, float* maxima) {
   const LABEL* labels = static_cast<const LABEL*>(c.labels);
   int xb = 0, wb = 0;
   if constexpr (T == MI_TYPE_F32) {
-    xb = ceil_div(p.rows, 16), wb = ceil_div(p.classes, 16);
+    xb = ceil_div(p.rows, 4), wb = ceil_div(p.classes, 4);
     xb = xb > kMaxParts ? kMaxParts : xb, wb = wb > kMaxParts ? kMaxParts : wb;
     largest<LABEL><<<xb + wb, 256, 0, c.stream>>>(static_cast<const float*>(c.x), c.x_stride,
                                                   static_cast<const float*>(c.weight), c.w_stride, labels, c.ignore, p.rows,
                                                   p.classes, p.dim, xb, maxima);
   }
-  const int rows = p.rows_p + (p.copy_w ? p.classes : 0);
-  const int grid = ceil_div(rows, 4) < 4 * compute_units() ? ceil_div(rows, 4) : 4 * compute_units();
+  const int rows = p.rows_p + (p.copy_w ? p.classes : 0), most = 8 * compute_units();
+  const int grid = ceil_div(rows, 4) < most ? ceil_div(rows, 4) : most;
   lay_out<T, LABEL><<<grid, 256, 0, c.stream>>>(
       c.x, c.x_stride, c.weight, c.w_stride, labels, c.ignore, p.rows, p.rows_p, p.classes, p.dim, p.dim_p,
       reinterpret_cast<uint16_t*>(c.saved + p.x_at), p.copy_w ? reinterpret_cast<uint16_t*>(c.saved + p.w_at) : nullptr,
@@ -631,7 +760,7 @@ int launch_logits(const Plan& p, const Call& c, const ForwardRoom& f, bool with_
   kernel<<<tm * tn, P::kThreads, P::kLds, c.stream>>>(
       x, w, c.bias, reinterpret_cast<const int*>(c.saved + p.lab_at), reinterpret_cast<const Scalars*>(c.saved + p.scalars_at),
       p.rows, p.rows_p, p.classes, tm, tn, p.dim_p / P::kStep, reinterpret_cast<float2*>(c.room + f.parts_at),
-      reinterpret_cast<Best*>(c.room + f.best_at), reinterpret_cast<float*>(c.room + f.target_at));
+      reinterpret_cast<int*>(c.room + f.best_at), reinterpret_cast<float*>(c.room + f.target_at));
   return tn * P::WC;
 }
 
@@ -644,19 +773,16 @@ int forward(const Plan& p, const Call& c, float* loss, float* losses, int64_t* p
     lay_out_all<T, int64_t>(p, c, maxima);
   else
     lay_out_all<T, int32_t>(p, c, maxima);
-  const int tile = tile_for(p.rows, p.classes, split);
+  const int tile = tile_for(p.rows, p.classes, p.dim_p, split);
   const int strips = tile == 256   ? launch_logits<Tile256<split, bf16, false, false>, T>(p, c, f, pred != nullptr)
                      : tile == 128 ? launch_logits<Tile128<split, bf16, false, false>, T>(p, c, f, pred != nullptr)
                                    : launch_logits<Tile64<split, bf16, false, false>, T>(p, c, f, pred != nullptr);
-  float* per_row = losses != nullptr ? losses : reinterpret_cast<float*>(c.room + f.losses_at);
-  const int* lab = reinterpret_cast<const int*>(c.saved + p.lab_at);
-  join_strips<<<ceil_div(p.rows_p, 16), 256, 0, c.stream>>>(
-      reinterpret_cast<const float2*>(c.room + f.parts_at), pred ? reinterpret_cast<const Best*>(c.room + f.best_at) : nullptr,
-      strips, lab, p.rows, p.rows_p, reinterpret_cast<const float*>(c.room + f.target_at),
-      reinterpret_cast<float*>(c.saved + p.lse_at), per_row, pred);
-  if (c.reduction != MI_REDUCTION_NONE)
-    sum_rows<<<1, 1024, 0, c.stream>>>(per_row, lab, p.rows, c.reduction == MI_REDUCTION_MEAN, loss,
-                                     reinterpret_cast<Scalars*>(c.saved + p.scalars_at));
+  join_strips<<<p.rows_p / 16, 256, 0, c.stream>>>(
+      reinterpret_cast<const float2*>(c.room + f.parts_at), pred ? reinterpret_cast<const int*>(c.room + f.best_at) : nullptr,
+      strips, reinterpret_cast<const int*>(c.saved + p.lab_at), p.rows, p.rows_p,
+      reinterpret_cast<const float*>(c.room + f.target_at), reinterpret_cast<float*>(c.saved + p.lse_at), losses, pred,
+      c.reduction == MI_REDUCTION_MEAN, loss, reinterpret_cast<Sum*>(c.room + f.sums_at),
+      reinterpret_cast<Scalars*>(c.saved + p.scalars_at));
   return check_launch("mi_linear_cross_entropy_forward");
 }
 
@@ -669,19 +795,24 @@ int launch_q(const Plan& p, const Call& c, const Pieces& s, int class0, int clas
   allow_lds(logits_backward<P, T>, P::kLds);
   logits_backward<P, T><<<tm * tn, P::kThreads, P::kLds, c.stream>>>(
       x, w, c.bias, reinterpret_cast<const int*>(c.saved + p.lab_at), reinterpret_cast<const float*>(c.saved + p.lse_at),
-      reinterpret_cast<const float*>(c.room + s.factors_at), reinterpret_cast<const Scalars*>(c.saved + p.scalars_at), p.rows_p,
-      class0, classes, classes_p, tm, tn, p.dim_p / P::kStep, reinterpret_cast<uint16_t*>(c.room + s.q_at),
+      c.reduction == MI_REDUCTION_NONE ? reinterpret_cast<const float*>(c.room + s.factors_at) : nullptr,
+      reinterpret_cast<const Scalars*>(c.saved + p.scalars_at), p.rows_p, class0, classes, classes_p, tm, tn,
+      p.dim_p / P::kStep, reinterpret_cast<uint16_t*>(c.room + s.q_at),
       want_bias ? reinterpret_cast<float*>(c.room + s.sums_at) : nullptr);
   return tm * P::WR;
 }
 
-template <class P, int T, bool OF_WEIGHT>
-void launch_gradient(const Operand& a, const Operand& b, int rows, int cols, int steps, int slices, const Scalars* sc,
-                     const float* factor, void* out, float* room, int add, hipStream_t stream) {
-  const int tm = ceil_div(rows, P::BM), tn = ceil_div(cols, P::BN), per = ceil_div(steps, slices);
-  allow_lds(gradient_product<P, T, OF_WEIGHT>, P::kLds);
-  gradient_product<P, T, OF_WEIGHT><<<dim3(tm * tn, slices), P::kThreads, P::kLds, stream>>>(
-      a, b, rows, cols, tm, tn, steps, per, sc, factor, out, room, add);
+template <class PX, class PW, int T>
+void launch_gradients(Gradient x, Gradient w, const BiasGradient& b, const Cut& cut, const Factor& factor, hipStream_t stream) {
+  const auto blocks = [](Gradient& g, int slices) {
+    if (g.out == nullptr) return 0;
+    g.tiles_m = ceil_div(g.rows, PX::BM), g.tiles_n = ceil_div(g.cols, PX::BN), g.per_slice = ceil_div(g.steps, slices);
+    return g.tiles_m * g.tiles_n * slices;
+  };
+  const int nx = blocks(x, cut.x), nw = blocks(w, cut.w), nb = b.out != nullptr ? ceil_div(b.classes, 64) : 0;
+  if (nx + nw + nb == 0) return;
+  allow_lds(gradients<PX, PW, T>, PX::kLds);
+  gradients<PX, PW, T><<<nx + nw + nb, PX::kThreads, PX::kLds, stream>>>(x, w, b, nx, nw, factor);
 }
 
 template <int T>
@@ -691,65 +822,44 @@ int backward(const Plan& p, const Call& c, const float* grad, void* grad_x, void
   const Pieces s = make_pieces(p);
   const Scalars* sc = reinterpret_cast<const Scalars*>(c.saved + p.scalars_at);
   float* factors = reinterpret_cast<float*>(c.room + s.factors_at);
-  const float* factor = factors + p.rows_p;
-  row_factors<<<1, 1024, 0, c.stream>>>(grad, c.reduction, reinterpret_cast<const int*>(c.saved + p.lab_at), p.rows, p.rows_p,
-                                        factors, sc);
+  const bool by_row = c.reduction == MI_REDUCTION_NONE;
+  if (by_row)
+    row_factors<<<1, 1024, 0, c.stream>>>(grad, reinterpret_cast<const int*>(c.saved + p.lab_at), p.rows, p.rows_p, factors);
+  const Factor factor = {by_row ? nullptr : grad, sc, factors + p.rows_p, c.reduction == MI_REDUCTION_MEAN};
   const uint16_t* q = reinterpret_cast<const uint16_t*>(c.room + s.q_at);
   const long long ldw = weights_ld(p, c);
-  const bool x_joined = s.n > 1 || s.x.slices > 1;
-  float* x_room = reinterpret_cast<float*>(c.room + s.slices_at);
-  float* w_room = reinterpret_cast<float*>(c.room + s.slices_at + (x_joined ? up((size_t)s.x.slices * p.rows * p.dim * 4) : 0));
+  float* x_room = s.x_joined ? reinterpret_cast<float*>(c.room + s.x_at) : nullptr;
+  float* w_room = s.cut.w > 1 ? reinterpret_cast<float*>(c.room + s.w_at) : nullptr;
   for (int k = 0; k < s.n; ++k) {
     const int class0 = k * s.width, classes = p.classes - class0 < s.width ? p.classes - class0 : s.width;
     const int classes_p = ceil_div(classes, kPad) * kPad;
-    const int tile = tile_for(p.rows_p, classes_p, split);
-    const bool want_b = grad_b != nullptr;
+    const int tile = tile_for(p.rows_p, classes_p, p.dim_p, split);
+    const bool want_b = grad_b != nullptr, ends = k + 1 == s.n;
     const int strips =
         tile == 256   ? launch_q<Tile256<split, bf16, false, false>, T>(p, c, s, class0, classes, classes_p, want_b)
         : tile == 128 ? launch_q<Tile128<split, bf16, false, false>, T>(p, c, s, class0, classes, classes_p, want_b)
                       : launch_q<Tile64<split, bf16, false, false>, T>(p, c, s, class0, classes, classes_p, want_b);
-    if (grad_b != nullptr)
-      bias_gradient<T><<<ceil_div(classes, 256), 256, 0, c.stream>>>(reinterpret_cast<const float*>(c.room + s.sums_at), strips,
-                                                                   classes, classes_p, factor, grad_b, class0);
-    if (grad_x != nullptr) {
-      const Operand a = {q, (long long)classes_p * words, p.rows_p, classes_p};
-      const Operand b = {weights_of(p, c) + class0 * ldw, ldw, p.dim, classes};
-      // every piece has the same slices: a last, shorter piece leaves some of them empty
-      const int steps = classes_p / step;
-      float* room = x_joined ? x_room : nullptr;
-      if (s.x.tile == 256)
-        launch_gradient<Tile256<split, bf16, false, true>, T, false>(a, b, p.rows, p.dim, steps, s.x.slices, sc, factor, grad_x,
-                                                                     room, k > 0, c.stream);
-      else if (s.x.tile == 128)
-        launch_gradient<Tile128<split, bf16, false, true>, T, false>(a, b, p.rows, p.dim, steps, s.x.slices, sc, factor, grad_x,
-                                                                     room, k > 0, c.stream);
-      else
-        launch_gradient<Tile64<split, bf16, false, true>, T, false>(a, b, p.rows, p.dim, steps, s.x.slices, sc, factor, grad_x,
-                                                                    room, k > 0, c.stream);
-    }
-    if (grad_w != nullptr) {
-      const Operand a = {q, (long long)classes_p * words, classes_p, p.rows_p};
-      const Operand b = {reinterpret_cast<uint16_t*>(c.saved + p.x_at), p.ld, p.dim, p.rows_p};
-      void* out = static_cast<char*>(grad_w) + (size_t)class0 * p.dim * out_bytes;
-      float* room = s.w.slices > 1 ? w_room : nullptr;
-      if (s.w.tile == 256)
-        launch_gradient<Tile256<split, bf16, true, true>, T, true>(a, b, classes, p.dim, p.rows_p / step, s.w.slices, sc, factor,
-                                                                   out, room, 0, c.stream);
-      else if (s.w.tile == 128)
-        launch_gradient<Tile128<split, bf16, true, true>, T, true>(a, b, classes, p.dim, p.rows_p / step, s.w.slices, sc, factor,
-                                                                   out, room, 0, c.stream);
-      else
-        launch_gradient<Tile64<split, bf16, true, true>, T, true>(a, b, classes, p.dim, p.rows_p / step, s.w.slices, sc, factor,
-                                                                  out, room, 0, c.stream);
-      if (room != nullptr) {
-        const long long n = (long long)classes * p.dim;
-        join_slices<T, true><<<grid_for(n, 256), 256, 0, c.stream>>>(room, s.w.slices, n, sc, factor, out);
-      }
-    }
-  }
-  if (grad_x != nullptr && x_joined) {
-    const long long n = (long long)p.rows * p.dim;
-    join_slices<T, false><<<grid_for(n, 256), 256, 0, c.stream>>>(x_room, s.x.slices, n, sc, factor, grad_x);
+    // every piece has the same slices of q W: a last, shorter piece leaves some of them empty
+    const Gradient x = {{q, (long long)classes_p * words, p.rows_p, classes_p},
+                        {weights_of(p, c) + class0 * ldw, ldw, p.dim, classes},
+                        p.rows, p.dim, 0, 0, classes_p / step, 0, grad_x, x_room, k > 0};
+    void* w_out = grad_w == nullptr ? nullptr : static_cast<char*>(grad_w) + (size_t)class0 * p.dim * out_bytes;
+    const Gradient w = {{q, (long long)classes_p * words, classes_p, p.rows_p},
+                        {reinterpret_cast<uint16_t*>(c.saved + p.x_at), p.ld, p.dim, p.rows_p},
+                        classes, p.dim, 0, 0, p.rows_p / step, 0, w_out, w_room, 0};
+    const BiasGradient b = {reinterpret_cast<const float*>(c.room + s.sums_at), strips, classes, classes_p,
+                            want_b ? static_cast<char*>(grad_b) + (size_t)class0 * out_bytes : nullptr};
+    if (s.cut.tile == 256)
+      launch_gradients<Tile256<split, bf16, false, true>, Tile256<split, bf16, true, true>, T>(x, w, b, s.cut, factor, c.stream);
+    else if (s.cut.tile == 128)
+      launch_gradients<Tile128<split, bf16, false, true>, Tile128<split, bf16, true, true>, T>(x, w, b, s.cut, factor, c.stream);
+    else
+      launch_gradients<Tile64<split, bf16, false, true>, Tile64<split, bf16, true, true>, T>(x, w, b, s.cut, factor, c.stream);
+    const Joined jx = {x_room, s.cut.x, (long long)p.rows * p.dim, grad_x};
+    const Joined jw = {w_room, s.cut.w, (long long)classes * p.dim, w_out};
+    const int bx = ends && grad_x != nullptr && x_room != nullptr ? grid_for(jx.count / 4, 256) : 0;
+    const int bw = grad_w != nullptr && w_room != nullptr ? grid_for(jw.count / 4, 256) : 0;
+    if (bx + bw > 0) join_slices<T><<<bx + bw, 256, 0, c.stream>>>(jx, jw, bx, factor);
   }
   return check_launch("mi_linear_cross_entropy_backward");
 }

@@ -390,11 +390,13 @@ struct Dealt {
   Tiles tiles;
   int side;
 };
-template <class F>
-Dealt choose(const Table& t, F tiles_of) {
+template <class F, class G>
+Dealt choose(const Table& t, F tiles_of, G steps_of) {
   const Tiles a = deal(t, [&](const Mat& q) { return tiles_of(q, 256); }), b = deal(t, [&](const Mat& q) { return tiles_of(q, 128); }),
               c = deal(t, [&](const Mat& q) { return tiles_of(q, 64); });
-  const int side = choose_tile(a.first[t.count], b.first[t.count], c.first[t.count], true);
+  double stages = 0;
+  for (int i = 0; i < t.count; ++i) stages += (double)(c.first[i + 1] - c.first[i]) * steps_of(t.m[i]);
+  const int side = choose_tile(a.first[t.count], b.first[t.count], c.first[t.count], (float)(stages / c.first[t.count]), true);
   return {side == 256 ? a : side == 128 ? b : c, side};
 }
 
@@ -407,9 +409,11 @@ void iterate(const Table& t, const Step& s, int steps, char* ws, hipStream_t str
   momentum_and_norm<T><<<norm.first[t.count], 256, 0, stream>>>(t, norm, s, ws);
   const Tiles squares = deal(t, [](const Mat& q) { return div_up(q.m, 64) * div_up(q.n, 64); });
   normalize<T><<<squares.first[t.count], 256, 0, stream>>>(t, squares, norm, s, ws);
-  const Dealt g = choose(t, [](const Mat& q, int side) { return triangle_tiles(div_up(q.m, side)) * q.slices; });
-  const Dealt p = choose(t, [](const Mat& q, int side) { return triangle_tiles(div_up(q.m, side)); });
-  const Dealt f = choose(t, [](const Mat& q, int side) { return div_up(q.m, side) * div_up(q.n, side); });
+  const Dealt g = choose(t, [](const Mat& q, int side) { return triangle_tiles(div_up(q.m, side)) * q.slices; },
+                         [](const Mat& q) { return up32(q.n) / 32 / q.slices; });
+  const auto short_steps = [](const Mat& q) { return up32(q.m) / 32; };
+  const Dealt p = choose(t, [](const Mat& q, int side) { return triangle_tiles(div_up(q.m, side)); }, short_steps);
+  const Dealt f = choose(t, [](const Mat& q, int side) { return div_up(q.m, side) * div_up(q.n, side); }, short_steps);
   const Tiles joined = deal(t, [](const Mat& q) { return triangle_tiles(div_up(q.m, 64)); });
   for (int i = 0; i < steps; ++i) {
     const int flip = i & 1;

@@ -331,24 +331,28 @@ using Tile64 = TileProduct<64, 64, 2, 2, 4, SPLIT, BF16, AKM, BKM>;
 template <class P>
 constexpr int kWavesPerSimd = P::BM == 256 ? 1 : 2;
 
-// What a stage of a launch takes, in us: one 256 tile fits a compute unit, two of the others do.  Measured on products from one tile per
-// unit up to 8192 x 8192; `alone` is a launch that leaves every second place empty.  In float32 terms the large
-// tile reaches 450 TFLOP/s there and the others 420 and 280, in bf16 1190, 1060 and 570.
-struct StageTime {
-  float alone, full;
+// What a launch takes, in us: a stage of a tile where it shares its compute unit with nothing (`alone`) and where all places are taken
+// (`full`; one 256 tile fits a compute unit, two of the others do), and what is around a tile's stages.  Measured on products
+// from one tile up to 8192 x 8192; in float32 terms the tiles of 256, 128 and 64 reach 450, 420 and 280 TFLOP/s
+// there, in bf16 1190, 1060 and 570, and 1024 x 1204 x 1024 in bf16 takes 26, 11 and 9 us.
+struct TileTime {
+  float alone, full, around;
 };
-inline float stage_us(int tile, bool split, long long tiles) {
-  const StageTime t = tile == 256   ? (split ? StageTime{1.7f, 2.4f} : StageTime{1.1f, 1.8f})
-                      : tile == 128 ? (split ? StageTime{0.58f, 1.28f} : StageTime{0.61f, 1.09f})
-                                    : (split ? StageTime{0.31f, 0.51f} : StageTime{0.29f, 0.51f});
-  const long long cus = compute_units(), places = tile == 256 ? cus : 2 * cus;
-  if (tiles <= places / 2) return t.alone;
-  const long long rounds = tiles / places, rest = tiles % places;
-  return rounds * t.full + (rest == 0 ? 0.f : rest <= places / 2 && tile != 256 ? t.alone : t.full);
+inline TileTime tile_time(int tile, bool split) {
+  return tile == 256   ? (split ? TileTime{1.7f, 2.4f, 8.f} : TileTime{1.1f, 1.8f, 8.f})
+         : tile == 128 ? (split ? TileTime{0.58f, 1.28f, 3.f} : TileTime{0.61f, 1.09f, 3.f})
+                       : (split ? TileTime{0.31f, 0.51f, 2.f} : TileTime{0.29f, 0.51f, 2.f});
+}
+inline long long tile_places(int tile) { return (long long)compute_units() * (tile == 256 ? 1 : 2); }
+inline float launch_us(int tile, bool split, long long tiles, float steps) {
+  const TileTime t = tile_time(tile, split);
+  const long long places = tile_places(tile), rounds = tiles / places, rest = tiles % places;
+  const float last = rest == 0 ? 0.f : t.around + steps * (rest <= places / 2 ? t.alone : t.full);
+  return rounds * (t.around + steps * t.full) + last;
 }
 // The tile side with the least estimated time for a launch with that many tiles of 256, 128 and 64.
-inline int choose_tile(long long t256, long long t128, long long t64, bool split) {
-  const float a = stage_us(256, split, t256), b = stage_us(128, split, t128), c = stage_us(64, split, t64);
+inline int choose_tile(long long t256, long long t128, long long t64, float steps, bool split) {
+  const float a = launch_us(256, split, t256, steps), b = launch_us(128, split, t128, steps), c = launch_us(64, split, t64, steps);
   return a <= b && a <= c ? 256 : b <= c ? 128 : 64;
 }
 
