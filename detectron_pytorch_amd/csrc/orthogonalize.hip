@@ -1,31 +1,50 @@
 // orthogonalize.hip -- orthogonalised updates of weight matrices by Newton-Schulz products, and the optimiser step around them.
 //
 // Mathematics, for a matrix G [m, n] with m <= n (a taller one is turned first and turned back at the end):
-//   X_0 = G / max(|G|_F, eps);   A = X X',  B = b A + c A A,  X <- a X + B X     `steps` times
+//   X_0 = G / max(|G|_F, eps);   A = X X',  C = a I + b A + c A A,  X <- C X     `steps` times
 // X keeps the singular vectors of G and sends each singular value s to p(p(...p(s))) with p(s) = a s + b s^3 + c s^5, near 1 for
 // all but the smallest.  The step of the optimiser around it:
 //   M <- mu M + G,  U = G + mu M (nesterov) or M,  W <- (1 - lr wd) W - lr sqrt(max(1, rows / cols)) X(U)
 //
-// Work per iteration: m^2 n for A (upper triangle), m^3 for A A (upper triangle), 2 m^2 n for B X; all on the matrix cores
-// (tile_product.h).  X, A and B are kept as hi + lo fp16 times 2^12 (22 bits): their magnitudes are known -- |X| is bounded
-// by the polynomial's largest value, which the host checks -- so no pass looks for a scale.  Products of plain fp16 would lose the
-// small singular directions, whose noise the iteration amplifies by up to a^steps (485 for the usual a = 3.4445 and 5 steps).
-// Accumulators are float32; the norm is summed in fp64, so no gradient is too small or too large for it.
+// Two ways, by size:
 //
-// All matrices of a call go through each stage in one launch: a workgroup finds its matrix in the launch's table.
+// Short side up to 64 (and long side up to 16384): everything happens in the m x m space, in fp64.  A_0 = G G' / |G|^2 (the
+// norm is its trace), Q = product of the C_k with A_k+1 = C_k A_k C_k, result Q G / |G|: three launches, of which the second
+// is one workgroup per matrix with all its matrices in LDS.  A_0 has squared singular values, so float32 would not do.
+//
+// Larger: the products run on the matrix cores (tile_product.h) with X, A and C as hi + lo fp16 times a power of two (22
+// bits).  Their magnitudes are known -- |X| is bounded by the polynomial's largest value, which the host checks -- so no pass
+// looks for a scale.  Products of plain fp16 would lose the small singular directions, whose noise the iteration
+// amplifies by up to a^steps (485 for the usual a = 3.4445 and 5 steps).  Work per iteration: m^2 n for A (upper triangle), m^3
+// for A A (upper triangle), 2 m^2 n for C X.  Where n is a multiple of m, two or three iterations share one pass over the
+// long side: A_k+1 = C_k A_k C_k and Q = C_k+1 C_k are m x m products.  A pass in between renews A from X, which keeps the
+// error at that of separate iterations (2.1e-6 to 5.2e-6 of the norm against 2.1e-6 to 4.9e-6 on Gaussian and strongly
+// low-rank 256 x 1024; with all five in one pass 1e-4).
+//
+// Accumulators are float32; the norm is summed in fp64, so no gradient is too small or too large for it.
+// All matrices of a call go through each stage in one launch: a workgroup finds its matrix in the call's table.
 #include "common.h"
 #include "tile_product.h"
 
 #include <cmath>
+#include <cstring>
+#include <type_traits>
 
 namespace mi {
 namespace {
 
-constexpr int kMany = 32;            // matrices of one table (it is passed by value: 4 KB of kernel arguments)
-constexpr float kScale = 4096.f;     // X, A and B are stored times this
-constexpr double kMostMagnitude = 15.0;
-constexpr int kNormBlocks = 256;     // workgroups that sum one matrix' squares, at most
+constexpr int kMany = 32;            // matrices of one table (it goes to the first kernel by value: 4 KB of kernel arguments)
+constexpr float kScaleX = 4096.f;    // X is stored times this,
+constexpr float kScaleA = 8192.f;    // A and C A times this,
+constexpr float kScaleC = 1024.f;    // C and products of several C times this
+constexpr double kMostX = 2.8;       // bounds of |X| and of |C_k ... C_1| that keep the stored forms below 65504
+constexpr double kMostC = 60.0;
+constexpr int kNormBlocks = 1024;    // workgroups that sum one matrix' squares, at most
 constexpr int kNormElements = 8192;  // elements for which one more workgroup is worth its launch
+constexpr int kNarrow = 64, kNarrowLong = 16384;
+constexpr int kParts = 32;           // partial sums of A_0 in the fp64 way, at most
+
+enum { kA = 0, kC = 1, kQ = 2, kT = 3, kSquares = 4 };
 
 struct Mat {
   const void* grad;
@@ -33,12 +52,14 @@ struct Mat {
   float* momentum;   // NULL: no momentum
   int m, n;          // m <= n, after turning
   int tall;          // the matrix itself is [n, m]
-  int slices;        // of the sum over n in A
+  int slices;        // of the sum over n in A (fp64 way: partial sums)
   float shape;       // sqrt(max(1, rows / cols))
-  long long norm_at, x_at, y_at, a_at, b_at, c_at;  // bytes into the workspace
+  int pad;
+  long long norm_at, x_at, y_at, square_at, square_bytes, parts_at;  // bytes into the workspace
 };
 struct Table {
   int count;
+  int pad;
   Mat m[kMany];
 };
 struct Tiles {       // first workgroup of each matrix in a launch
@@ -48,14 +69,16 @@ struct Tiles {       // first workgroup of each matrix in a launch
 struct Step {
   float a, b, c, eps;
   float mu, lr, decay;  // decay = 1 - lr * weight decay
-  int nesterov, update;
+  int nesterov, update, steps;
 };
+
+using f64x4 = __attribute__((ext_vector_type(4))) double;
 
 __host__ __device__ inline int div_up(int a, int b) { return (a + b - 1) / b; }
 __host__ __device__ inline int up32(int v) { return (v + 31) & ~31; }
 
 __device__ __forceinline__ int find(const Tiles& t, int count, int block) {
-  int i = 0;
+  int i = 0;  // matrices without a workgroup in this launch are passed over
   while (i + 1 < count && block >= t.first[i + 1]) ++i;
   return i;
 }
@@ -75,6 +98,26 @@ __device__ __forceinline__ void store_float(void* p, long long i, float v) {
   else
     static_cast<__bf16*>(p)[i] = (__bf16)v;
 }
+// four elements from i on; `whole`: all four exist and lie on their own alignment
+template <int T>
+__device__ __forceinline__ f32x4 load_four(const void* p, long long i, int left, bool whole) {
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (whole && left >= 4) {
+    if constexpr (T == MI_TYPE_F32) return *reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + i);
+    const s16x4 h = *reinterpret_cast<const s16x4*>(static_cast<const uint16_t*>(p) + i);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const short one = h[r];
+      v[r] = load_float<T>(&one, 0);
+    }
+    return v;
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (r < left) v[r] = load_float<T>(p, i + r);
+  return v;
+}
+__device__ __forceinline__ bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // element (row, col) of a split matrix with `ld` elements a row: its hi word, the lo one is 32 words on
 __device__ __forceinline__ long long split_at(int row, int col, int ld) {
@@ -105,30 +148,261 @@ __device__ __forceinline__ void put_split4(uint16_t* p, f32x4 v) {
   *reinterpret_cast<s16x4*>(p + 32) = l;
 }
 
-// ---- momentum, norm, X_0 -------------------------------------------------------------------------------------------------
-
-template <int T>
-__device__ __forceinline__ float update_of(const Mat& q, const Step& s, long long i, float momentum) {
-  if (q.momentum == nullptr) return load_float<T>(q.grad, i);
-  return s.nesterov ? load_float<T>(q.grad, i) + s.mu * momentum : momentum;
+// The first kernel of a call has the table in its arguments and leaves it in the workspace for the others.
+__device__ __forceinline__ void leave_table(const Table& t, char* ws) {
+  if (blockIdx.x != 0) return;
+  const int* from = reinterpret_cast<const int*>(&t);
+  int* to = reinterpret_cast<int*>(ws);
+  for (int i = threadIdx.x; i < (int)(sizeof(Table) / 4); i += blockDim.x) to[i] = from[i];
 }
+__device__ __forceinline__ const Table& table_of(const char* ws) { return *reinterpret_cast<const Table*>(ws); }
+constexpr size_t kTableBytes = (sizeof(Table) + 255) / 256 * 256;
+
+// M <- mu M + G in place where there is a momentum; the update U.
+template <int T>
+__device__ __forceinline__ float advance(const Mat& q, const Step& s, long long i) {
+  const float g = load_float<T>(q.grad, i);
+  if (q.momentum == nullptr) return g;
+  const float m = s.mu * q.momentum[i] + g;
+  q.momentum[i] = m;
+  return s.nesterov ? g + s.mu * m : m;
+}
+// U once M is new
+template <int T>
+__device__ __forceinline__ float update_of(const Mat& q, const Step& s, long long i) {
+  if (q.momentum == nullptr) return load_float<T>(q.grad, i);
+  const float m = q.momentum[i];
+  return s.nesterov ? load_float<T>(q.grad, i) + s.mu * m : m;
+}
+template <int T>
+__device__ __forceinline__ void put_result(const Mat& q, const Step& s, long long i, float o) {
+  store_float<T>(q.out, i, s.update ? load_float<T>(q.out, i) * s.decay - s.lr * q.shape * o : o);
+}
+
+// four of them, on their alignment
+template <int T>
+__device__ __forceinline__ void put_result4(const Mat& q, const Step& s, long long i, f32x4 o) {
+  if (s.update) o = load_four<T>(q.out, i, 4, true) * s.decay - (s.lr * q.shape) * o;
+  if constexpr (T == MI_TYPE_F32) {
+    *reinterpret_cast<f32x4*>(static_cast<float*>(q.out) + i) = o;
+  } else {
+    s16x4 h;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      short one;
+      store_float<T>(&one, 0, o[r]);
+      h[r] = one;
+    }
+    *reinterpret_cast<s16x4*>(static_cast<uint16_t*>(q.out) + i) = h;
+  }
+}
+
+// ---- the fp64 way for a short side up to 64 ------------------------------------------------------------------------------
+
+constexpr int kLdU = 66;  // LDS row of 64 columns of U, doubles
+constexpr int kLdM = 66;  // LDS row of an m x m matrix
+
+// 64 columns of U from column `col0` of the long side on, as doubles; rows and columns behind the matrix are zeros.
+template <int T, bool ADVANCE>
+__device__ __forceinline__ void load_columns(const Mat& q, const Step& s, int col0, double (*u)[kLdU]) {
+  const int rows = (q.m + 15) & ~15;
+#pragma unroll 8
+  for (int e = threadIdx.x; e < rows * 64; e += 256) {
+    const int i = q.tall ? e % rows : e >> 6, j = q.tall ? e / rows : e & 63;
+    float v = 0.f;
+    if (i < q.m && col0 + j < q.n) {
+      const long long at = q.tall ? (long long)(col0 + j) * q.m + i : (long long)i * q.n + col0 + j;
+      v = ADVANCE ? advance<T>(q, s, at) : update_of<T>(q, s, at);
+    }
+    u[i][j] = (double)v;
+  }
+}
+
+// tile `id` of the upper triangle of n x n tiles, row by row
+__device__ __forceinline__ void triangle(int id, int n, int& i, int& j) {
+  i = 0;
+  while (id >= n - i) id -= n - i, ++i;
+  j = i + id;
+}
+__host__ __device__ inline int triangle_tiles(int n) { return n * (n + 1) / 2; }
+
+// Partial sums of U U': a workgroup adds up its share of 64-column chunks, each wave its tiles of the upper triangle (16 x 16;
+// a lane holds column l & 15, rows (l >> 4) + 4 r) and writes them as they lie in its registers.
+template <int T>
+__global__ __launch_bounds__(256) void narrow_gram(Table t, Tiles tiles, Step s, char* ws) {
+  leave_table(t, ws);
+  const int k = find(tiles, t.count, blockIdx.x);
+  const Mat& q = t.m[k];
+  __shared__ double u[kNarrow][kLdU];
+  const int part = blockIdx.x - tiles.first[k], chunks = div_up(q.n, 64), each = div_up(chunks, q.slices);
+  const int nt = div_up(q.m, 16), total = triangle_tiles(nt), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  f64x4 acc[3] = {};
+  for (int c = part * each; c < min(chunks, (part + 1) * each); ++c) {
+    __syncthreads();
+    load_columns<T, true>(q, s, c * 64, u);
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < 3; ++x) {
+      const int id = wave + x * 4;
+      if (id >= total) continue;
+      int i, j;
+      triangle(id, nt, i, j);
+      const double *a = &u[i * 16 + (lane & 15)][lane >> 4], *b = &u[j * 16 + (lane & 15)][lane >> 4];
+#pragma unroll
+      for (int p = 0; p < 64; p += 4) acc[x] = __builtin_amdgcn_mfma_f64_16x16x4f64(a[p], b[p], acc[x], 0, 0, 0);
+    }
+  }
+  f64x4* out = reinterpret_cast<f64x4*>(ws + q.parts_at) + (long long)part * total * 64;
+#pragma unroll
+  for (int x = 0; x < 3; ++x)
+    if (wave + x * 4 < total) out[(wave + x * 4) * 64 + lane] = acc[x];
+}
+
+// Symmetric product of commuting symmetric matrices in LDS, one tile of the upper triangle per wave; `put(i, j, v)` gets each element of the upper triangle's tiles.
+template <class F>
+__device__ __forceinline__ void narrow_product(const double (*x)[kLdM], const double (*y)[kLdM], int nt, F put) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (wave >= triangle_tiles(nt)) return;
+  int i, j;
+  triangle(wave, nt, i, j);
+  const double *a = &x[i * 16 + (lane & 15)][lane >> 4], *b = &y[j * 16 + (lane & 15)][lane >> 4];
+  f64x4 acc = {};
+  for (int p = 0; p < nt * 16; p += 16) {
+    double u[4], v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) u[k] = a[p + 4 * k], v[k] = b[p + 4 * k];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(u[k], v[k], acc, 0, 0, 0);
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) put(i * 16 + (lane >> 4) + 4 * r, j * 16 + (lane & 15), acc[r]);
+}
+
+// Q / max(|G|, eps) of one matrix per workgroup.
+constexpr int kPolyThreads = 640;  // ten tiles of 16 x 16 make the upper triangle of 64 x 64
+__global__ __launch_bounds__(kPolyThreads) void narrow_polynomial(Step s, char* ws) {
+  const Mat& q = table_of(ws).m[blockIdx.x];
+  extern __shared__ char smem[];
+  using Square = double (*)[kLdM];
+  const int nt = div_up(q.m, 16), total = triangle_tiles(nt), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const size_t bytes = sizeof(double) * kNarrow * kLdM;
+  Square a = reinterpret_cast<Square>(smem), c = reinterpret_cast<Square>(smem + bytes),
+         p = reinterpret_cast<Square>(smem + 2 * bytes), t = reinterpret_cast<Square>(smem + 3 * bytes);
+  const f64x4* parts = reinterpret_cast<const f64x4*>(ws + q.parts_at);
+  if (wave < total) {
+    f64x4 v = {};
+#pragma unroll 8
+    for (int k = 0; k < q.slices; ++k) v += parts[((long long)k * total + wave) * 64 + lane];
+    int i, j;
+    triangle(wave, nt, i, j);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = i * 16 + (lane >> 4) + 4 * r, col = j * 16 + (lane & 15);
+      a[row][col] = v[r];
+      if (i != j) a[col][row] = v[r];
+    }
+  }
+  __syncthreads();
+  double trace = 0;
+  for (int i = 0; i < q.m; ++i) trace += a[i][i];
+  const double length = sqrt(trace);
+  const double inv = 1.0 / (length < (double)s.eps ? (double)s.eps : length);  // not fmax: a NaN stays one
+  __syncthreads();
+  for (int e = threadIdx.x; e < nt * 16 * nt * 16; e += kPolyThreads) a[e / (nt * 16)][e % (nt * 16)] *= inv * inv;
+  __syncthreads();
+  const auto both = [](Square to) {
+    return [to](int i, int j, double v) {
+      to[i][j] = v;
+      if ((i >> 4) != (j >> 4)) to[j][i] = v;
+    };
+  };
+  for (int k = 0; k < s.steps; ++k) {
+    const Square poly = k == 0 ? p : c;
+    const auto put = both(poly);
+    narrow_product(a, a, nt, [&](int i, int j, double v) {
+      put(i, j, (i == j ? (double)s.a : 0.0) + (double)s.b * a[i][j] + (double)s.c * v);
+    });
+    __syncthreads();
+    if (k > 0) {
+      narrow_product(c, p, nt, both(t));
+      __syncthreads();
+      const Square old = p;
+      p = t, t = old;
+    }
+    if (k + 1 == s.steps) break;
+    const Square now = k == 0 ? p : c;
+    narrow_product(now, a, nt, both(t));
+    __syncthreads();
+    narrow_product(t, now, nt, both(a));
+    __syncthreads();
+  }
+  double* out = reinterpret_cast<double*>(ws + q.square_at);
+  for (int e = threadIdx.x; e < nt * 16 * nt * 16; e += kPolyThreads) out[e] = p[e / (nt * 16)][e % (nt * 16)] * inv;
+}
+
+// Q U, 64 columns per workgroup.
+template <int T>
+__global__ __launch_bounds__(256) void narrow_apply(Tiles tiles, Step s, char* ws) {
+  const Table& t = table_of(ws);
+  const int k = find(tiles, t.count, blockIdx.x);
+  const Mat& q = t.m[k];
+  __shared__ double u[kNarrow][kLdU], w[kNarrow][kLdM];
+  const int nt = div_up(q.m, 16), col0 = (blockIdx.x - tiles.first[k]) * 64, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  load_columns<T, false>(q, s, col0, u);
+  const double* in = reinterpret_cast<const double*>(ws + q.square_at);
+#pragma unroll 8
+  for (int e = threadIdx.x; e < nt * 16 * nt * 16; e += 256) w[e / (nt * 16)][e % (nt * 16)] = in[e];
+  __syncthreads();
+  const int j0 = wave * 16;  // 16 columns a wave
+  for (int i = 0; i < nt; ++i) {
+    f64x4 acc = {};
+    // the matrix' own order of elements decides which side lies along the lanes; Q is symmetric
+    for (int p = 0; p < nt * 16; p += 16) {
+      double x[4], y[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        x[k] = w[p + 4 * k + (lane >> 4)][i * 16 + (lane & 15)], y[k] = u[p + 4 * k + (lane >> 4)][j0 + (lane & 15)];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        acc = q.tall ? __builtin_amdgcn_mfma_f64_16x16x4f64(y[k], x[k], acc, 0, 0, 0)
+                     : __builtin_amdgcn_mfma_f64_16x16x4f64(x[k], y[k], acc, 0, 0, 0);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int d = (lane >> 4) + 4 * r, row = i * 16 + (q.tall ? lane & 15 : d), col = col0 + j0 + (q.tall ? d : lane & 15);
+      if (row < q.m && col < q.n)
+        put_result<T>(q, s, q.tall ? (long long)col * q.m + row : (long long)row * q.n + col, (float)acc[r]);
+    }
+  }
+}
+
+// ---- larger matrices: momentum, norm, X_0 --------------------------------------------------------------------------------
 
 // M <- mu M + G, and the squares of U: one fp64 sum per workgroup.
 template <int T>
 __global__ __launch_bounds__(256) void momentum_and_norm(Table t, Tiles tiles, Step s, char* ws) {
+  leave_table(t, ws);
   const int k = find(tiles, t.count, blockIdx.x);
   const Mat& q = t.m[k];
   const int block = blockIdx.x - tiles.first[k], blocks = tiles.first[k + 1] - tiles.first[k];
   const long long n = (long long)q.m * q.n;
+  const bool whole = aligned16(q.grad) && aligned16(q.momentum);
   double sum = 0;
-  for (long long i = block * 256LL + threadIdx.x; i < n; i += blocks * 256LL) {
-    float m = 0.f;
+#pragma unroll 2
+  for (long long i = (block * 256LL + threadIdx.x) * 4; i < n; i += blocks * 1024LL) {
+    const int left = n - i < 4 ? (int)(n - i) : 4;
+    f32x4 u = load_four<T>(q.grad, i, left, whole);
     if (q.momentum != nullptr) {
-      m = s.mu * q.momentum[i] + load_float<T>(q.grad, i);
-      q.momentum[i] = m;
+      const f32x4 m = s.mu * load_four<MI_TYPE_F32>(q.momentum, i, left, whole) + u;
+      if (whole && left == 4) {
+        *reinterpret_cast<f32x4*>(q.momentum + i) = m;
+      } else {
+        for (int r = 0; r < left; ++r) q.momentum[i + r] = m[r];
+      }
+      u = s.nesterov ? u + s.mu * m : m;
     }
-    const double u = (double)update_of<T>(q, s, i, m);
-    sum += u * u;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sum += r < left ? (double)u[r] * (double)u[r] : 0.0;
   }
   for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
   __shared__ double part[4];
@@ -139,13 +413,31 @@ __global__ __launch_bounds__(256) void momentum_and_norm(Table t, Tiles tiles, S
 
 // X_0, 64 x 64 of the given matrix per workgroup, turned on the way if it is tall.
 template <int T>
-__global__ __launch_bounds__(256) void normalize(Table t, Tiles tiles, Tiles norm, Step s, char* ws) {
+__global__ __launch_bounds__(256) void normalize(Tiles tiles, Tiles norm, Step s, char* ws) {
+  const Table& t = table_of(ws);
   const int k = find(tiles, t.count, blockIdx.x);
   const Mat& q = t.m[k];
   const int rows = q.tall ? q.n : q.m, cols = q.tall ? q.m : q.n;
   const int tiles_c = div_up(cols, 64), tile = blockIdx.x - tiles.first[k];
   const int row0 = tile / tiles_c * 64, col0 = tile % tiles_c * 64;
   __shared__ double part[4];
+  __shared__ float buf[64][68];
+  const bool whole = aligned16(q.grad) && aligned16(q.momentum) && cols % 4 == 0;
+  f32x4 u[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int r = row0 + e * 16 + (threadIdx.x >> 4), c = col0 + (threadIdx.x & 15) * 4;
+    u[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (r < rows && c < cols) {
+      const long long i = (long long)r * cols + c;
+      const int left = cols - c < 4 ? cols - c : 4;
+      u[e] = load_four<T>(q.grad, i, left, whole);
+      if (q.momentum != nullptr) {
+        const f32x4 m = load_four<MI_TYPE_F32>(q.momentum, i, left, whole);
+        u[e] = s.nesterov ? u[e] + s.mu * m : m;
+      }
+    }
+  }
   const double* sums = reinterpret_cast<const double*>(ws + q.norm_at);
   double sum = 0;
   for (int i = threadIdx.x; i < norm.first[k + 1] - norm.first[k]; i += 256) sum += sums[i];
@@ -153,132 +445,160 @@ __global__ __launch_bounds__(256) void normalize(Table t, Tiles tiles, Tiles nor
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
   __syncthreads();
   const double length = sqrt(part[0] + part[1] + part[2] + part[3]);
-  // not fmax: a NaN stays one
-  const double inv = (double)kScale / (length < (double)s.eps ? (double)s.eps : length);
+  const double inv = (double)kScaleX / (length < (double)s.eps ? (double)s.eps : length);  // not fmax: a NaN stays one
   uint16_t* x = reinterpret_cast<uint16_t*>(ws + q.x_at);
   const int ld = up32(q.n);
-  __shared__ float buf[64][65];
-  for (int e = threadIdx.x; e < 4096; e += 256) {
-    const int r = row0 + (e >> 6), c = col0 + (e & 63);
-    float v = 0.f;
-    if (r < rows && c < cols) {
-      const long long i = (long long)r * cols + c;
-      v = (float)((double)update_of<T>(q, s, i, q.momentum != nullptr ? q.momentum[i] : 0.f) * inv);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int r = e * 16 + (threadIdx.x >> 4), c = (threadIdx.x & 15) * 4;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      u[e][v] = (float)((double)u[e][v] * inv);
+      if (q.tall) buf[c + v][r] = u[e][v];
     }
-    buf[e >> 6][e & 63] = v;
+    if (!q.tall && row0 + r < q.m && col0 + c < ld) put_split4(x + split_at(row0 + r, col0 + c, ld), u[e]);
   }
+  if (!q.tall) return;
   __syncthreads();
-  for (int e = threadIdx.x; e < 4096; e += 256) {
-    const int i = e >> 6, j = e & 63;
-    const int r = q.tall ? col0 + i : row0 + i, c = q.tall ? row0 + j : col0 + j;
-    if (r < q.m && c < ld) put_split(x + split_at(r, c, ld), q.tall ? buf[j][i] : buf[i][j]);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int r = e * 16 + (threadIdx.x >> 4), c = (threadIdx.x & 15) * 4;
+    if (col0 + r < q.m && row0 + c < ld)
+      put_split4(x + split_at(col0 + r, row0 + c, ld), *reinterpret_cast<const f32x4*>(&buf[r][c]));
   }
 }
 
-// ---- the iteration -------------------------------------------------------------------------------------------------------
+// ---- larger matrices: the products ---------------------------------------------------------------------------------------
 
-// tile `id` of the upper triangle of n x n tiles, row by row
-__device__ __forceinline__ void triangle(int id, int n, int& i, int& j) {
-  i = 0;
-  while (id >= n - i) id -= n - i, ++i;
-  j = i + id;
-}
-__host__ __device__ inline int triangle_tiles(int n) { return n * (n + 1) / 2; }
-
-// X X': one tile of the upper triangle and one slice of the sum over n, in float32.
-template <class P>
-__global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void gram(Table t, Tiles tiles, char* ws, int flip) {
-  extern __shared__ char smem[];
-  const int k = find(tiles, t.count, blockIdx.x);
-  const Mat& q = t.m[k];
-  const int nt = div_up(q.m, P::BM), per = triangle_tiles(nt);
-  const int id = blockIdx.x - tiles.first[k], slice = id / per;
-  int ti, tj;
-  triangle(id - slice * per, nt, ti, tj);
-  const int ld = up32(q.n), steps = ld / 32, each = div_up(steps, q.slices), step0 = slice * each;
-  const Operand x = {reinterpret_cast<const uint16_t*>(ws + (flip ? q.y_at : q.x_at)), (long long)ld * 2, q.m, ld};
-  f32x16 acc[P::FM][P::FN];
-  P::run(acc, x, x, ti * P::BM, tj * P::BN, step0, min(each, steps - step0), (lds_bytes)smem);
-  float* c = reinterpret_cast<float*>(ws + q.c_at) + (long long)slice * q.m * up32(q.m);
-  const int row0 = ti * P::BM + P::lane_row(), col0 = tj * P::BN + P::lane_col();
+// A symmetric result's tile of the upper triangle, on both sides (the padding of a row lies in its upper half).
+template <class P, class F>
+__device__ __forceinline__ void put_symmetric(uint16_t* out, int m, int ti, int tj, F element) {
+  const int ld = up32(m), row0 = ti * P::BM + P::lane_row(), col0 = tj * P::BN + P::lane_col();
 #pragma unroll
   for (int i = 0; i < P::FM; ++i)
 #pragma unroll
     for (int j = 0; j < P::FN; ++j)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-      const int row = row0 + i * 32, col = col0 + j * 32 + g * 8;
-      if (row < q.m && col < up32(q.m)) *reinterpret_cast<f32x4*>(c + (long long)row * up32(q.m) + col) = P::quad(acc[i][j], g);
-    }
+        const int row = row0 + i * 32, col = col0 + j * 32 + g * 8;
+        if (row >= m || col >= ld) continue;
+        f32x4 v = element(i, j, g, row, col);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (col + r >= m) v[r] = 0.f;
+        put_split4(out + split_at(row, col, ld), v);
+        if (ti != tj)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (col + r < m) put_split(out + split_at(col + r, row, ld), v[r]);
+      }
 }
 
-// A from the slices of its upper triangle: a workgroup joins 64 x 64 of them and writes both halves.
-__global__ __launch_bounds__(256) void join_gram(Table t, Tiles tiles, char* ws) {
+// A = X X': one tile of the upper triangle and one slice of the sum over n.  With one slice the tile is written as it is; slices leave
+// their float32 sums in the workspace, as they lie in the registers, for join_gram.  (Having the slice that comes last join
+// them saves that launch, but each workgroup then writes its L2 back first: 241 us instead of 70 + 8 at 1024 x 12544.)
+template <class P>
+__device__ __forceinline__ f32x4* slice_sums(const Mat& q, char* ws, int per, int tile, int slice, int i, int j, int g) {
+  return reinterpret_cast<f32x4*>(ws + q.parts_at) +
+         (((long long)slice * per + tile) * (P::FM * P::FN * 4) + (i * P::FN + j) * 4 + g) * P::kThreads + threadIdx.x;
+}
+constexpr float kGramFactor = kScaleA / (kScaleX * kScaleX);
+template <class P>
+__global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void gram(Tiles tiles, char* ws, int flip) {
+  extern __shared__ char smem[];
+  const Table& t = table_of(ws);
   const int k = find(tiles, t.count, blockIdx.x);
   const Mat& q = t.m[k];
-  const int nt = div_up(q.m, 64), ld = up32(q.m);
+  const int nt = div_up(q.m, P::BM), per = triangle_tiles(nt);
+  const int id = blockIdx.x - tiles.first[k], slice = id / per, tile = id - slice * per;
   int ti, tj;
-  triangle(blockIdx.x - tiles.first[k], nt, ti, tj);
-  const float* c = reinterpret_cast<const float*>(ws + q.c_at);
-  uint16_t* a = reinterpret_cast<uint16_t*>(ws + q.a_at);
-  __shared__ float buf[64][65];
-  for (int e = threadIdx.x; e < 4096; e += 256) {
-    const int r = ti * 64 + (e >> 6), col = tj * 64 + (e & 63);
-    float v = 0.f;
-    if (r < q.m && col < q.m) {
-      for (int s = 0; s < q.slices; ++s) v += c[((long long)s * q.m + r) * ld + col];
-      v *= 1.f / kScale;
-    }
-    buf[e >> 6][e & 63] = v;
-    if (r < q.m && col < ld) put_split(a + split_at(r, col, ld), v);
+  triangle(tile, nt, ti, tj);
+  const int ld = up32(q.n), steps = ld / 32, each = div_up(steps, q.slices), step0 = slice * each;
+  const Operand x = {reinterpret_cast<const uint16_t*>(ws + (flip ? q.y_at : q.x_at)), (long long)ld * 2, q.m, ld};
+  f32x16 acc[P::FM][P::FN];
+  P::run(acc, x, x, ti * P::BM, tj * P::BN, step0, min(each, steps - step0), (lds_bytes)smem);
+  if (q.slices == 1) {
+    put_symmetric<P>(reinterpret_cast<uint16_t*>(ws + q.square_at), q.m, ti, tj,
+                     [&](int i, int j, int g, int, int) { return P::quad(acc[i][j], g) * kGramFactor; });
+    return;
   }
-  if (ti == tj) return;
-  __syncthreads();
-  for (int e = threadIdx.x; e < 4096; e += 256) {
-    const int r = tj * 64 + (e >> 6), col = ti * 64 + (e & 63);
-    if (r < q.m && col < ld) put_split(a + split_at(r, col, ld), buf[e & 63][e >> 6]);
+#pragma unroll
+  for (int i = 0; i < P::FM; ++i)
+#pragma unroll
+    for (int j = 0; j < P::FN; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) *slice_sums<P>(q, ws, per, tile, slice, i, j, g) = P::quad(acc[i][j], g);
+}
+
+// Adds the slices up in their order, one 32 x 32 fragment of each wave of a tile per workgroup.
+template <class P>
+__global__ __launch_bounds__(P::kThreads) void join_gram(Tiles tiles, char* ws) {
+  const Table& t = table_of(ws);
+  const int k = find(tiles, t.count, blockIdx.x);
+  const Mat& q = t.m[k];
+  const int nt = div_up(q.m, P::BM), per = triangle_tiles(nt), ld = up32(q.m);
+  const int id = blockIdx.x - tiles.first[k], tile = id / (P::FM * P::FN), f = id % (P::FM * P::FN), i = f / P::FN, j = f % P::FN;
+  int ti, tj;
+  triangle(tile, nt, ti, tj);
+  f32x4 v[4] = {};
+#pragma unroll 2
+  for (int s = 0; s < q.slices; ++s)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) v[g] += *slice_sums<P>(q, ws, per, tile, s, i, j, g);
+  uint16_t* a = reinterpret_cast<uint16_t*>(ws + q.square_at);
+  const int row = ti * P::BM + P::lane_row() + i * 32;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int col = tj * P::BN + P::lane_col() + j * 32 + g * 8;
+    if (row >= q.m || col >= ld) continue;
+    f32x4 w = v[g] * kGramFactor;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (col + r >= q.m) w[r] = 0.f;
+    put_split4(a + split_at(row, col, ld), w);
+    if (ti != tj)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (col + r < q.m) put_split(a + split_at(col + r, row, ld), w[r]);
   }
 }
 
-// B = b A + c A A: one tile of the upper triangle, written on both sides (the padding of a row lies in its upper half).
+// out = f0 L R + f1 L + fi I of the m x m matrices, all symmetric and polynomials of one another: one tile of the upper triangle.
+struct Square {
+  int left, right, out;
+  float f0, f1, fi;
+};
 template <class P>
-__global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void polynomial(Table t, Tiles tiles, Step s, char* ws) {
+__global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void square(Tiles tiles, Square s, char* ws) {
   extern __shared__ char smem[];
+  const Table& t = table_of(ws);
   const int k = find(tiles, t.count, blockIdx.x);
   const Mat& q = t.m[k];
   int ti, tj;
   triangle(blockIdx.x - tiles.first[k], div_up(q.m, P::BM), ti, tj);
   const int ld = up32(q.m);
-  const uint16_t* a = reinterpret_cast<const uint16_t*>(ws + q.a_at);
-  uint16_t* b = reinterpret_cast<uint16_t*>(ws + q.b_at);
-  const Operand o = {a, (long long)ld * 2, q.m, ld};
+  const auto at = [&](int i) { return reinterpret_cast<uint16_t*>(ws + q.square_at + i * q.square_bytes); };
+  const uint16_t* l = at(s.left);
   f32x16 acc[P::FM][P::FN];
-  P::run(acc, o, o, ti * P::BM, tj * P::BN, 0, ld / 32, (lds_bytes)smem);
-  const int row0 = ti * P::BM + P::lane_row(), col0 = tj * P::BN + P::lane_col();
+  P::run(acc, {l, (long long)ld * 2, q.m, ld}, {at(s.right), (long long)ld * 2, q.m, ld}, ti * P::BM, tj * P::BN, 0, ld / 32,
+         (lds_bytes)smem);
+  put_symmetric<P>(at(s.out), q.m, ti, tj, [&](int i, int j, int g, int row, int col) {
+    f32x4 v = P::quad(acc[i][j], g) * s.f0;
+    if (s.f1 != 0.f) {
+      v += get_split4(l + split_at(row, col, ld)) * s.f1;
 #pragma unroll
-  for (int i = 0; i < P::FM; ++i)
-#pragma unroll
-    for (int j = 0; j < P::FN; ++j)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-      const int row = row0 + i * 32, col = col0 + j * 32 + g * 8;
-      if (row >= q.m || col >= ld) continue;
-      const f32x4 here = get_split4(a + split_at(row, col, ld));
-      f32x4 v;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = col + r < q.m ? s.b * here[r] + s.c * (acc[i][j][g * 4 + r] * (1.f / kScale)) : 0.f;
-      put_split4(b + split_at(row, col, ld), v);
-      if (ti != tj)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (col + r < q.m) put_split(b + split_at(col + r, row, ld), v[r]);
+      for (int r = 0; r < 4; ++r)
+        if (row == col + r) v[r] += s.fi;
     }
+    return v;
+  });
 }
 
-// X <- a X + B X, or in the last iteration the result itself.
+// X <- C X (or Q X, several iterations at once), or in the last pass the result itself.
 template <class P, int T, bool LAST>
-__global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void apply(Table t, Tiles tiles, Step s, char* ws, int flip) {
+__global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void apply(Tiles tiles, Step s, char* ws, int factor, int flip) {
   extern __shared__ char smem[];
+  const Table& t = table_of(ws);
   const int k = find(tiles, t.count, blockIdx.x);
   const Mat& q = t.m[k];
   int tm, tn;
@@ -286,35 +606,32 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void apply(Table t, 
   const int ldm = up32(q.m), ld = up32(q.n);
   const uint16_t* x = reinterpret_cast<const uint16_t*>(ws + (flip ? q.y_at : q.x_at));
   uint16_t* y = reinterpret_cast<uint16_t*>(ws + (flip ? q.x_at : q.y_at));
-  const Operand b = {reinterpret_cast<const uint16_t*>(ws + q.b_at), (long long)ldm * 2, q.m, ldm};
-  const Operand xo = {x, (long long)ld * 2, q.n, q.m};
+  const uint16_t* c = reinterpret_cast<const uint16_t*>(ws + q.square_at + factor * q.square_bytes);
   f32x16 acc[P::FM][P::FN];
-  P::run(acc, b, xo, tm * P::BM, tn * P::BN, 0, ldm / 32, (lds_bytes)smem);
+  P::run(acc, {c, (long long)ldm * 2, q.m, ldm}, {x, (long long)ld * 2, q.n, q.m}, tm * P::BM, tn * P::BN, 0, ldm / 32,
+         (lds_bytes)smem);
   const int row0 = tm * P::BM + P::lane_row(), col0 = tn * P::BN + P::lane_col();
+  const bool whole = LAST && aligned16(q.out) && q.n % 4 == 0;
 #pragma unroll
   for (int i = 0; i < P::FM; ++i)
 #pragma unroll
     for (int j = 0; j < P::FN; ++j)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-      const int row = row0 + i * 32, col = col0 + j * 32 + g * 8;
-      if (row >= q.m || col >= ld) continue;
-      const f32x4 here = get_split4(x + split_at(row, col, ld));
-      f32x4 v;
+        const int row = row0 + i * 32, col = col0 + j * 32 + g * 8;
+        if (row >= q.m || col >= (LAST ? q.n : ld)) continue;
+        const f32x4 v = P::quad(acc[i][j], g) * (1.f / kScaleC);
+        if constexpr (!LAST) {
+          put_split4(y + split_at(row, col, ld), v);
+        } else if (!q.tall && whole) {
+          put_result4<T>(q, s, (long long)row * q.n + col, v * (1.f / kScaleX));
+        } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = s.a * here[r] + acc[i][j][g * 4 + r] * (1.f / kScale);
-      if constexpr (!LAST) {
-        put_split4(y + split_at(row, col, ld), v);
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (col + r >= q.n) continue;
-          const long long at = q.tall ? (long long)(col + r) * q.m + row : (long long)row * q.n + col + r;
-          const float o = v[r] * (1.f / kScale);
-          store_float<T>(q.out, at, s.update ? load_float<T>(q.out, at) * s.decay - s.lr * q.shape * o : o);
+          for (int r = 0; r < 4; ++r)
+            if (col + r < q.n)
+              put_result<T>(q, s, q.tall ? (long long)(col + r) * q.m + row : (long long)row * q.n + col + r, v[r] * (1.f / kScaleX));
         }
       }
-    }
 }
 
 // ---- launching -----------------------------------------------------------------------------------------------------------
@@ -324,50 +641,81 @@ struct TileOf {
   using type = TileProduct<SIDE, SIDE, 2, 2, SIDE == 64 ? 4 : 2, true, false, false, BKM>;
 };
 template <int SIDE>
-using Gram = typename TileOf<SIDE, false>::type;
+using Rows = typename TileOf<SIDE, false>::type;
 template <int SIDE>
-using Apply = typename TileOf<SIDE, true>::type;
+using Columns = typename TileOf<SIDE, true>::type;
 
 size_t up(size_t v) { return (v + 255) & ~size_t(255); }
 
-// Slices of the sum over n: the launch's stages are dealt to two workgroups per compute unit, each at least 8 stages long.
-void choose_slices(Table& t) {
-  long long stages = 0;
-  for (int i = 0; i < t.count; ++i) stages += (long long)triangle_tiles(div_up(t.m[i].m, 64)) * (up32(t.m[i].n) / 32);
-  long long each = stages / (2 * compute_units());
-  if (each < 8) each = 8;
-  for (int i = 0; i < t.count; ++i) {
-    const long long s = up32(t.m[i].n) / 32 / each;
-    t.m[i].slices = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
-  }
+bool is_narrow(int rows, int cols) {
+  const int m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
+  return m <= kNarrow && n <= kNarrowLong;
 }
 
-size_t lay_out_workspace(Table& t) {
-  choose_slices(t);
-  size_t at = 0;
+// Tiles and slices of X X': per side the slices that deal the launch's stages evenly to all places, each at least 8 stages long, and
+// the side with the least estimated time; joining costs the slices' way to memory and back.
+struct GramPlan {
+  int side;
+  float us;
+};
+GramPlan plan_gram(Table& t) {
+  GramPlan best = {64, INFINITY};
+  int slices[kMany];
+  for (int side : {256, 128, 64}) {
+    double stages = 0;
+    for (int i = 0; i < t.count; ++i) stages += (double)triangle_tiles(div_up(t.m[i].m, side)) * (up32(t.m[i].n) / 32);
+    double each = stages / tile_places(side);
+    if (each < 8) each = 8;
+    long long tiles = 0;
+    double bytes = 0, longest = 0;
+    int mine[kMany];
+    for (int i = 0; i < t.count; ++i) {
+      const int steps = up32(t.m[i].n) / 32, per = triangle_tiles(div_up(t.m[i].m, side));
+      const double want = steps / each;
+      mine[i] = want < 1.5 ? 1 : want > 32 ? 32 : (int)(want + 0.5);
+      tiles += (long long)per * mine[i];
+      if (mine[i] > 1) bytes += 8.0 * mine[i] * per * side * side;
+      const double len = (double)div_up(steps, mine[i]);
+      longest = len > longest ? len : longest;
+    }
+    const TileTime time = tile_time(side, true);
+    float us = launch_us(side, true, tiles, (float)(stages / tiles));
+    const float least = time.around + (float)longest * time.alone;
+    us = (us > least ? us : least) + (bytes > 0 ? 4.f + (float)(bytes / 4e6) : 0.f);
+    if (us < best.us) {
+      best = {side, us};
+      for (int i = 0; i < t.count; ++i) slices[i] = mine[i];
+    }
+  }
+  for (int i = 0; i < t.count; ++i) t.m[i].slices = slices[i];
+  return best;
+}
+
+size_t lay_out_workspace(Table& t, bool narrow, GramPlan* plan) {
+  size_t at = kTableBytes;
+  if (narrow) {
+    for (int i = 0; i < t.count; ++i) {
+      Mat& q = t.m[i];
+      const int chunks = div_up(q.n, 64), mt = div_up(q.m, 16);
+      q.slices = chunks < 16 ? chunks : div_up(chunks, 8) > 16 ? div_up(chunks, 8) : 16;
+      if (q.slices > kParts) q.slices = kParts;
+      q.parts_at = at, at += up((size_t)q.slices * triangle_tiles(mt) * 64 * 32);
+      q.square_at = at, at += up((size_t)mt * 16 * mt * 16 * 8);
+    }
+    return at;
+  }
+  *plan = plan_gram(t);
   for (int i = 0; i < t.count; ++i) {
     Mat& q = t.m[i];
     const size_t x = up((size_t)q.m * up32(q.n) * 4), a = up((size_t)q.m * up32(q.m) * 4);
     q.norm_at = at, at += up(kNormBlocks * 8);
     q.x_at = at, at += x;
     q.y_at = at, at += x;
-    q.a_at = at, at += a;
-    q.b_at = at, at += a;
-    q.c_at = at, at += a * q.slices;
+    q.square_at = at, q.square_bytes = (long long)a, at += kSquares * a;
+    q.parts_at = at;
+    if (q.slices > 1) at += (size_t)q.slices * triangle_tiles(div_up(q.m, plan->side)) * plan->side * plan->side * 4;
   }
   return at;
-}
-
-void fill(Table& t, int first, int count, const int* rows, const int* cols) {
-  t.count = count;
-  for (int i = 0; i < count; ++i) {
-    Mat& q = t.m[i];
-    const int r = rows[first + i], c = cols[first + i];
-    q = Mat{};
-    q.tall = r > c;
-    q.m = r < c ? r : c, q.n = r < c ? c : r;
-    q.shape = r > c ? std::sqrt((float)r / (float)c) : 1.f;
-  }
 }
 
 template <class F>
@@ -378,69 +726,125 @@ Tiles deal(const Table& t, F per) {
   return d;
 }
 
-template <class P, class K, class... A>
-void launch(K kernel, int blocks, hipStream_t stream, A... args) {
-  if (P::kLds > 65536)
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)P::kLds);
-  kernel<<<blocks, P::kThreads, P::kLds, stream>>>(args...);
+template <int THREADS = 256, class K, class... A>
+void launch(K kernel, unsigned lds, int blocks, hipStream_t stream, A... args) {
+  if (lds >= 65536)  // with a kernel's own variables more than what is given unasked
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  kernel<<<blocks, THREADS, lds, stream>>>(args...);
 }
 
-// One stage of the iteration over all matrices: the workgroups of each for tiles of 256, 128 and 64, and the side that is taken.
+// One stage of the iteration over all matrices: the workgroups of each, the tile side with the least estimated time, that time.
 struct Dealt {
   Tiles tiles;
   int side;
+  float us;
 };
-template <class F, class G>
-Dealt choose(const Table& t, F tiles_of, G steps_of) {
+template <class F>
+Dealt choose(const Table& t, F tiles_of) {
   const Tiles a = deal(t, [&](const Mat& q) { return tiles_of(q, 256); }), b = deal(t, [&](const Mat& q) { return tiles_of(q, 128); }),
               c = deal(t, [&](const Mat& q) { return tiles_of(q, 64); });
   double stages = 0;
-  for (int i = 0; i < t.count; ++i) stages += (double)(c.first[i + 1] - c.first[i]) * steps_of(t.m[i]);
-  const int side = choose_tile(a.first[t.count], b.first[t.count], c.first[t.count], (float)(stages / c.first[t.count]), true);
-  return {side == 256 ? a : side == 128 ? b : c, side};
+  for (int i = 0; i < t.count; ++i) stages += (double)(c.first[i + 1] - c.first[i]) * (up32(t.m[i].m) / 32);
+  const float steps = (float)(stages / c.first[t.count]);
+  const int side = choose_tile(a.first[t.count], b.first[t.count], c.first[t.count], steps, true);
+  const Tiles& d = side == 256 ? a : side == 128 ? b : c;
+  return {d, side, launch_us(side, true, d.first[t.count], steps)};
+}
+
+// How many iterations share a pass over the long side (1, 2 or 3): the least estimated time among those whose product of factors C
+// stays within the stored form's range.
+int iterations_a_pass(int steps, float gram_us, float square_us, float apply_us, const double* growth) {
+  int best = 1;
+  float least = INFINITY;
+  for (int g = 1; g <= 3 && g <= steps; ++g) {
+    if (g > 1 && !(growth[g] <= kMostC)) break;
+    float us = 0.f;
+    for (int done = 0; done < steps; done += g) {
+      const int now = steps - done < g ? steps - done : g;
+      us += gram_us + apply_us + (4 * now - 3) * square_us;
+    }
+    if (us < least) least = us, best = g;
+  }
+  return best;
 }
 
 template <int T>
-void iterate(const Table& t, const Step& s, int steps, char* ws, hipStream_t stream) {
+void iterate(const Table& t, const Step& s, const GramPlan& plan, const double* growth, char* ws, hipStream_t stream) {
   const Tiles norm = deal(t, [](const Mat& q) {
     const int b = ceil_div((long long)q.m * q.n, kNormElements);
     return b > kNormBlocks ? kNormBlocks : b;
   });
   momentum_and_norm<T><<<norm.first[t.count], 256, 0, stream>>>(t, norm, s, ws);
   const Tiles squares = deal(t, [](const Mat& q) { return div_up(q.m, 64) * div_up(q.n, 64); });
-  normalize<T><<<squares.first[t.count], 256, 0, stream>>>(t, squares, norm, s, ws);
-  const Dealt g = choose(t, [](const Mat& q, int side) { return triangle_tiles(div_up(q.m, side)) * q.slices; },
-                         [](const Mat& q) { return up32(q.n) / 32 / q.slices; });
-  const auto short_steps = [](const Mat& q) { return up32(q.m) / 32; };
-  const Dealt p = choose(t, [](const Mat& q, int side) { return triangle_tiles(div_up(q.m, side)); }, short_steps);
-  const Dealt f = choose(t, [](const Mat& q, int side) { return div_up(q.m, side) * div_up(q.n, side); }, short_steps);
-  const Tiles joined = deal(t, [](const Mat& q) { return triangle_tiles(div_up(q.m, 64)); });
-  for (int i = 0; i < steps; ++i) {
-    const int flip = i & 1;
-    if (g.side == 256)
-      launch<Gram<256>>(gram<Gram<256>>, g.tiles.first[t.count], stream, t, g.tiles, ws, flip);
-    else if (g.side == 128)
-      launch<Gram<128>>(gram<Gram<128>>, g.tiles.first[t.count], stream, t, g.tiles, ws, flip);
-    else
-      launch<Gram<64>>(gram<Gram<64>>, g.tiles.first[t.count], stream, t, g.tiles, ws, flip);
-    join_gram<<<joined.first[t.count], 256, 0, stream>>>(t, joined, ws);
+  normalize<T><<<squares.first[t.count], 256, 0, stream>>>(squares, norm, s, ws);
+  const Tiles g = deal(t, [&](const Mat& q) { return triangle_tiles(div_up(q.m, plan.side)) * q.slices; });
+  const int frags = plan.side / 64 * (plan.side / 64);
+  const Tiles joins = deal(t, [&](const Mat& q) { return q.slices > 1 ? triangle_tiles(div_up(q.m, plan.side)) * frags : 0; });
+  const Dealt p = choose(t, [](const Mat& q, int side) { return triangle_tiles(div_up(q.m, side)); });
+  const Dealt f = choose(t, [](const Mat& q, int side) { return div_up(q.m, side) * div_up(q.n, side); });
+  const auto do_square = [&](int left, int right, int out, float f0, float f1, float fi) {
+    const Square q = {left, right, out, f0, f1, fi};
     if (p.side == 256)
-      launch<Gram<256>>(polynomial<Gram<256>>, p.tiles.first[t.count], stream, t, p.tiles, s, ws);
+      launch(square<Rows<256>>, Rows<256>::kLds, p.tiles.first[t.count], stream, p.tiles, q, ws);
     else if (p.side == 128)
-      launch<Gram<128>>(polynomial<Gram<128>>, p.tiles.first[t.count], stream, t, p.tiles, s, ws);
+      launch(square<Rows<128>>, Rows<128>::kLds, p.tiles.first[t.count], stream, p.tiles, q, ws);
     else
-      launch<Gram<64>>(polynomial<Gram<64>>, p.tiles.first[t.count], stream, t, p.tiles, s, ws);
-    const bool last = i + 1 == steps;
+      launch(square<Rows<64>>, Rows<64>::kLds, p.tiles.first[t.count], stream, p.tiles, q, ws);
+  };
+  const int a_pass = iterations_a_pass(s.steps, plan.us, p.us, f.us, growth);
+  int flip = 0;
+  for (int done = 0; done < s.steps; flip ^= 1) {
+    const int now = s.steps - done < a_pass ? s.steps - done : a_pass;
+    done += now;
+    if (plan.side == 256)
+      launch(gram<Rows<256>>, Rows<256>::kLds, g.first[t.count], stream, g, ws, flip);
+    else if (plan.side == 128)
+      launch(gram<Rows<128>>, Rows<128>::kLds, g.first[t.count], stream, g, ws, flip);
+    else
+      launch(gram<Rows<64>>, Rows<64>::kLds, g.first[t.count], stream, g, ws, flip);
+    if (joins.first[t.count] > 0) {
+      if (plan.side == 256)
+        launch(join_gram<Rows<256>>, 0, joins.first[t.count], stream, joins, ws);
+      else if (plan.side == 128)
+        launch(join_gram<Rows<128>>, 0, joins.first[t.count], stream, joins, ws);
+      else
+        launch(join_gram<Rows<64>>, 0, joins.first[t.count], stream, joins, ws);
+    }
+    int product = kQ, spare = kT;
+    for (int i = 0; i < now; ++i) {
+      const int c = i == 0 ? kQ : kC;
+      do_square(kA, kA, c, s.c * kScaleC / (kScaleA * kScaleA), s.b * kScaleC / kScaleA, s.a * kScaleC);
+      if (i > 0) {
+        do_square(kC, product, spare, 1.f / kScaleC, 0.f, 0.f);
+        const int old = product;
+        product = spare, spare = old;
+      }
+      if (i + 1 < now) {
+        const int factor = i == 0 ? product : kC;
+        do_square(factor, kA, spare, 1.f / kScaleC, 0.f, 0.f);
+        do_square(spare, factor, kA, 1.f / kScaleC, 0.f, 0.f);
+      }
+    }
+    const bool last = done == s.steps;
     if (f.side == 256)
-      launch<Apply<256>>(last ? apply<Apply<256>, T, true> : apply<Apply<256>, T, false>, f.tiles.first[t.count], stream, t, f.tiles,
-                         s, ws, flip);
+      launch(last ? apply<Columns<256>, T, true> : apply<Columns<256>, T, false>, Columns<256>::kLds, f.tiles.first[t.count], stream,
+             f.tiles, s, ws, product, flip);
     else if (f.side == 128)
-      launch<Apply<128>>(last ? apply<Apply<128>, T, true> : apply<Apply<128>, T, false>, f.tiles.first[t.count], stream, t, f.tiles,
-                         s, ws, flip);
+      launch(last ? apply<Columns<128>, T, true> : apply<Columns<128>, T, false>, Columns<128>::kLds, f.tiles.first[t.count], stream,
+             f.tiles, s, ws, product, flip);
     else
-      launch<Apply<64>>(last ? apply<Apply<64>, T, true> : apply<Apply<64>, T, false>, f.tiles.first[t.count], stream, t, f.tiles, s,
-                        ws, flip);
+      launch(last ? apply<Columns<64>, T, true> : apply<Columns<64>, T, false>, Columns<64>::kLds, f.tiles.first[t.count], stream,
+             f.tiles, s, ws, product, flip);
   }
+}
+
+template <int T>
+void iterate_narrow(const Table& t, const Step& s, char* ws, hipStream_t stream) {
+  const Tiles parts = deal(t, [](const Mat& q) { return q.slices; });
+  narrow_gram<T><<<parts.first[t.count], 256, 0, stream>>>(t, parts, s, ws);
+  launch<kPolyThreads>(narrow_polynomial, 4 * sizeof(double) * kNarrow * kLdM, t.count, stream, s, ws);
+  const Tiles columns = deal(t, [](const Mat& q) { return div_up(q.n, 64); });
+  narrow_apply<T><<<columns.first[t.count], 256, 0, stream>>>(columns, s, ws);
 }
 
 int check_matrices(int count, const int* rows, const int* cols) {
@@ -452,42 +856,91 @@ int check_matrices(int count, const int* rows, const int* cols) {
   return MI_OK;
 }
 
-// The largest magnitude that X, A or B can reach from |X| <= 1.  It is also the test that the scale of the stored forms holds.
-int check_coefficients(const float* c, int steps, float eps) {
+// growth[g]: the largest product of g successive factors C.  False for coefficients with which X or a single C leaves the range of
+// the stored forms.  Sampled over the singular values, with a margin for what lies between the samples.
+bool range_of(const float* c, int steps, double* growth) {
+  bool fits = std::isfinite(c[0]) && std::isfinite(c[1]) && std::isfinite(c[2]);
+  growth[1] = growth[2] = growth[3] = 0;
+  double top = 1.0;
+  for (int i = 0; i < steps && fits; ++i) {
+    double next = 0;
+    for (int k = 0; k <= 1024; ++k) {
+      double x = top * k / 1024, product = 1;
+      for (int g = 1; g <= 3 && i + g <= steps; ++g) {
+        const double x2 = x * x, factor = c[0] + x2 * (c[1] + x2 * c[2]);
+        product *= factor;
+        x *= factor;
+        if (g == 1) next = std::fmax(next, std::fabs(x));
+        growth[g] = std::fmax(growth[g], 1.001 * std::fabs(product));
+      }
+    }
+    next *= 1.001;
+    fits = next <= kMostX && growth[1] <= kMostC;
+    top = next;
+  }
+  return fits;
+}
+
+int check_coefficients(const float* c, int steps, float eps, double* growth) {
   MI_REQUIRE(c != nullptr && steps >= 1 && steps <= 64, "orthogonalize: %d steps, 1 to 64 are taken", steps);
   MI_REQUIRE(eps > 0.f, "orthogonalize: eps must be positive");
-  const bool finite = std::isfinite(c[0]) && std::isfinite(c[1]) && std::isfinite(c[2]);
-  double top = 1.0;
-  for (int i = 0; i < steps; ++i) {
-    double next = 0, inner = 0;
-    for (int k = 0; k <= 4096; ++k) {
-      const double x = top * k / 4096, x2 = x * x;
-      next = std::fmax(next, std::fabs(x * (c[0] + x2 * (c[1] + x2 * c[2]))));
-      inner = std::fmax(inner, std::fabs(x2 * (c[1] + x2 * c[2])));
-    }
-    next *= 1.001, inner *= 1.001;
-    if (!(next <= kMostMagnitude && inner <= kMostMagnitude && top * top <= kMostMagnitude && finite)) {
-      set_error("orthogonalize: coefficients (%g, %g, %g) let the iteration grow beyond %g", c[0], c[1], c[2], kMostMagnitude);
-      return MI_ERR_UNSUPPORTED;
-    }
-    top = next;
+  // a program asks for the same polynomial all the time, and sampling it takes longer than launching: the last answer is kept
+  struct Answer {
+    float c[3];
+    int steps;
+    bool fits;
+    double growth[4];
+  };
+  thread_local Answer last = {};
+  if (last.steps != steps || std::memcmp(last.c, c, sizeof last.c) != 0) {
+    std::memcpy(last.c, c, sizeof last.c);
+    last.steps = steps;
+    last.fits = range_of(c, steps, last.growth);
+  }
+  for (int g = 1; g <= 3; ++g) growth[g] = last.growth[g];
+  if (!last.fits) {
+    set_error("orthogonalize: coefficients (%g, %g, %g) let the iteration grow beyond %g", c[0], c[1], c[2], kMostX);
+    return MI_ERR_UNSUPPORTED;
   }
   return MI_OK;
 }
 
+// Calls `visit(table, indices, narrow)` for tables of up to kMany matrices of one way, narrow ones first.
+template <class F>
+void each_table(int count, const int* rows, const int* cols, F visit) {
+  for (int narrow = 1; narrow >= 0; --narrow) {
+    Table t = {};
+    int index[kMany];
+    for (int i = 0; i <= count; ++i) {
+      if (i < count && is_narrow(rows[i], cols[i]) == (narrow != 0)) {
+        Mat& q = t.m[t.count];
+        q = Mat{};
+        q.tall = rows[i] > cols[i];
+        q.m = q.tall ? cols[i] : rows[i], q.n = q.tall ? rows[i] : cols[i];
+        q.shape = q.tall ? std::sqrt((float)rows[i] / (float)cols[i]) : 1.f;
+        index[t.count++] = i;
+      }
+      if (t.count == kMany || (i == count && t.count > 0)) {
+        visit(t, index, narrow != 0);
+        t.count = 0;
+      }
+    }
+  }
+}
+
 size_t workspace_bytes_of(int count, const int* rows, const int* cols) {
   size_t most = 0;
-  for (int first = 0; first < count; first += kMany) {
-    Table t;
-    fill(t, first, count - first < kMany ? count - first : kMany, rows, cols);
-    const size_t b = lay_out_workspace(t);
+  each_table(count, rows, cols, [&](Table& t, const int*, bool narrow) {
+    GramPlan plan;
+    const size_t b = lay_out_workspace(t, narrow, &plan);
     most = b > most ? b : most;
-  }
+  });
   return most;
 }
 
 int run_all(int count, const void* const* grads, void* const* outs, float* const* momenta, const int* rows, const int* cols,
-            int dtype, const Step& s, int steps, void* workspace, size_t workspace_bytes, hipStream_t stream, const char* what) {
+            int dtype, const Step& s, const double* growth, void* workspace, size_t workspace_bytes, hipStream_t stream,
+            const char* what) {
   MI_REQUIRE(grads != nullptr && outs != nullptr && workspace != nullptr, "%s: null pointer", what);
   MI_REQUIRE(dtype == MI_TYPE_F32 || dtype == MI_TYPE_F16 || dtype == MI_TYPE_BF16, "%s: dtype %d", what, dtype);
   MI_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "%s: the workspace starts on 256 bytes", what);
@@ -500,23 +953,29 @@ int run_all(int count, const void* const* grads, void* const* outs, float* const
     return MI_ERR_WORKSPACE;
   }
   begin_call();
-  for (int first = 0; first < count; first += kMany) {
-    Table t;
-    fill(t, first, count - first < kMany ? count - first : kMany, rows, cols);
-    lay_out_workspace(t);
+  char* ws = static_cast<char*>(workspace);
+  each_table(count, rows, cols, [&](Table& t, const int* index, bool narrow) {
+    GramPlan plan;
+    lay_out_workspace(t, narrow, &plan);
     for (int i = 0; i < t.count; ++i) {
-      t.m[i].grad = grads[first + i];
-      t.m[i].out = outs[first + i];
-      t.m[i].momentum = momenta != nullptr ? momenta[first + i] : nullptr;
+      t.m[i].grad = grads[index[i]];
+      t.m[i].out = outs[index[i]];
+      t.m[i].momentum = momenta != nullptr ? momenta[index[i]] : nullptr;
     }
-    char* ws = static_cast<char*>(workspace);
+    const auto go = [&](auto type) {
+      constexpr int T = decltype(type)::value;
+      if (narrow)
+        iterate_narrow<T>(t, s, ws, stream);
+      else
+        iterate<T>(t, s, plan, growth, ws, stream);
+    };
     if (dtype == MI_TYPE_F32)
-      iterate<MI_TYPE_F32>(t, s, steps, ws, stream);
+      go(std::integral_constant<int, MI_TYPE_F32>{});
     else if (dtype == MI_TYPE_F16)
-      iterate<MI_TYPE_F16>(t, s, steps, ws, stream);
+      go(std::integral_constant<int, MI_TYPE_F16>{});
     else
-      iterate<MI_TYPE_BF16>(t, s, steps, ws, stream);
-  }
+      go(std::integral_constant<int, MI_TYPE_BF16>{});
+  });
   return check_launch(what);
 }
 
@@ -534,21 +993,23 @@ size_t mi_orthogonalize_workspace_bytes(int count, const int* rows, const int* c
 
 int mi_orthogonalize(int count, const void* const* in, void* const* out, const int* rows, const int* cols, int dtype, int steps,
                      const float* coefficients, float eps, void* workspace, size_t workspace_bytes, mi_stream_t stream) {
+  double growth[4];
   if (const int rc = check_matrices(count, rows, cols)) return rc;
-  if (const int rc = check_coefficients(coefficients, steps, eps)) return rc;
-  const Step s = {coefficients[0], coefficients[1], coefficients[2], eps, 0.f, 0.f, 1.f, 0, 0};
-  return run_all(count, in, out, nullptr, rows, cols, dtype, s, steps, workspace, workspace_bytes, as_stream(stream),
+  if (const int rc = check_coefficients(coefficients, steps, eps, growth)) return rc;
+  const Step s = {coefficients[0], coefficients[1], coefficients[2], eps, 0.f, 0.f, 1.f, 0, 0, steps};
+  return run_all(count, in, out, nullptr, rows, cols, dtype, s, growth, workspace, workspace_bytes, as_stream(stream),
                  "mi_orthogonalize");
 }
 
 int mi_muon_step(int count, void* const* params, const void* const* grads, float* const* momenta, const int* rows, const int* cols,
                  int dtype, float lr, float momentum, int nesterov, float weight_decay, int steps, const float* coefficients,
                  float eps, void* workspace, size_t workspace_bytes, mi_stream_t stream) {
+  double growth[4];
   if (const int rc = check_matrices(count, rows, cols)) return rc;
-  if (const int rc = check_coefficients(coefficients, steps, eps)) return rc;
+  if (const int rc = check_coefficients(coefficients, steps, eps, growth)) return rc;
   MI_REQUIRE(momenta != nullptr, "mi_muon_step: null pointer");
-  const Step s = {coefficients[0], coefficients[1], coefficients[2], eps, momentum, lr, 1.f - lr * weight_decay, nesterov, 1};
-  return run_all(count, grads, params, momenta, rows, cols, dtype, s, steps, workspace, workspace_bytes, as_stream(stream),
+  const Step s = {coefficients[0], coefficients[1], coefficients[2], eps, momentum, lr, 1.f - lr * weight_decay, nesterov, 1, steps};
+  return run_all(count, grads, params, momenta, rows, cols, dtype, s, growth, workspace, workspace_bytes, as_stream(stream),
                  "mi_muon_step");
 }
 

@@ -518,8 +518,9 @@ int mi_linear_cross_entropy_backward(const float* grad_loss, const void* weight,
  * mi_orthogonalize: Newton-Schulz iteration.  For each matrix G (turned when it has more rows than columns)
  *   X = G / max(|G|_F, eps);   `steps` times  A = X X^T, X = a X + (b A + c A A) X   with coefficients = (a, b, c)
  * dense row-major matrices of one dtype (MI_TYPE_*); `in`, `out`, rows, cols and coefficients are HOST arrays, out[i] may be
- * in[i].  Products carry 22 bits and accumulate in float32.  All matrices go through the stages together.
- * Coefficients that let the iteration leave [-15, 15] from |X| <= 1 are refused (MI_ERR_UNSUPPORTED).
+ * in[i].  Products carry 22 bits and accumulate in float32 (fp64 where the short side is at most 64).  All matrices go through the
+ * stages together.
+ * Coefficients that let singular values grow beyond 2.8 from at most 1 are refused (MI_ERR_UNSUPPORTED).
  * mi_muon_step: the optimiser step around it, per matrix (momenta float32, params and grads of `dtype`):
  *   M = momentum M + G;  U = G + momentum M (nesterov) or M;
  *   W = (1 - lr weight_decay) W - lr sqrt(max(1, rows / cols)) orthogonalize(U)
