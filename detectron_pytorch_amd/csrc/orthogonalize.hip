@@ -174,26 +174,45 @@ __device__ __forceinline__ float update_of(const Mat& q, const Step& s, long lon
   const float m = q.momentum[i];
   return s.nesterov ? load_float<T>(q.grad, i) + s.mu * m : m;
 }
-template <int T>
-__device__ __forceinline__ void put_result(const Mat& q, const Step& s, long long i, float o) {
-  store_float<T>(q.out, i, s.update ? load_float<T>(q.out, i) * s.decay - s.lr * q.shape * o : o);
-}
-
-// four of them, on their alignment
-template <int T>
-__device__ __forceinline__ void put_result4(const Mat& q, const Step& s, long long i, f32x4 o) {
-  if (s.update) o = load_four<T>(q.out, i, 4, true) * s.decay - (s.lr * q.shape) * o;
-  if constexpr (T == MI_TYPE_F32) {
-    *reinterpret_cast<f32x4*>(static_cast<float*>(q.out) + i) = o;
-  } else {
-    s16x4 h;
+// The results of a lane, sixteen of them at at(e) where inside(e): the old weights are all asked for before the first result is written.
+template <int T, class A, class I>
+__device__ __forceinline__ void put_results(const Mat& q, const Step& s, A at, I inside, const float (&o)[16]) {
+  float w[16] = {};
+  if (s.update) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      short one;
-      store_float<T>(&one, 0, o[r]);
-      h[r] = one;
+    for (int e = 0; e < 16; ++e)
+      if (inside(e)) w[e] = load_float<T>(q.out, at(e));
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    if (inside(e)) store_float<T>(q.out, at(e), s.update ? w[e] * s.decay - s.lr * q.shape * o[e] : o[e]);
+}
+// The same for four groups of four on their alignment.
+template <int T, class A, class I>
+__device__ __forceinline__ void put_results4(const Mat& q, const Step& s, A at, I inside, const float (&o)[16]) {
+  f32x4 w[4] = {};
+  if (s.update) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      if (inside(g * 4)) w[g] = load_four<T>(q.out, at(g * 4), 4, true);
+  }
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    if (!inside(g * 4)) continue;
+    f32x4 v = {o[g * 4], o[g * 4 + 1], o[g * 4 + 2], o[g * 4 + 3]};
+    if (s.update) v = w[g] * s.decay - (s.lr * q.shape) * v;
+    if constexpr (T == MI_TYPE_F32) {
+      *reinterpret_cast<f32x4*>(static_cast<float*>(q.out) + at(g * 4)) = v;
+    } else {
+      s16x4 h;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        short one;
+        store_float<T>(&one, 0, v[r]);
+        h[r] = one;
+      }
+      *reinterpret_cast<s16x4*>(static_cast<uint16_t*>(q.out) + at(g * 4)) = h;
     }
-    *reinterpret_cast<s16x4*>(static_cast<uint16_t*>(q.out) + i) = h;
   }
 }
 
@@ -224,7 +243,7 @@ __device__ __forceinline__ void triangle(int id, int n, int& i, int& j) {
   while (id >= n - i) id -= n - i, ++i;
   j = i + id;
 }
-__host__ __device__ inline int triangle_tiles(int n) { return n * (n + 1) / 2; }
+__host__ __device__ constexpr int triangle_tiles(int n) { return n * (n + 1) / 2; }
 
 // Partial sums of U U': a workgroup adds up its share of 64-column chunks, each wave its tiles of the upper triangle (16 x 16;
 // a lane holds column l & 15, rows (l >> 4) + 4 r) and writes them as they lie in its registers.
@@ -258,33 +277,35 @@ __global__ __launch_bounds__(256) void narrow_gram(Table t, Tiles tiles, Step s,
     if (wave + x * 4 < total) out[(wave + x * 4) * 64 + lane] = acc[x];
 }
 
-// Symmetric product of commuting symmetric matrices in LDS, one tile of the upper triangle per wave; `put(i, j, v)` gets each element of the upper triangle's tiles.
-template <class F>
-__device__ __forceinline__ void narrow_product(const double (*x)[kLdM], const double (*y)[kLdM], int nt, F put) {
+// Symmetric product of commuting symmetric matrices in LDS, one tile of the upper triangle per wave; `put(i, j, v)` gets each
+// element of them.  Two accumulators: a product of this type waits for the one it adds to.
+template <int NT, class F>
+__device__ __forceinline__ void narrow_product(const double (*x)[kLdM], const double (*y)[kLdM], F put) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (wave >= triangle_tiles(nt)) return;
+  if (wave >= triangle_tiles(NT)) return;
   int i, j;
-  triangle(wave, nt, i, j);
+  triangle(wave, NT, i, j);
   const double *a = &x[i * 16 + (lane & 15)][lane >> 4], *b = &y[j * 16 + (lane & 15)][lane >> 4];
-  f64x4 acc = {};
-  for (int p = 0; p < nt * 16; p += 16) {
-    double u[4], v[4];
+  double u[NT * 4], v[NT * 4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) u[k] = a[p + 4 * k], v[k] = b[p + 4 * k];
+  for (int k = 0; k < NT * 4; ++k) u[k] = a[4 * k], v[k] = b[4 * k];
+  f64x4 even = {}, odd = {};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(u[k], v[k], acc, 0, 0, 0);
+  for (int k = 0; k < NT * 4; k += 2) {
+    even = __builtin_amdgcn_mfma_f64_16x16x4f64(u[k], v[k], even, 0, 0, 0);
+    odd = __builtin_amdgcn_mfma_f64_16x16x4f64(u[k + 1], v[k + 1], odd, 0, 0, 0);
   }
 #pragma unroll
-  for (int r = 0; r < 4; ++r) put(i * 16 + (lane >> 4) + 4 * r, j * 16 + (lane & 15), acc[r]);
+  for (int r = 0; r < 4; ++r) put(i * 16 + (lane >> 4) + 4 * r, j * 16 + (lane & 15), even[r] + odd[r]);
 }
 
 // Q / max(|G|, eps) of one matrix per workgroup.
 constexpr int kPolyThreads = 640;  // ten tiles of 16 x 16 make the upper triangle of 64 x 64
-__global__ __launch_bounds__(kPolyThreads) void narrow_polynomial(Step s, char* ws) {
-  const Mat& q = table_of(ws).m[blockIdx.x];
-  extern __shared__ char smem[];
+template <int NT>
+__device__ __forceinline__ void polynomial_of(const Mat& q, const Step& s, char* ws, char* smem) {
   using Square = double (*)[kLdM];
-  const int nt = div_up(q.m, 16), total = triangle_tiles(nt), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int nt = NT, total = triangle_tiles(NT);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const size_t bytes = sizeof(double) * kNarrow * kLdM;
   Square a = reinterpret_cast<Square>(smem), c = reinterpret_cast<Square>(smem + bytes),
          p = reinterpret_cast<Square>(smem + 2 * bytes), t = reinterpret_cast<Square>(smem + 3 * bytes);
@@ -319,25 +340,38 @@ __global__ __launch_bounds__(kPolyThreads) void narrow_polynomial(Step s, char* 
   for (int k = 0; k < s.steps; ++k) {
     const Square poly = k == 0 ? p : c;
     const auto put = both(poly);
-    narrow_product(a, a, nt, [&](int i, int j, double v) {
+    narrow_product<NT>(a, a, [&](int i, int j, double v) {
       put(i, j, (i == j ? (double)s.a : 0.0) + (double)s.b * a[i][j] + (double)s.c * v);
     });
     __syncthreads();
     if (k > 0) {
-      narrow_product(c, p, nt, both(t));
+      narrow_product<NT>(c, p, both(t));
       __syncthreads();
       const Square old = p;
       p = t, t = old;
     }
     if (k + 1 == s.steps) break;
     const Square now = k == 0 ? p : c;
-    narrow_product(now, a, nt, both(t));
+    narrow_product<NT>(now, a, both(t));
     __syncthreads();
-    narrow_product(t, now, nt, both(a));
+    narrow_product<NT>(t, now, both(a));
     __syncthreads();
   }
   double* out = reinterpret_cast<double*>(ws + q.square_at);
   for (int e = threadIdx.x; e < nt * 16 * nt * 16; e += kPolyThreads) out[e] = p[e / (nt * 16)][e % (nt * 16)] * inv;
+}
+
+__global__ __launch_bounds__(kPolyThreads) void narrow_polynomial(Step s, char* ws) {
+  const Mat& q = table_of(ws).m[blockIdx.x];
+  extern __shared__ char smem[];
+  if (q.m <= 16)
+    polynomial_of<1>(q, s, ws, smem);
+  else if (q.m <= 32)
+    polynomial_of<2>(q, s, ws, smem);
+  else if (q.m <= 48)
+    polynomial_of<3>(q, s, ws, smem);
+  else
+    polynomial_of<4>(q, s, ws, smem);
 }
 
 // Q U, 64 columns per workgroup.
@@ -367,12 +401,13 @@ __global__ __launch_bounds__(256) void narrow_apply(Tiles tiles, Step s, char* w
         acc = q.tall ? __builtin_amdgcn_mfma_f64_16x16x4f64(y[k], x[k], acc, 0, 0, 0)
                      : __builtin_amdgcn_mfma_f64_16x16x4f64(x[k], y[k], acc, 0, 0, 0);
     }
+    const auto row = [&](int r) { return i * 16 + (q.tall ? lane & 15 : (lane >> 4) + 4 * r); };
+    const auto col = [&](int r) { return col0 + j0 + (q.tall ? (lane >> 4) + 4 * r : lane & 15); };
+    float o[16];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int d = (lane >> 4) + 4 * r, row = i * 16 + (q.tall ? lane & 15 : d), col = col0 + j0 + (q.tall ? d : lane & 15);
-      if (row < q.m && col < q.n)
-        put_result<T>(q, s, q.tall ? (long long)col * q.m + row : (long long)row * q.n + col, (float)acc[r]);
-    }
+    for (int r = 0; r < 4; ++r) o[r] = (float)acc[r];
+    put_results<T>(q, s, [&](int r) { return q.tall ? (long long)col(r) * q.m + row(r) : (long long)row(r) * q.n + col(r); },
+                   [&](int r) { return r < 4 && row(r) < q.m && col(r) < q.n; }, o);
   }
 }
 
@@ -611,27 +646,32 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void apply(Tiles til
   P::run(acc, {c, (long long)ldm * 2, q.m, ldm}, {x, (long long)ld * 2, q.n, q.m}, tm * P::BM, tn * P::BN, 0, ldm / 32,
          (lds_bytes)smem);
   const int row0 = tm * P::BM + P::lane_row(), col0 = tn * P::BN + P::lane_col();
-  const bool whole = LAST && aligned16(q.out) && q.n % 4 == 0;
+  const bool whole = LAST && !q.tall && aligned16(q.out) && q.n % 4 == 0;
 #pragma unroll
-  for (int i = 0; i < P::FM; ++i)
+  for (int i = 0; i < P::FM; ++i) {
+    const int row = row0 + i * 32;
+    if (row >= q.m) continue;
 #pragma unroll
-    for (int j = 0; j < P::FN; ++j)
+    for (int j = 0; j < P::FN; ++j) {
+      const int col = col0 + j * 32;
+      if constexpr (!LAST) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int row = row0 + i * 32, col = col0 + j * 32 + g * 8;
-        if (row >= q.m || col >= (LAST ? q.n : ld)) continue;
-        const f32x4 v = P::quad(acc[i][j], g) * (1.f / kScaleC);
-        if constexpr (!LAST) {
-          put_split4(y + split_at(row, col, ld), v);
-        } else if (!q.tall && whole) {
-          put_result4<T>(q, s, (long long)row * q.n + col, v * (1.f / kScaleX));
-        } else {
+        for (int g = 0; g < 4; ++g)
+          if (col + g * 8 < ld) put_split4(y + split_at(row, col + g * 8, ld), P::quad(acc[i][j], g) * (1.f / kScaleC));
+      } else {
+        float o[16];
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (col + r < q.n)
-              put_result<T>(q, s, q.tall ? (long long)(col + r) * q.m + row : (long long)row * q.n + col + r, v[r] * (1.f / kScaleX));
-        }
+        for (int e = 0; e < 16; ++e) o[e] = acc[i][j][e] * (1.f / (kScaleC * kScaleX));
+        const auto column = [&](int e) { return col + (e >> 2) * 8 + (e & 3); };
+        const auto at = [&](int e) { return q.tall ? (long long)column(e) * q.m + row : (long long)row * q.n + column(e); };
+        const auto inside = [&](int e) { return column(e) < q.n; };
+        if (whole)
+          put_results4<T>(q, s, at, inside, o);
+        else
+          put_results<T>(q, s, at, inside, o);
       }
+    }
+  }
 }
 
 // ---- launching -----------------------------------------------------------------------------------------------------------

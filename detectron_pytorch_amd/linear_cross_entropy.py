@@ -23,24 +23,24 @@ REDUCTIONS = {"none": _lib.REDUCTION_NONE, "mean": _lib.REDUCTION_MEAN, "sum": _
 
 
 def _check(x, weight, bias, labels, reduction):
-    for t, name in ((x, "x"), (weight, "weight"), (labels, "labels")):
-        _lib.require_cuda(t, name)
+    device, dtype = x.device, x.dtype
+    for t, name in ((x, "x"), (weight, "weight"), (labels, "labels"), (bias, "bias")):
+        if t is not None:
+            _lib.require_cuda(t, name)
+            if t.device != device:
+                raise ValueError("linear_cross_entropy takes tensors on one device")
     if x.dim() != 2 or weight.dim() != 2 or x.size(1) != weight.size(1):
         raise ValueError("linear_cross_entropy takes x [rows, dim] and weight [classes, dim], got %s and %s"
                          % (tuple(x.shape), tuple(weight.shape)))
-    if weight.size(0) < 1 or weight.size(1) < 1:
+    if weight.numel() == 0:
         raise ValueError("linear_cross_entropy needs at least one class and one feature, got weight %s" % (tuple(weight.shape),))
-    if x.dtype not in TYPES or weight.dtype != x.dtype:
+    if dtype not in TYPES or weight.dtype != dtype:
         raise ValueError("linear_cross_entropy takes float32, float16 or bfloat16 x and weight of one type, got %s and %s"
-                         % (x.dtype, weight.dtype))
-    if bias is not None:
-        _lib.require_cuda(bias, "bias")
-        if bias.dtype != weight.dtype or bias.shape != weight.shape[:1]:
-            raise ValueError("bias must be %s [%d], got %s %s" % (weight.dtype, weight.size(0), bias.dtype, tuple(bias.shape)))
-    if labels.dtype not in (torch.int32, torch.int64) or labels.shape != x.shape[:1]:
+                         % (dtype, weight.dtype))
+    if bias is not None and (bias.dtype != dtype or bias.shape != weight.shape[:1]):
+        raise ValueError("bias must be %s [%d], got %s %s" % (dtype, weight.size(0), bias.dtype, tuple(bias.shape)))
+    if (labels.dtype is not torch.int64 and labels.dtype is not torch.int32) or labels.shape != x.shape[:1]:
         raise ValueError("labels must be int32 or int64 [%d], got %s %s" % (x.size(0), labels.dtype, tuple(labels.shape)))
-    if any(t is not None and t.device != x.device for t in (weight, bias, labels)):
-        raise ValueError("linear_cross_entropy takes tensors on one device")
     if reduction not in REDUCTIONS:
         raise ValueError("reduction must be 'none', 'mean' or 'sum', got %r" % (reduction,))
 
