@@ -158,22 +158,6 @@ __device__ __forceinline__ void leave_table(const Table& t, char* ws) {
 __device__ __forceinline__ const Table& table_of(const char* ws) { return *reinterpret_cast<const Table*>(ws); }
 constexpr size_t kTableBytes = (sizeof(Table) + 255) / 256 * 256;
 
-// M <- mu M + G in place where there is a momentum; the update U.
-template <int T>
-__device__ __forceinline__ float advance(const Mat& q, const Step& s, long long i) {
-  const float g = load_float<T>(q.grad, i);
-  if (q.momentum == nullptr) return g;
-  const float m = s.mu * q.momentum[i] + g;
-  q.momentum[i] = m;
-  return s.nesterov ? g + s.mu * m : m;
-}
-// U once M is new
-template <int T>
-__device__ __forceinline__ float update_of(const Mat& q, const Step& s, long long i) {
-  if (q.momentum == nullptr) return load_float<T>(q.grad, i);
-  const float m = q.momentum[i];
-  return s.nesterov ? load_float<T>(q.grad, i) + s.mu * m : m;
-}
 // The results of a lane, sixteen of them at at(e) where inside(e): the old weights are all asked for before the first result is written.
 template <int T, class A, class I>
 __device__ __forceinline__ void put_results(const Mat& q, const Step& s, A at, I inside, const float (&o)[16]) {
@@ -221,17 +205,40 @@ __device__ __forceinline__ void put_results4(const Mat& q, const Step& s, A at, 
 constexpr int kLdU = 66;  // LDS row of 64 columns of U, doubles
 constexpr int kLdM = 66;  // LDS row of an m x m matrix
 
-// 64 columns of U from column `col0` of the long side on, as doubles; rows and columns behind the matrix are zeros.
+// 64 columns of U from column `col0` of the long side on, as doubles; rows and columns behind the matrix are zeros.  A thread's
+// loads are all on their way before the first of them is used.
 template <int T, bool ADVANCE>
 __device__ __forceinline__ void load_columns(const Mat& q, const Step& s, int col0, double (*u)[kLdU]) {
-  const int rows = (q.m + 15) & ~15;
-#pragma unroll 8
-  for (int e = threadIdx.x; e < rows * 64; e += 256) {
-    const int i = q.tall ? e % rows : e >> 6, j = q.tall ? e / rows : e & 63;
-    float v = 0.f;
-    if (i < q.m && col0 + j < q.n) {
-      const long long at = q.tall ? (long long)(col0 + j) * q.m + i : (long long)i * q.n + col0 + j;
-      v = ADVANCE ? advance<T>(q, s, at) : update_of<T>(q, s, at);
+  const int rows = (q.m + 15) & ~15, each = rows / 4;  // elements a thread
+  const auto place = [&](int e, int& i, int& j) {
+    const int id = e * 256 + threadIdx.x;
+    j = q.tall ? id / rows : id & 63;
+    i = q.tall ? id - j * rows : id >> 6;
+    return i < q.m && col0 + j < q.n;
+  };
+  const auto at = [&](int i, int j) { return q.tall ? (long long)(col0 + j) * q.m + i : (long long)i * q.n + col0 + j; };
+  float g[16], m[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    int i, j;
+    g[e] = m[e] = 0.f;
+    if (e < each && place(e, i, j)) {
+      g[e] = load_float<T>(q.grad, at(i, j));
+      if (q.momentum != nullptr) m[e] = q.momentum[at(i, j)];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    if (e >= each) continue;
+    int i, j;
+    const bool inside = place(e, i, j);
+    float v = g[e];
+    if (q.momentum != nullptr) {
+      if (ADVANCE) {
+        m[e] = s.mu * m[e] + g[e];
+        if (inside) q.momentum[at(i, j)] = m[e];
+      }
+      v = s.nesterov ? g[e] + s.mu * m[e] : m[e];
     }
     u[i][j] = (double)v;
   }
@@ -374,41 +381,69 @@ __global__ __launch_bounds__(kPolyThreads) void narrow_polynomial(Step s, char* 
     polynomial_of<4>(q, s, ws, smem);
 }
 
-// Q U, 64 columns per workgroup.
+// Q U, 64 columns per workgroup, 16 of them a wave.
+template <int T, int NT>
+__device__ __forceinline__ void apply_of(const Mat& q, const Step& s, char* ws, int col0, double (*u)[kLdU], double (*w)[kLdM]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j0 = wave * 16;
+  const double* in = reinterpret_cast<const double*>(ws + q.square_at);
+  double v[NT * NT];  // asked for before the columns, whose loads wait for nothing of it
+#pragma unroll
+  for (int k = 0; k < NT * NT; ++k) v[k] = in[k * 256 + threadIdx.x];
+  load_columns<T, false>(q, s, col0, u);
+#pragma unroll
+  for (int k = 0; k < NT * NT; ++k) {
+    const int e = k * 256 + threadIdx.x;
+    w[e / (NT * 16)][e % (NT * 16)] = v[k];
+  }
+  __syncthreads();
+  double y[NT * 4];
+#pragma unroll
+  for (int k = 0; k < NT * 4; ++k) y[k] = u[4 * k + (lane >> 4)][j0 + (lane & 15)];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    double x[NT * 4];
+#pragma unroll
+    for (int k = 0; k < NT * 4; ++k) x[k] = w[4 * k + (lane >> 4)][i * 16 + (lane & 15)];
+    // the matrix' own order of elements decides which side lies along the lanes; Q is symmetric
+    f64x4 even = {}, odd = {};
+    if (q.tall) {
+#pragma unroll
+      for (int k = 0; k < NT * 4; k += 2) {
+        even = __builtin_amdgcn_mfma_f64_16x16x4f64(y[k], x[k], even, 0, 0, 0);
+        odd = __builtin_amdgcn_mfma_f64_16x16x4f64(y[k + 1], x[k + 1], odd, 0, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < NT * 4; k += 2) {
+        even = __builtin_amdgcn_mfma_f64_16x16x4f64(x[k], y[k], even, 0, 0, 0);
+        odd = __builtin_amdgcn_mfma_f64_16x16x4f64(x[k + 1], y[k + 1], odd, 0, 0, 0);
+      }
+    }
+    const auto row = [&](int r) { return i * 16 + (q.tall ? lane & 15 : (lane >> 4) + 4 * r); };
+    const auto col = [&](int r) { return col0 + j0 + (q.tall ? (lane >> 4) + 4 * r : lane & 15); };
+    float o[16];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = (float)(even[r] + odd[r]);
+    put_results<T>(q, s, [&](int r) { return q.tall ? (long long)col(r) * q.m + row(r) : (long long)row(r) * q.n + col(r); },
+                   [&](int r) { return r < 4 && row(r) < q.m && col(r) < q.n; }, o);
+  }
+}
+
 template <int T>
 __global__ __launch_bounds__(256) void narrow_apply(Tiles tiles, Step s, char* ws) {
   const Table& t = table_of(ws);
   const int k = find(tiles, t.count, blockIdx.x);
   const Mat& q = t.m[k];
   __shared__ double u[kNarrow][kLdU], w[kNarrow][kLdM];
-  const int nt = div_up(q.m, 16), col0 = (blockIdx.x - tiles.first[k]) * 64, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  load_columns<T, false>(q, s, col0, u);
-  const double* in = reinterpret_cast<const double*>(ws + q.square_at);
-#pragma unroll 8
-  for (int e = threadIdx.x; e < nt * 16 * nt * 16; e += 256) w[e / (nt * 16)][e % (nt * 16)] = in[e];
-  __syncthreads();
-  const int j0 = wave * 16;  // 16 columns a wave
-  for (int i = 0; i < nt; ++i) {
-    f64x4 acc = {};
-    // the matrix' own order of elements decides which side lies along the lanes; Q is symmetric
-    for (int p = 0; p < nt * 16; p += 16) {
-      double x[4], y[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        x[k] = w[p + 4 * k + (lane >> 4)][i * 16 + (lane & 15)], y[k] = u[p + 4 * k + (lane >> 4)][j0 + (lane & 15)];
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        acc = q.tall ? __builtin_amdgcn_mfma_f64_16x16x4f64(y[k], x[k], acc, 0, 0, 0)
-                     : __builtin_amdgcn_mfma_f64_16x16x4f64(x[k], y[k], acc, 0, 0, 0);
-    }
-    const auto row = [&](int r) { return i * 16 + (q.tall ? lane & 15 : (lane >> 4) + 4 * r); };
-    const auto col = [&](int r) { return col0 + j0 + (q.tall ? (lane >> 4) + 4 * r : lane & 15); };
-    float o[16];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) o[r] = (float)acc[r];
-    put_results<T>(q, s, [&](int r) { return q.tall ? (long long)col(r) * q.m + row(r) : (long long)row(r) * q.n + col(r); },
-                   [&](int r) { return r < 4 && row(r) < q.m && col(r) < q.n; }, o);
-  }
+  const int col0 = (blockIdx.x - tiles.first[k]) * 64;
+  if (q.m <= 16)
+    apply_of<T, 1>(q, s, ws, col0, u, w);
+  else if (q.m <= 32)
+    apply_of<T, 2>(q, s, ws, col0, u, w);
+  else if (q.m <= 48)
+    apply_of<T, 3>(q, s, ws, col0, u, w);
+  else
+    apply_of<T, 4>(q, s, ws, col0, u, w);
 }
 
 // ---- larger matrices: momentum, norm, X_0 --------------------------------------------------------------------------------
