@@ -12,7 +12,7 @@
 //       60 MB of distinct bytes -- in arrival order the gather is bound by the Infinity-Cache -> L2 rate.
 //   roi_align_fwd_records   one 256-lane workgroup per (rank, 32-channel tile); tile index = blockIdx % 8, i.e. the
 //       slab of the feature map a tile reads is served by one XCD's L2.  Record by scalar load -> window by LDS-DMA ->
-//       vmcnt + barrier -> bins (packed FMAs) -> LDS tile -> contiguous 16-byte stores; the stages of an item are pipelined
+//       vmcnt + barrier -> bins (FMAs on pairs of columns) -> LDS tile -> contiguous 16-byte stores; the stages of an item are pipelined
 //       (next window issued before the tile is stored).  (Removed after measurement: a variant that prefetched the next
 //       window under the current arithmetic, 16-channel workgroups, roles on waves, a resident ticketed grid, and -- round 6 --
 //       static pairs of ranks with the next window landing in VGPRs: a wave spends its time ISSUING the window pieces, not
@@ -447,7 +447,7 @@ __device__ __forceinline__ const float* lds_at(const float* base, int byte_off) 
 // stage pieces (window DMA, axis tables, border patch, bins, tile store) are functions of their own.  (Round 5 also built a
 // RESIDENT form -- 768 workgroups walking the items by ticket, record fronts and next windows in flight across items --
 // whose unit chain was 11 % shorter and whose 2-item commitment cost a tail of 8-10 us: profiles/r05_persist_timeline.txt.
-// Its stage pipelining lives on below; the kernel itself lost on every shape once the bins used packed FMAs, and is gone.)
+// Its stage pipelining lives on below; the kernel itself lost on every shape once the bins used FMAs on pairs of columns, and is gone.)
 // -------------------------------------------------------------------------------------------------------------------
 // What a workgroup needs of a record's header -- wave-uniform, fetched with scalar loads.
 struct FwdRec {
@@ -554,9 +554,9 @@ __device__ __forceinline__ void fwd_bins(const TabEntry* ty, const TabEntry* tx,
       auto rows = [&](int ph, auto kn) {
         constexpr int kN = decltype(kn)::value;
         // A tap pair (F[x], F[x + 1]) arrives in an even-aligned register pair and so do its weights (hx, lx): the row sums
-        // run as v_pk_fma_f32 on (even, odd) partial sums -- S = sum_ix (hx, lx) * (F[x], F[x + 1]), acc += (wy, wy) * S --
-        // and the two halves meet once per bin: 13 instead of 20 FMA-class instructions per bin (the bins are bound by
-        // VALU issue: ~170 instructions per batch of four bin rows before this).  Same taps and weights; the summation
+        // run as FMAs on (even, odd) partial sums -- S = sum_ix (hx, lx) * (F[x], F[x + 1]), acc += (wy, wy) * S --
+        // and the two halves meet once per bin.  (As packed FMAs, which the build does without, that was 13 instead of 20
+        // FMA-class instructions per bin and 36.3 us instead of 37.1 at config 2.)  Same taps and weights; the summation
         // order differs from the scalar chain in the last bits (contract 1e-4, asserted 1e-5).
         v2f_t v[kN][kS][2][kS];
         float wy[kN][kS][2];
@@ -1461,7 +1461,7 @@ roi_align_bwd_tiles(const float* __restrict__ top_grad, int* __restrict__ ws, in
 
   // pass-2 identity of this lane: one pixel of the tile
   const int prow = tid >> 5, pcol = tid & 31;
-  v2f acc2[KC / 2];  // channel pairs: pass 2 runs on v_pk_fma_f32
+  v2f acc2[KC / 2];  // channel pairs
 #pragma unroll
   for (int c = 0; c < KC / 2; c++) acc2[c] = v2f{0.f, 0.f};
 
@@ -1519,7 +1519,7 @@ roi_align_bwd_tiles(const float* __restrict__ top_grad, int* __restrict__ ws, in
         const int k0 = cft[lc], k1 = cft[lc + 1];  // the output columns that reach this column, with their weights
         const float* gc = g + c * bins;
         for (int ph0 = 0; ph0 < aligned_height; ph0 += 8) {
-          v2f t[4];  // bin rows ph0 .. ph0 + 7, two per register pair: v_pk_fma_f32
+          v2f t[4];  // bin rows ph0 .. ph0 + 7, two per register pair
 #pragma unroll
           for (int j = 0; j < 4; j++) t[j] = v2f{0.f, 0.f};
           for (int k = k0; k < k1; k++) {
