@@ -77,8 +77,9 @@ def build(force=False, verbose=True):
         out, _ = p.communicate()
         if p.returncode != 0:
             raise RuntimeError("hipcc failed on %s:\n%s" % (src, out.decode(errors="replace")))
-        if verbose and out.strip():
-            sys.stderr.write(out.decode(errors="replace"))
+        said = [line for line in out.decode(errors="replace").splitlines() if "not a recognized feature" not in line]
+        if verbose and any(line.strip() for line in said):   # (the host pass does not know the device's feature names)
+            sys.stderr.write("\n".join(said) + "\n")
         objs.append(obj)
     tmp = LIB_PATH + ".tmp"
     subprocess.check_call([hipcc(), "--offload-arch=" + ARCH, "-shared", "-fPIC"] + objs + ["-o", tmp])

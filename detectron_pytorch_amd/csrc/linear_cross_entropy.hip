@@ -874,6 +874,9 @@ int check_sizes(int rows, int dim, int classes, int dtype) {
   MI_REQUIRE(dim >= 1 && dim <= (1 << 20), "linear_cross_entropy: %d features, 1 to 2^20 are taken", dim);
   MI_REQUIRE(classes >= 1 && classes <= (1 << 24), "linear_cross_entropy: %d classes, 1 to 2^24 are taken", classes);
   MI_REQUIRE(dtype == MI_TYPE_F32 || dtype == MI_TYPE_F16 || dtype == MI_TYPE_BF16, "linear_cross_entropy: dtype %d", dtype);
+  const long long r = ceil_div(rows, 64), d = ceil_div(dim, 64), c = ceil_div(classes, 64);
+  MI_REQUIRE(r * c < (1LL << 30) && r * d < (1LL << 30) && c * d < (1LL << 30),
+             "linear_cross_entropy: %d rows x %d features x %d classes are more tiles than a launch takes", rows, dim, classes);
   return MI_OK;
 }
 

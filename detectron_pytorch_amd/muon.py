@@ -58,17 +58,24 @@ def as_matrix(t):
     """A dense parameter of two or more dimensions as a contiguous matrix [out, rest] over the same memory, None for other
     layouts.  A channels-last weight is the matrix with its columns in memory order: orthogonalisation does not depend on the
     order of columns."""
+    rows = t.size(0)
+    cols = t.numel() // rows if rows else 0
     if t.is_contiguous():
-        return t.view(t.size(0), -1)
+        return t.view(rows, cols)
     if t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last):
-        return t.permute(0, 2, 3, 1).reshape(t.size(0), -1)
+        return t.permute(0, 2, 3, 1).reshape(rows, cols)
     return None
+
+
+def _same_order(t, like):
+    """Whether `t` lies in memory as `like` does (dimensions of one element aside)."""
+    return (t.is_contiguous() and like.is_contiguous()) or t.stride() == like.stride()
 
 
 class Muon(torch.optim.Optimizer):
     """Parameters of two or more dimensions take the orthogonalised step with `lr`, the others momentum SGD with `sgd_lr`
     (lr when None) and `sgd_momentum`.  Per group as usual: {"params": ..., "lr": ..., "sgd_lr": ..., "weight_decay": ...};
-    "orthogonalize": False keeps a group's matrices on SGD too."""
+    "orthogonalize": False keeps a group's matrices on SGD too.  Momenta are float32, whatever the parameter's type."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, sgd_lr=None, sgd_momentum=0.9,
                  steps=STEPS, coefficients=COEFFICIENTS, eps=EPS, orthogonalize=True):
@@ -80,9 +87,21 @@ class Muon(torch.optim.Optimizer):
 
     def _momentum(self, p):
         state = self.state[p]
-        if "momentum_buffer" not in state:
-            state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
-        return state["momentum_buffer"]
+        buf = state.get("momentum_buffer")
+        if buf is None:
+            buf = state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+        elif not _same_order(buf, p):   # the parameter was given another memory format
+            buf = state["momentum_buffer"] = torch.empty_like(p, dtype=torch.float32).copy_(buf)
+        return buf
+
+    def load_state_dict(self, state_dict):
+        """As torch's, which gives states their parameter's type; momenta keep their own."""
+        super().load_state_dict(state_dict)
+        for group, saved in zip(self.param_groups, state_dict["param_groups"]):
+            for p, key in zip(group["params"], saved["params"]):
+                buf = state_dict["state"].get(key, {}).get("momentum_buffer")
+                if buf is not None:
+                    self.state[p]["momentum_buffer"] = torch.empty_like(p, dtype=torch.float32).copy_(buf)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -91,36 +110,42 @@ class Muon(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for group in self.param_groups:
-            by_kind = {}
+            matrices, others = {}, {}
             for p in group["params"]:
-                if p.grad is None:
+                if p.grad is None or p.numel() == 0:
                     continue
                 if p.grad.is_sparse:
                     raise ValueError("Muon does not take sparse gradients")
                 if group["orthogonalize"] and p.dim() >= 2:
-                    m = as_matrix(p)
-                    if m is None:
+                    if as_matrix(p) is None:
                         raise ValueError("Muon updates dense parameters (contiguous or channels-last), got strides %s"
                                          % (p.stride(),))
-                    buf = self._momentum(p)
-                    grad = p.grad if p.grad.stride() == p.stride() else torch.empty_like(p).copy_(p.grad)
-                    mats = by_kind.setdefault((p.device, p.dtype), ([], [], []))
-                    for to, t in zip(mats, (p, grad, buf)):
+                    grad = p.grad if _same_order(p.grad, p) else torch.empty_like(p).copy_(p.grad)
+                    mats = matrices.setdefault((p.device, p.dtype), ([], [], []))
+                    for to, t in zip(mats, (p, grad, self._momentum(p))):
                         to.append(as_matrix(t))
                 else:
-                    self._sgd(p, group)
-            for params, grads, momenta in by_kind.values():
+                    for to, t in zip(others.setdefault((p.device, p.dtype), ([], [], [])), (p, p.grad, self._momentum(p))):
+                        to.append(t)
+            for params, grads, momenta in matrices.values():
                 muon_step_(params, grads, momenta, lr=group["lr"], momentum=group["momentum"],
                            weight_decay=group["weight_decay"], nesterov=group["nesterov"], steps=group["steps"],
                            coefficients=group["coefficients"], eps=group["eps"])
+            for params, grads, momenta in others.values():
+                _sgd_step_(params, grads, momenta, group["lr"] if group["sgd_lr"] is None else group["sgd_lr"],
+                           group["sgd_momentum"], group["weight_decay"])
         return loss
 
-    def _sgd(self, p, group):
-        """torch.optim.SGD's momentum step (coupled weight decay, no dampening)."""
-        lr = group["lr"] if group["sgd_lr"] is None else group["sgd_lr"]
-        buf = self._momentum(p)
-        g = p.grad.float()
-        if group["weight_decay"]:
-            g = g + group["weight_decay"] * p.float()
-        buf.mul_(group["sgd_momentum"]).add_(g)
-        p.sub_((lr * buf).to(p.dtype))
+
+def _sgd_step_(params, grads, momenta, lr, momentum, weight_decay):
+    """torch.optim.SGD's momentum step (coupled weight decay, no dampening) of a list, in float32."""
+    grads = [g.float() for g in grads]
+    torch._foreach_mul_(momenta, momentum)
+    torch._foreach_add_(momenta, grads)
+    if weight_decay:
+        torch._foreach_add_(momenta, [p.float() for p in params], alpha=weight_decay)
+    if params[0].dtype == torch.float32:
+        torch._foreach_add_(params, momenta, alpha=-lr)
+    else:   # rounded once
+        for p, m in zip(params, momenta):
+            p.copy_(p.float() - lr * m)

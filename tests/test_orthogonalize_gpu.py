@@ -230,6 +230,13 @@ def test_optimizer_over_a_module():
         opt.step()
         for p in net.parameters():
             assert float((p.detach().double() - want[p]).abs().max()) <= 1e-3 * 0.02 + 2.0 ** -22 * float(want[p].abs().max())
+    net[0] = net[0].to(memory_format=torch.channels_last)      # in the middle of training
+    opt.zero_grad()
+    net(torch.randn(2, 3, 8, 8, device=DEV)).square().sum().backward()
+    p = net[0].weight
+    w, _ = reference_step(p.detach().reshape(8, -1), p.grad.reshape(8, -1), momenta[p].reshape(8, -1), 0.02, 0.95, 0.01)
+    opt.step()
+    assert float((p.detach().reshape(8, -1).double() - w).abs().max()) <= 1e-3 * 0.02 + 2.0 ** -22
     saved = opt.state_dict()
     other = Muon(net.parameters(), lr=0.02, sgd_lr=0.1, weight_decay=0.01)
     other.load_state_dict(saved)

@@ -56,6 +56,39 @@ def test_biases_take_the_sgd_step():
         assert torch.allclose(ours, theirs, rtol=0, atol=2.0 ** -20)
 
 
+def test_momenta_stay_float32_through_a_checkpoint():
+    p = torch.nn.Parameter(torch.randn(7).bfloat16())
+    opt = Muon([p], lr=0.3)
+    p.grad = torch.randn(7).bfloat16() / 3
+    opt.step()
+    opt.step()
+    buf = opt.state[p]["momentum_buffer"]
+    assert buf.dtype == torch.float32
+    q = torch.nn.Parameter(p.detach().clone())
+    other = Muon([q], lr=0.3)
+    other.load_state_dict(opt.state_dict())
+    assert other.state[q]["momentum_buffer"].dtype == torch.float32
+    assert torch.equal(other.state[q]["momentum_buffer"], buf) and other.state[q]["momentum_buffer"] is not buf
+    q.grad = p.grad.clone()
+    opt.step()
+    other.step()
+    assert torch.equal(p, q)
+
+
+def test_momentum_follows_the_parameters_memory_format():
+    w = torch.nn.Parameter(torch.randn(4, 3, 2, 2))
+    opt = Muon([w], orthogonalize=False)
+    w.grad = torch.randn(4, 3, 2, 2)
+    opt.step()
+    before = opt.state[w]["momentum_buffer"].clone()
+    w.data = w.data.contiguous(memory_format=torch.channels_last)
+    assert torch.equal(opt._momentum(w), before) and opt._momentum(w).stride() == w.stride()
+    empty = torch.nn.Parameter(torch.zeros(0, 5))
+    empty.grad = torch.zeros(0, 5)
+    Muon([empty]).step()
+    assert as_matrix(empty).shape == (0, 0)
+
+
 def test_as_matrix():
     w = torch.arange(2 * 3 * 4 * 5.0).view(2, 3, 4, 5)
     assert torch.equal(as_matrix(w), w.view(2, 60)) and as_matrix(w).data_ptr() == w.data_ptr()
@@ -74,7 +107,8 @@ def test_loss_arguments_at_the_boundary(hip_lib_path):
                                                  saved, saved_bytes, room, room_bytes, NULL)
 
     for bad in (dict(x=NULL), dict(w=NULL), dict(y=NULL), dict(loss=NULL), dict(saved=NULL), dict(room=NULL), dict(rows=0),
-                dict(rows=-1), dict(rows=1 << 25), dict(dim=0), dict(classes=0), dict(classes=1 << 25), dict(dtype=3),
+                dict(rows=-1), dict(rows=1 << 25), dict(dim=0), dict(classes=0), dict(classes=1 << 25),
+                dict(rows=1 << 24, classes=1 << 24), dict(dtype=3),
                 dict(dtype=-1), dict(xs=7), dict(ws=7), dict(ws=1 << 23), dict(reduction=3), dict(reduction=-1),
                 dict(saved=ctypes.c_void_p(4100)), dict(room=ctypes.c_void_p(4100))):
         assert forward(**bad) == 1 and b"linear_cross_entropy" in h.mi_last_error(), bad
