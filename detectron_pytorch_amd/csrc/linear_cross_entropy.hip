@@ -477,32 +477,30 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_backward
 #pragma unroll
     for (int j = 0; j < P::FN; ++j)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int col = col0 + j * 32 + g * 8;
-        s16x4 hi, lo;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float v = acc[i][j][g * 4 + r];
-          sum[j][g * 4 + r] += v;
-          if constexpr (P::SPLIT) {
-            const _Float16 h = (_Float16)v;
-            hi[r] = __builtin_bit_cast(short, h);
-            lo[r] = (short)half_bits(v - (float)h);
-          } else {
-            hi[r] = (short)round16<T>(v);
-          }
-        }
-        if (in && col < classes_p) {
-          if constexpr (P::SPLIT) {
-            uint16_t* at = q + row * ld + (col >> 5) * 64 + (col & 31);
-            *reinterpret_cast<s16x4*>(at) = hi;
-            *reinterpret_cast<s16x4*>(at + 32) = lo;
-          } else {
-            *reinterpret_cast<s16x4*>(q + row * ld + col) = hi;
-          }
-        }
-      }
+      for (int e = 0; e < 16; ++e) sum[j][e] += acc[i][j][e];
   }
+  P::hand_out(acc, (lds_bytes)smem, [&](int r, int c, f32x4 v) {
+    const int row = tm * P::BM + r, col = tn * P::BN + c;
+    if (row >= rows_p || col >= classes_p) return;
+    s16x4 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (P::SPLIT) {
+        const _Float16 h = (_Float16)v[k];
+        hi[k] = __builtin_bit_cast(short, h);
+        lo[k] = (short)half_bits(v[k] - (float)h);
+      } else {
+        hi[k] = (short)round16<T>(v[k]);
+      }
+    }
+    if constexpr (P::SPLIT) {
+      uint16_t* at = q + row * ld + (col >> 5) * 64 + (col & 31);
+      *reinterpret_cast<s16x4*>(at) = hi;
+      *reinterpret_cast<s16x4*>(at + 32) = lo;
+    } else {
+      *reinterpret_cast<s16x4*>(q + row * ld + col) = hi;
+    }
+  });
   if (sums == nullptr) return;
   const int strip = tm * P::WR + uniform((int)(threadIdx.x >> 6)) / P::WC;
 #pragma unroll
@@ -539,45 +537,35 @@ __device__ __forceinline__ void gradient_tile(const Gradient& g, int id, const F
   f32x16 acc[P::FM][P::FN];
   const int step0 = slice * g.per_slice;
   P::run(acc, g.a, g.b, tm * P::BM, tn * P::BN, step0, min(g.per_slice, g.steps - step0), lds);
-  const int row0 = tm * P::BM + P::lane_row(), col0 = tn * P::BN + P::lane_col();
   const float f = value(factor) * (P::SPLIT ? (OF_WEIGHT ? factor.sc->inv_x : factor.sc->inv_w) : 1.f);
   const bool whole = (g.cols & 3) == 0;  // then every four columns of a lane are inside or outside together, and aligned
-#pragma unroll
-  for (int i = 0; i < P::FM; ++i) {
-    const int row = row0 + i * 32;
-    if (row >= g.rows) continue;
-#pragma unroll
-    for (int j = 0; j < P::FN; ++j)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int col = col0 + j * 32 + k * 8;
-        if (col >= g.cols) continue;
-        f32x4 v = P::quad(acc[i][j], k);
-        if (g.slices != nullptr) {
-          float* at = g.slices + ((long long)slice * g.rows + row) * g.cols + col;
-          if (whole) {
-            if (g.add) v += *reinterpret_cast<const f32x4*>(at);
-            *reinterpret_cast<f32x4*>(at) = v;
-          } else {
-            for (int r = 0; r < 4; ++r)
-              if (col + r < g.cols) at[r] = g.add ? at[r] + v[r] : v[r];
-          }
-        } else {
-          v *= f;
-          const long long at = (long long)row * g.cols + col;
-          if (whole && T == MI_TYPE_F32) {
-            *reinterpret_cast<f32x4*>(static_cast<float*>(g.out) + at) = v;
-          } else if (whole) {
-            s16x4 h;
-            for (int r = 0; r < 4; ++r) h[r] = (short)round16<T>(v[r]);
-            *reinterpret_cast<s16x4*>(static_cast<uint16_t*>(g.out) + at) = h;
-          } else {
-            for (int r = 0; r < 4; ++r)
-              if (col + r < g.cols) store_from_float<T>(g.out, at + r, v[r]);
-          }
-        }
+  P::hand_out(acc, lds, [&](int r0, int c0, f32x4 v) {
+    const int row = tm * P::BM + r0, col = tn * P::BN + c0;
+    if (row >= g.rows || col >= g.cols) return;
+    if (g.slices != nullptr) {
+      float* at = g.slices + ((long long)slice * g.rows + row) * g.cols + col;
+      if (whole) {
+        if (g.add) v += *reinterpret_cast<const f32x4*>(at);
+        *reinterpret_cast<f32x4*>(at) = v;
+      } else {
+        for (int r = 0; r < 4; ++r)
+          if (col + r < g.cols) at[r] = g.add ? at[r] + v[r] : v[r];
       }
-  }
+      return;
+    }
+    v *= f;
+    const long long at = (long long)row * g.cols + col;
+    if (whole && T == MI_TYPE_F32) {
+      *reinterpret_cast<f32x4*>(static_cast<float*>(g.out) + at) = v;
+    } else if (whole) {
+      s16x4 h;
+      for (int r = 0; r < 4; ++r) h[r] = (short)round16<T>(v[r]);
+      *reinterpret_cast<s16x4*>(static_cast<uint16_t*>(g.out) + at) = h;
+    } else {
+      for (int r = 0; r < 4; ++r)
+        if (col + r < g.cols) store_from_float<T>(g.out, at + r, v[r]);
+    }
+  });
 }
 
 // All gradients of a piece in one launch: the tiles of q W, those of q' x, and the bias' columns, 64 a workgroup.

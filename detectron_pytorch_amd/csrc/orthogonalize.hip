@@ -171,32 +171,21 @@ __device__ __forceinline__ void put_results(const Mat& q, const Step& s, A at, I
   for (int e = 0; e < 16; ++e)
     if (inside(e)) store_float<T>(q.out, at(e), s.update ? w[e] * s.decay - s.lr * q.shape * o[e] : o[e]);
 }
-// The same for four groups of four on their alignment.
-template <int T, class A, class I>
-__device__ __forceinline__ void put_results4(const Mat& q, const Step& s, A at, I inside, const float (&o)[16]) {
-  f32x4 w[4] = {};
-  if (s.update) {
+// Four of them on their alignment, with the old weights.
+template <int T>
+__device__ __forceinline__ void put_result4(const Mat& q, const Step& s, long long i, f32x4 o, f32x4 w) {
+  if (s.update) o = w * s.decay - (s.lr * q.shape) * o;
+  if constexpr (T == MI_TYPE_F32) {
+    *reinterpret_cast<f32x4*>(static_cast<float*>(q.out) + i) = o;
+  } else {
+    s16x4 h;
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
-      if (inside(g * 4)) w[g] = load_four<T>(q.out, at(g * 4), 4, true);
-  }
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    if (!inside(g * 4)) continue;
-    f32x4 v = {o[g * 4], o[g * 4 + 1], o[g * 4 + 2], o[g * 4 + 3]};
-    if (s.update) v = w[g] * s.decay - (s.lr * q.shape) * v;
-    if constexpr (T == MI_TYPE_F32) {
-      *reinterpret_cast<f32x4*>(static_cast<float*>(q.out) + at(g * 4)) = v;
-    } else {
-      s16x4 h;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        short one;
-        store_float<T>(&one, 0, v[r]);
-        h[r] = one;
-      }
-      *reinterpret_cast<s16x4*>(static_cast<uint16_t*>(q.out) + at(g * 4)) = h;
+    for (int r = 0; r < 4; ++r) {
+      short one;
+      store_float<T>(&one, 0, o[r]);
+      h[r] = one;
     }
+    *reinterpret_cast<s16x4*>(static_cast<uint16_t*>(q.out) + i) = h;
   }
 }
 
@@ -540,28 +529,35 @@ __global__ __launch_bounds__(256) void normalize(Tiles tiles, Tiles norm, Step s
 
 // ---- larger matrices: the products ---------------------------------------------------------------------------------------
 
-// A symmetric result's tile of the upper triangle, on both sides (the padding of a row lies in its upper half).
-template <class P, class F>
-__device__ __forceinline__ void put_symmetric(uint16_t* out, int m, int ti, int tj, F element) {
-  const int ld = up32(m), row0 = ti * P::BM + P::lane_row(), col0 = tj * P::BN + P::lane_col();
+// A symmetric result's tile of the upper triangle, on both sides (the padding of a row lies in its upper half).  `finish(row, col,
+// v, old)` is what is still done to four columns of a row, `before(row, col)` what it wants to know of the place.
+template <class P, class B, class F>
+__device__ __forceinline__ void put_symmetric(f32x16 (&acc)[P::FM][P::FN], lds_bytes lds, uint16_t* out, int m, int ti, int tj,
+                                              B before, F finish) {
+  const int ld = up32(m);
+  const auto asked = [&](int r, int c, bool turned) {
+    const int row = ti * P::BM + r, col = tj * P::BN + c;
+    if (turned ? col >= m : row >= m || col >= ld) return f32x4{0.f, 0.f, 0.f, 0.f};
+    return turned ? before(col, row) : before(row, col);
+  };
+  const auto by_row = [&](int r, int c, f32x4 v, f32x4 old) {
+    const int row = ti * P::BM + r, col = tj * P::BN + c;
+    if (row >= m || col >= ld) return;
+    v = finish(row, col, v, old);
 #pragma unroll
-  for (int i = 0; i < P::FM; ++i)
-#pragma unroll
-    for (int j = 0; j < P::FN; ++j)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int row = row0 + i * 32, col = col0 + j * 32 + g * 8;
-        if (row >= m || col >= ld) continue;
-        f32x4 v = element(i, j, g, row, col);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (col + r >= m) v[r] = 0.f;
-        put_split4(out + split_at(row, col, ld), v);
-        if (ti != tj)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (col + r < m) put_split(out + split_at(col + r, row, ld), v[r]);
-      }
+    for (int k = 0; k < 4; ++k)
+      if (col + k >= m) v[k] = 0.f;
+    put_split4(out + split_at(row, col, ld), v);
+  };
+  if (ti == tj) {
+    P::template hand_out<false>(acc, lds, asked, by_row, typename P::Nothing{});
+    return;
+  }
+  // rows of the transposed tile: ti is not the last tile, so its 4 rows are all inside
+  P::template hand_out<true>(acc, lds, asked, by_row, [&](int r, int c, f32x4 v, f32x4 old) {
+    const int row = ti * P::BM + r, col = tj * P::BN + c;
+    if (col < m) put_split4(out + split_at(col, row, ld), finish(col, row, v, old));
+  });
 }
 
 // A = X X': one tile of the upper triangle and one slice of the sum over n.  With one slice the tile is written as it is; slices leave
@@ -588,8 +584,9 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void gram(Tiles tile
   f32x16 acc[P::FM][P::FN];
   P::run(acc, x, x, ti * P::BM, tj * P::BN, step0, min(each, steps - step0), (lds_bytes)smem);
   if (q.slices == 1) {
-    put_symmetric<P>(reinterpret_cast<uint16_t*>(ws + q.square_at), q.m, ti, tj,
-                     [&](int i, int j, int g, int, int) { return P::quad(acc[i][j], g) * kGramFactor; });
+    put_symmetric<P>(acc, (lds_bytes)smem, reinterpret_cast<uint16_t*>(ws + q.square_at), q.m, ti, tj,
+                     [](int, int) { return f32x4{0.f, 0.f, 0.f, 0.f}; },
+                     [](int, int, f32x4 v, f32x4) { return v * kGramFactor; });
     return;
   }
 #pragma unroll
@@ -652,16 +649,17 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void square(Tiles ti
   f32x16 acc[P::FM][P::FN];
   P::run(acc, {l, (long long)ld * 2, q.m, ld}, {at(s.right), (long long)ld * 2, q.m, ld}, ti * P::BM, tj * P::BN, 0, ld / 32,
          (lds_bytes)smem);
-  put_symmetric<P>(at(s.out), q.m, ti, tj, [&](int i, int j, int g, int row, int col) {
-    f32x4 v = P::quad(acc[i][j], g) * s.f0;
-    if (s.f1 != 0.f) {
-      v += get_split4(l + split_at(row, col, ld)) * s.f1;
+  // L is symmetric, so the transposed side finds its element of it at its own place
+  put_symmetric<P>(acc, (lds_bytes)smem, at(s.out), q.m, ti, tj,
+                   [&](int row, int col) {
+                     return s.f1 != 0.f ? get_split4(l + split_at(row, col, ld)) : f32x4{0.f, 0.f, 0.f, 0.f};
+                   },
+                   [&](int row, int col, f32x4 v, f32x4 old) {
+                     v = v * s.f0 + old * s.f1;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (row == col + r) v[r] += s.fi;
-    }
-    return v;
-  });
+                     for (int r = 0; r < 4; ++r) v[r] += row == col + r ? s.fi : 0.f;
+                     return v;
+                   });
 }
 
 // X <- C X (or Q X, several iterations at once), or in the last pass the result itself.
@@ -680,31 +678,42 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void apply(Tiles til
   f32x16 acc[P::FM][P::FN];
   P::run(acc, {c, (long long)ldm * 2, q.m, ldm}, {x, (long long)ld * 2, q.n, q.m}, tm * P::BM, tn * P::BN, 0, ldm / 32,
          (lds_bytes)smem);
+  if constexpr (!LAST) {
+    P::hand_out(acc, (lds_bytes)smem, [&](int r, int c, f32x4 v) {
+      const int row = tm * P::BM + r, col = tn * P::BN + c;
+      if (row < q.m && col < ld) put_split4(y + split_at(row, col, ld), v * (1.f / kScaleC));
+    });
+    return;
+  }
+  constexpr float f = 1.f / (kScaleC * kScaleX);
+  if (!q.tall && aligned16(q.out) && q.n % 4 == 0) {
+    P::template hand_out<false>(
+        acc, (lds_bytes)smem,
+        [&](int r, int c, bool) {
+          const int row = tm * P::BM + r, col = tn * P::BN + c;
+          if (!s.update || row >= q.m || col >= q.n) return f32x4{0.f, 0.f, 0.f, 0.f};
+          return load_four<T>(q.out, (long long)row * q.n + col, 4, true);
+        },
+        [&](int r, int c, f32x4 v, f32x4 old) {
+          const int row = tm * P::BM + r, col = tn * P::BN + c;
+          if (row < q.m && col < q.n) put_result4<T>(q, s, (long long)row * q.n + col, v * f, old);
+        },
+        typename P::Nothing{});
+    return;
+  }
   const int row0 = tm * P::BM + P::lane_row(), col0 = tn * P::BN + P::lane_col();
-  const bool whole = LAST && !q.tall && aligned16(q.out) && q.n % 4 == 0;
 #pragma unroll
   for (int i = 0; i < P::FM; ++i) {
     const int row = row0 + i * 32;
     if (row >= q.m) continue;
 #pragma unroll
     for (int j = 0; j < P::FN; ++j) {
-      const int col = col0 + j * 32;
-      if constexpr (!LAST) {
+      float o[16];
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-          if (col + g * 8 < ld) put_split4(y + split_at(row, col + g * 8, ld), P::quad(acc[i][j], g) * (1.f / kScaleC));
-      } else {
-        float o[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[e] = acc[i][j][e] * (1.f / (kScaleC * kScaleX));
-        const auto column = [&](int e) { return col + (e >> 2) * 8 + (e & 3); };
-        const auto at = [&](int e) { return q.tall ? (long long)column(e) * q.m + row : (long long)row * q.n + column(e); };
-        const auto inside = [&](int e) { return column(e) < q.n; };
-        if (whole)
-          put_results4<T>(q, s, at, inside, o);
-        else
-          put_results<T>(q, s, at, inside, o);
-      }
+      for (int e = 0; e < 16; ++e) o[e] = acc[i][j][e] * f;
+      const auto column = [&](int e) { return col0 + j * 32 + (e >> 2) * 8 + (e & 3); };
+      put_results<T>(q, s, [&](int e) { return q.tall ? (long long)column(e) * q.m + row : (long long)row * q.n + column(e); },
+                     [&](int e) { return column(e) < q.n; }, o);
     }
   }
 }
