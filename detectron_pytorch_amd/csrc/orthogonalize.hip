@@ -44,6 +44,8 @@ constexpr int kNormElements = 8192;  // elements for which one more workgroup is
 constexpr int kNarrow = 64, kNarrowLong = 16384;
 constexpr int kParts = 32;           // partial sums of A_0 in the fp64 way, at most
 
+constexpr int kBand = 4;             // tile rows of a band of the tiles' order
+
 enum { kA = 0, kC = 1, kQ = 2, kT = 3, kSquares = 4 };
 
 struct Mat {
@@ -573,12 +575,12 @@ template <class P>
 __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void gram(Tiles tiles, char* ws, int flip) {
   extern __shared__ char smem[];
   const Table& t = table_of(ws);
-  const int k = find(tiles, t.count, blockIdx.x);
+  const int block = run_of_xcd(blockIdx.x, gridDim.x), k = find(tiles, t.count, block);
   const Mat& q = t.m[k];
   const int nt = div_up(q.m, P::BM), per = triangle_tiles(nt);
-  const int id = blockIdx.x - tiles.first[k], slice = id / per, tile = id - slice * per;
+  const int id = block - tiles.first[k], slice = id / per, tile = id - slice * per;
   int ti, tj;
-  triangle(tile, nt, ti, tj);
+  tile_in_triangle(tile, nt, kBand, ti, tj);
   const int ld = up32(q.n), steps = ld / 32, each = div_up(steps, q.slices), step0 = slice * each;
   const Operand x = {reinterpret_cast<const uint16_t*>(ws + (flip ? q.y_at : q.x_at)), (long long)ld * 2, q.m, ld};
   f32x16 acc[P::FM][P::FN];
@@ -606,7 +608,7 @@ __global__ __launch_bounds__(P::kThreads) void join_gram(Tiles tiles, char* ws) 
   const int nt = div_up(q.m, P::BM), per = triangle_tiles(nt), ld = up32(q.m);
   const int id = blockIdx.x - tiles.first[k], tile = id / (P::FM * P::FN), f = id % (P::FM * P::FN), i = f / P::FN, j = f % P::FN;
   int ti, tj;
-  triangle(tile, nt, ti, tj);
+  tile_in_triangle(tile, nt, kBand, ti, tj);
   f32x4 v[4] = {};
 #pragma unroll 2
   for (int s = 0; s < q.slices; ++s)
@@ -639,10 +641,10 @@ template <class P>
 __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void square(Tiles tiles, Square s, char* ws) {
   extern __shared__ char smem[];
   const Table& t = table_of(ws);
-  const int k = find(tiles, t.count, blockIdx.x);
+  const int block = run_of_xcd(blockIdx.x, gridDim.x), k = find(tiles, t.count, block);
   const Mat& q = t.m[k];
   int ti, tj;
-  triangle(blockIdx.x - tiles.first[k], div_up(q.m, P::BM), ti, tj);
+  tile_in_triangle(block - tiles.first[k], div_up(q.m, P::BM), kBand, ti, tj);
   const int ld = up32(q.m);
   const auto at = [&](int i) { return reinterpret_cast<uint16_t*>(ws + q.square_at + i * q.square_bytes); };
   const uint16_t* l = at(s.left);
@@ -670,7 +672,8 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void apply(Tiles til
   const int k = find(tiles, t.count, blockIdx.x);
   const Mat& q = t.m[k];
   int tm, tn;
-  tile_of(blockIdx.x - tiles.first[k], div_up(q.m, P::BM), div_up(q.n, P::BN), 4, tm, tn);
+  // per matrix, not over the launch: the matrices' tiles take different times, and a run of long ones would keep one XCD
+  tile_of(blockIdx.x - tiles.first[k], div_up(q.m, P::BM), div_up(q.n, P::BN), kBand, tm, tn);
   const int ldm = up32(q.m), ld = up32(q.n);
   const uint16_t* x = reinterpret_cast<const uint16_t*>(ws + (flip ? q.y_at : q.x_at));
   uint16_t* y = reinterpret_cast<uint16_t*>(ws + (flip ? q.x_at : q.y_at));

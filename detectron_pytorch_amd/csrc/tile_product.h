@@ -363,16 +363,44 @@ struct TileProduct {
   }
 };
 
-// Workgroup -> tile.  Consecutive workgroups go to the 8 XCDs in turn: each XCD gets one contiguous run of the tile order,
-// which walks bands of `band` tile rows column by column, so that the tiles an XCD works on at a time share
-// rows of A and columns of B in its L2.
-__device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int band, int& tm, int& tn) {
-  const int total = tiles_m * tiles_n, q = total >> 3, r = total & 7, xcd = id & 7, pos = id >> 3;
-  const int t = xcd * q + min(xcd, r) + pos;
+// Consecutive workgroups go to the 8 XCDs in turn.  Workgroup -> place in an order of which each XCD gets one contiguous run.
+__device__ __forceinline__ int run_of_xcd(int id, int total) {
+  const int q = total >> 3, r = total & 7, xcd = id & 7;
+  return xcd * q + min(xcd, r) + (id >> 3);
+}
+// The t-th tile of an order that walks bands of `band` tile rows column by column, so that tiles that are near in it share rows of A and
+// columns of B: those an XCD works on at a time, in its L2.
+__device__ __forceinline__ void tile_in_bands(int t, int tiles_m, int tiles_n, int band, int& tm, int& tn) {
   const int per = band * tiles_n, b = t / per, in = t - b * per;
   const int high = min(band, tiles_m - b * band);
   tn = in / high;
   tm = b * band + in - tn * high;
+}
+__device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int band, int& tm, int& tn) {
+  tile_in_bands(run_of_xcd(id, tiles_m * tiles_n), tiles_m, tiles_n, band, tm, tn);
+}
+// The same order of the tiles on and above the diagonal of n x n.
+__device__ __forceinline__ void tile_in_triangle(int t, int n, int band, int& tm, int& tn) {
+  int first = 0;  // tile row the band begins with; its columns begin there too
+  for (;; first += band) {
+    const int high = min(band, n - first), wide = n - first, corner = high * (high + 1) / 2;
+    const int all = corner + (wide - high) * high;
+    if (t >= all) {
+      t -= all;
+      continue;
+    }
+    if (t >= corner) {
+      t -= corner;
+      tn = first + high + t / high;
+      tm = first + t % high;
+    } else {
+      int c = 0;
+      while (t > c) t -= ++c;
+      tn = first + c;
+      tm = first + t;
+    }
+    return;
+  }
 }
 
 template <bool SPLIT, bool BF16, bool AKM, bool BKM>
