@@ -460,7 +460,8 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_backward
   for (int i = 0; i < P::FM; ++i) {
     const int row = row0 + i * 32;
     const bool in = row < rows_p;
-    const int y = (in ? lab[row] : kIgnored) - class0 - col0;
+    const int label = in ? lab[row] : kIgnored, y = label - class0 - col0;
+    const bool ignored = label == kIgnored;
     const float l = in ? lse[row] : INFINITY;
     const float f = factors != nullptr ? (in ? factors[row] : 0.f) : kQScale;
 #pragma unroll
@@ -468,6 +469,12 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_backward
 #pragma unroll
       for (int e = 0; e < 16; ++e)
         acc[i][j][e] = __expf((P::SPLIT ? acc[i][j][e] * ix * iw : acc[i][j][e]) + b[j][e] - l) * f;
+    if (__any(ignored)) {  // rows that do not count, also beside a bias or weight that is no number
+#pragma unroll
+      for (int j = 0; j < P::FN; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = ignored ? 0.f : acc[i][j][e];
+    }
     if (__any(y >= 0 && y < P::FN * 32)) {
 #pragma unroll
       for (int j = 0; j < P::FN; ++j)
@@ -863,7 +870,8 @@ int check_sizes(int rows, int dim, int classes, int dtype) {
   MI_REQUIRE(classes >= 1 && classes <= (1 << 24), "linear_cross_entropy: %d classes, 1 to 2^24 are taken", classes);
   MI_REQUIRE(dtype == MI_TYPE_F32 || dtype == MI_TYPE_F16 || dtype == MI_TYPE_BF16, "linear_cross_entropy: dtype %d", dtype);
   const long long r = ceil_div(rows, 64), d = ceil_div(dim, 64), c = ceil_div(classes, 64);
-  MI_REQUIRE(r * c < (1LL << 30) && r * d < (1LL << 30) && c * d < (1LL << 30),
+  // tiles of 64 x 64; where there are many, those of 128 or 256 are taken, and a launch has at most 2^32 threads, 256 a tile
+  MI_REQUIRE(r * c < (1LL << 25) && r * d < (1LL << 25) && c * d < (1LL << 25),
              "linear_cross_entropy: %d rows x %d features x %d classes are more tiles than a launch takes", rows, dim, classes);
   return MI_OK;
 }

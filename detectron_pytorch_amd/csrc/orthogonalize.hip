@@ -27,7 +27,6 @@
 #include "tile_product.h"
 
 #include <cmath>
-#include <cstring>
 #include <type_traits>
 
 namespace mi {
@@ -943,49 +942,42 @@ int check_matrices(int count, const int* rows, const int* cols) {
   return MI_OK;
 }
 
-// growth[g]: the largest product of g successive factors C.  False for coefficients with which X or a single C leaves the range of
-// the stored forms.  Sampled over the singular values, with a margin for what lies between the samples.
-bool range_of(const float* c, int steps, double* growth) {
-  bool fits = std::isfinite(c[0]) && std::isfinite(c[1]) && std::isfinite(c[2]);
-  growth[1] = growth[2] = growth[3] = 0;
-  double top = 1.0;
-  for (int i = 0; i < steps && fits; ++i) {
-    double next = 0;
-    for (int k = 0; k <= 1024; ++k) {
-      double x = top * k / 1024, product = 1;
-      for (int g = 1; g <= 3 && i + g <= steps; ++g) {
-        const double x2 = x * x, factor = c[0] + x2 * (c[1] + x2 * c[2]);
-        product *= factor;
-        x *= factor;
-        if (g == 1) next = std::fmax(next, std::fabs(x));
-        growth[g] = std::fmax(growth[g], 1.001 * std::fabs(product));
-      }
-    }
-    next *= 1.001;
-    fits = next <= kMostX && growth[1] <= kMostC;
-    top = next;
+// growth[g]: a bound of the product of g successive factors C.  False for coefficients with which X or a single C leaves the range of
+// the stored forms.  Of singular values up to `top`, C = a + b t + c t^2 (t = s^2) is largest in magnitude at an end or its
+// vertex, s C at `top` or where a + 3 b t + 5 c t^2 = 0.
+bool range_of(const float* coefficients, int steps, double* growth) {
+  const double a = coefficients[0], b = coefficients[1], c = coefficients[2];
+  if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
+  const auto factor = [&](double t) { return std::fabs(a + t * (b + t * c)); };
+  const double vertex = c != 0 ? -b / (2 * c) : 0;
+  double turns[2] = {0, 0};  // t where s C turns
+  const double inside = 9 * b * b - 20 * a * c;
+  if (c == 0) {
+    if (b != 0) turns[0] = -a / (3 * b);
+  } else if (inside >= 0) {
+    turns[0] = (-3 * b + std::sqrt(inside)) / (10 * c), turns[1] = (-3 * b - std::sqrt(inside)) / (10 * c);
   }
-  return fits;
+  double top = 1, before = 0, second = 0;  // the two factors before
+  growth[1] = growth[2] = growth[3] = 0;
+  for (int i = 0; i < steps; ++i) {
+    const double t = top * top;
+    double most = std::fmax(factor(0), factor(t)), next = top * factor(t);
+    if (vertex > 0 && vertex < t) most = std::fmax(most, factor(vertex));
+    for (double u : turns)
+      if (u > 0 && u < t) next = std::fmax(next, std::sqrt(u) * factor(u));
+    if (!(next <= kMostX && most <= kMostC)) return false;
+    growth[1] = std::fmax(growth[1], most);
+    growth[2] = std::fmax(growth[2], most * before);
+    growth[3] = std::fmax(growth[3], most * before * second);
+    second = before, before = most, top = next;
+  }
+  return true;
 }
 
 int check_coefficients(const float* c, int steps, float eps, double* growth) {
   MI_REQUIRE(c != nullptr && steps >= 1 && steps <= 64, "orthogonalize: %d steps, 1 to 64 are taken", steps);
   MI_REQUIRE(eps > 0.f, "orthogonalize: eps must be positive");
-  // a program asks for the same polynomial all the time, and sampling it takes longer than launching: the last answer is kept
-  struct Answer {
-    float c[3];
-    int steps;
-    bool fits;
-    double growth[4];
-  };
-  thread_local Answer last = {};
-  if (last.steps != steps || std::memcmp(last.c, c, sizeof last.c) != 0) {
-    std::memcpy(last.c, c, sizeof last.c);
-    last.steps = steps;
-    last.fits = range_of(c, steps, last.growth);
-  }
-  for (int g = 1; g <= 3; ++g) growth[g] = last.growth[g];
-  if (!last.fits) {
+  if (!range_of(c, steps, growth)) {
     set_error("orthogonalize: coefficients (%g, %g, %g) let the iteration grow beyond %g", c[0], c[1], c[2], kMostX);
     return MI_ERR_UNSUPPORTED;
   }

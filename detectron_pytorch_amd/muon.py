@@ -16,6 +16,23 @@ from . import _lib
 from .orthogonalize import COEFFICIENTS, EPS, STEPS, check_matrices, host_arrays, pointers, workspace_for
 
 
+def _check_apart(written, read):
+    """Refuses tensors of `written` (contiguous) that share memory with one another or with one of `read`."""
+    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), True) for t in written if t.numel()]
+    for t in read:
+        if t.numel():
+            last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+            spans.append((t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size(), False))
+    spans.sort()
+    end, end_written = 0, 0   # of what came before
+    for first, behind, is_written in spans:
+        if first < (end if is_written else end_written):
+            raise ValueError("a parameter or momentum shares memory with another tensor of the step")
+        end = max(end, behind)
+        if is_written:
+            end_written = max(end_written, behind)
+
+
 @torch.no_grad()
 def muon_step_(params, grads, momenta, lr, momentum=0.95, weight_decay=0.0, nesterov=True, steps=STEPS,
                coefficients=COEFFICIENTS, eps=EPS):
@@ -37,9 +54,7 @@ def muon_step_(params, grads, momenta, lr, momentum=0.95, weight_decay=0.0, nest
             raise ValueError("muon_step_ takes tensors on one device")
         if not (p.is_contiguous() and m.is_contiguous()):
             raise ValueError("parameters and momenta are updated in place: they must be contiguous")
-    written = [t.data_ptr() for t in params + momenta if t.numel()]
-    if len(set(written)) != len(written):
-        raise ValueError("a parameter or momentum appears twice")
+    _check_apart(params + momenta, grads)
     full = [(p, g.contiguous(), m) for p, g, m in zip(params, grads, momenta) if p.numel()]
     if not full:
         return

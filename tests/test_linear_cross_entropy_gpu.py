@@ -200,6 +200,22 @@ def test_ignored_rows_may_hold_anything(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_ignored_rows_beside_a_bias_that_is_no_number(reduction, dtype):
+    for value in (float("nan"), float("inf")):
+        x, w, b, y = make(200, 64, 70, dtype, ignored=0.4)
+        bad = b.detach().clone()
+        bad[11] = value
+        loss = linear_cross_entropy(x, w, bad, y, reduction=reduction).sum()
+        gx, gw = torch.autograd.grad(loss, (x, w))
+        rows = y == -1
+        assert bool((gx[rows] == 0).all()) and bool(torch.isnan(gx[~rows]).all()) and bool(torch.isnan(gw[11]).all())
+        none = torch.full_like(y, -1)
+        for t in torch.autograd.grad(linear_cross_entropy(x, w, bad, none, reduction=reduction).sum(), (x, w)):
+            assert bool((t == 0).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_no_row_counts(dtype):
     x, w, b, y = make(70, 64, 50, dtype, ignored=2.0)
     for reduction in ("mean", "sum", "none"):

@@ -6,7 +6,7 @@ import torch
 
 from detectron_pytorch_amd import _lib
 from detectron_pytorch_amd.linear_cross_entropy import linear_cross_entropy
-from detectron_pytorch_amd.muon import Muon, as_matrix, muon_step_
+from detectron_pytorch_amd.muon import Muon, _check_apart, as_matrix, muon_step_
 from detectron_pytorch_amd.orthogonalize import orthogonalize, orthogonalize_many
 
 NULL = ctypes.c_void_p(0)
@@ -98,6 +98,17 @@ def test_as_matrix():
     assert as_matrix(w.transpose(0, 1)) is None
 
 
+def test_tensors_of_a_step_share_no_memory():
+    flat, grad = torch.zeros(24), torch.zeros(24)
+    a, b, c = flat[:8], flat[8:16], flat[15:24]
+    _check_apart([b, a], [grad[:8], grad[4:12], torch.zeros(1).expand(8)])   # gradients may share memory among themselves
+    _check_apart([a, torch.zeros(0), flat[3:3]], [flat[8:]])
+    for written, read in (([a, a], []), ([b, c], []), ([c, b], []), ([flat, b], []), ([b], [flat[9:10]]), ([b], [flat]),
+                          ([flat], [b]), ([a, b], [flat.view(2, 12).t()])):
+        with pytest.raises(ValueError):
+            _check_apart(written, read)
+
+
 def test_loss_arguments_at_the_boundary(hip_lib_path):
     h = _lib.lib()
 
@@ -108,7 +119,7 @@ def test_loss_arguments_at_the_boundary(hip_lib_path):
 
     for bad in (dict(x=NULL), dict(w=NULL), dict(y=NULL), dict(loss=NULL), dict(saved=NULL), dict(room=NULL), dict(rows=0),
                 dict(rows=-1), dict(rows=1 << 25), dict(dim=0), dict(classes=0), dict(classes=1 << 25),
-                dict(rows=1 << 24, classes=1 << 24), dict(dtype=3),
+                dict(rows=1 << 24, classes=1 << 24), dict(rows=1 << 19, classes=1 << 18), dict(dtype=3),
                 dict(dtype=-1), dict(xs=7), dict(ws=7), dict(ws=1 << 23), dict(reduction=3), dict(reduction=-1),
                 dict(saved=ctypes.c_void_p(4100)), dict(room=ctypes.c_void_p(4100))):
         assert forward(**bad) == 1 and b"linear_cross_entropy" in h.mi_last_error(), bad
@@ -147,6 +158,23 @@ def test_matrix_arguments_at_the_boundary(hip_lib_path):
     assert call(size=64) == 3
     for c in (floats(40.0, 0.0, 0.0), floats(3.0, 3.0, 3.0), floats(1.0, -900.0, 0.0), floats(float("nan"), 0.0, 0.0)):
         assert call(c=c) == 4 and b"coefficients" in h.mi_last_error()
+    # the range of the iteration, found by sampling its singular values: taken or refused as that says, but for a narrow strip
+    g = torch.Generator().manual_seed(0)
+    seen = set()
+    for _ in range(300):
+        c = (torch.rand(3, generator=g) * 12 - 6).tolist()
+        c = floats(*c)
+        s, x, f = torch.linspace(0, 1, 4001, dtype=torch.float64), 0.0, 0.0
+        for _ in range(3):
+            factor = c[0] + c[1] * s ** 2 + c[2] * s ** 4
+            top = float((s * factor).abs().max())
+            x, f = max(x, top), max(f, float(factor.abs().max()))
+            s = torch.linspace(0, top, 4001, dtype=torch.float64)
+        if abs(max(x / 2.8, f / 60.0) - 1) > 0.01:
+            rc = call(c=c, steps=3, size=64)
+            seen.add(rc)
+            assert rc == (3 if max(x / 2.8, f / 60.0) < 1 else 4), list(c)
+    assert seen == {3, 4}
     assert h.mi_muon_step(1, one, one, NULL, ints(4), ints(6), 0, 0.1, 0.9, 1, 0.0, 5, usual, 1e-7, SOME, 1 << 30, NULL) == 1
     assert h.mi_muon_step(1, one, one, none, ints(4), ints(6), 0, 0.1, 0.9, 1, 0.0, 5, usual, 1e-7, SOME, 1 << 30, NULL) == 1
     assert h.mi_orthogonalize_workspace_bytes(1, ints(0), ints(3)) == 0
