@@ -722,14 +722,18 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void apply(Tiles til
 
 // ---- launching -----------------------------------------------------------------------------------------------------------
 
-template <int SIDE, bool BKM>
-struct TileOf {
-  using type = TileProduct<SIDE, SIDE, 2, 2, SIDE == 64 ? 4 : 2, true, false, false, BKM>;
-};
-template <int SIDE>
-using Rows = typename TileOf<SIDE, false>::type;
-template <int SIDE>
-using Columns = typename TileOf<SIDE, true>::type;
+// `go` with the tile of that side; `lone`: a launch of 128 tiles that each have a compute unit of their own.
+template <bool BKM, class F>
+void with_tile(int side, bool lone, F go) {
+  if (side == 256)
+    go(Tile256<true, false, false, BKM>{});
+  else if (side == 64)
+    go(Tile64<true, false, false, BKM>{});
+  else if (lone)
+    go(Lone128<true, false, false, BKM>{});
+  else
+    go(Tile128<true, false, false, BKM>{});
+}
 
 size_t up(size_t v) { return (v + 255) & ~size_t(255); }
 
@@ -812,7 +816,7 @@ Tiles deal(const Table& t, F per) {
   return d;
 }
 
-template <int THREADS = 256, class K, class... A>
+template <int THREADS, class K, class... A>
 void launch(K kernel, unsigned lds, int blocks, hipStream_t stream, A... args) {
   if (lds >= 65536)  // with a kernel's own variables more than what is given unasked
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -823,6 +827,7 @@ void launch(K kernel, unsigned lds, int blocks, hipStream_t stream, A... args) {
 struct Dealt {
   Tiles tiles;
   int side;
+  bool lone;
   float us;
 };
 template <class F>
@@ -834,7 +839,7 @@ Dealt choose(const Table& t, F tiles_of) {
   const float steps = (float)(stages / c.first[t.count]);
   const int side = choose_tile(a.first[t.count], b.first[t.count], c.first[t.count], steps, true);
   const Tiles& d = side == 256 ? a : side == 128 ? b : c;
-  return {d, side, launch_us(side, true, d.first[t.count], steps)};
+  return {d, side, d.first[t.count] <= compute_units(), launch_us(side, true, d.first[t.count], steps)};
 }
 
 // How many iterations share a pass over the long side (1, 2 or 3): the least estimated time among those whose product of factors C
@@ -870,32 +875,21 @@ void iterate(const Table& t, const Step& s, const GramPlan& plan, const double* 
   const Dealt f = choose(t, [](const Mat& q, int side) { return div_up(q.m, side) * div_up(q.n, side); });
   const auto do_square = [&](int left, int right, int out, float f0, float f1, float fi) {
     const Square q = {left, right, out, f0, f1, fi};
-    if (p.side == 256)
-      launch(square<Rows<256>>, Rows<256>::kLds, p.tiles.first[t.count], stream, p.tiles, q, ws);
-    else if (p.side == 128)
-      launch(square<Rows<128>>, Rows<128>::kLds, p.tiles.first[t.count], stream, p.tiles, q, ws);
-    else
-      launch(square<Rows<64>>, Rows<64>::kLds, p.tiles.first[t.count], stream, p.tiles, q, ws);
+    with_tile<false>(p.side, p.lone, [&](auto tile) {
+      using P = decltype(tile);
+      launch<P::kThreads>(square<P>, P::kLds, p.tiles.first[t.count], stream, p.tiles, q, ws);
+    });
   };
   const int a_pass = iterations_a_pass(s.steps, plan.us, p.us, f.us, growth);
   int flip = 0;
   for (int done = 0; done < s.steps; flip ^= 1) {
     const int now = s.steps - done < a_pass ? s.steps - done : a_pass;
     done += now;
-    if (plan.side == 256)
-      launch(gram<Rows<256>>, Rows<256>::kLds, g.first[t.count], stream, g, ws, flip);
-    else if (plan.side == 128)
-      launch(gram<Rows<128>>, Rows<128>::kLds, g.first[t.count], stream, g, ws, flip);
-    else
-      launch(gram<Rows<64>>, Rows<64>::kLds, g.first[t.count], stream, g, ws, flip);
-    if (joins.first[t.count] > 0) {
-      if (plan.side == 256)
-        launch(join_gram<Rows<256>>, 0, joins.first[t.count], stream, joins, ws);
-      else if (plan.side == 128)
-        launch(join_gram<Rows<128>>, 0, joins.first[t.count], stream, joins, ws);
-      else
-        launch(join_gram<Rows<64>>, 0, joins.first[t.count], stream, joins, ws);
-    }
+    with_tile<false>(plan.side, false, [&](auto tile) {
+      using P = decltype(tile);
+      launch<P::kThreads>(gram<P>, P::kLds, g.first[t.count], stream, g, ws, flip);
+      if (joins.first[t.count] > 0) launch<P::kThreads>(join_gram<P>, 0, joins.first[t.count], stream, joins, ws);
+    });
     int product = kQ, spare = kT;
     for (int i = 0; i < now; ++i) {
       const int c = i == 0 ? kQ : kC;
@@ -912,15 +906,11 @@ void iterate(const Table& t, const Step& s, const GramPlan& plan, const double* 
       }
     }
     const bool last = done == s.steps;
-    if (f.side == 256)
-      launch(last ? apply<Columns<256>, T, true> : apply<Columns<256>, T, false>, Columns<256>::kLds, f.tiles.first[t.count], stream,
-             f.tiles, s, ws, product, flip);
-    else if (f.side == 128)
-      launch(last ? apply<Columns<128>, T, true> : apply<Columns<128>, T, false>, Columns<128>::kLds, f.tiles.first[t.count], stream,
-             f.tiles, s, ws, product, flip);
-    else
-      launch(last ? apply<Columns<64>, T, true> : apply<Columns<64>, T, false>, Columns<64>::kLds, f.tiles.first[t.count], stream,
-             f.tiles, s, ws, product, flip);
+    with_tile<true>(f.side, f.lone, [&](auto tile) {
+      using P = decltype(tile);
+      launch<P::kThreads>(last ? apply<P, T, true> : apply<P, T, false>, P::kLds, f.tiles.first[t.count], stream, f.tiles, s, ws,
+                          product, flip);
+    });
   }
 }
 

@@ -409,6 +409,10 @@ template <bool SPLIT, bool BF16, bool AKM, bool BKM>
 using Tile128 = TileProduct<128, 128, 2, 2, 2, SPLIT, BF16, AKM, BKM>;
 template <bool SPLIT, bool BF16, bool AKM, bool BKM>
 using Tile64 = TileProduct<64, 64, 2, 2, 4, SPLIT, BF16, AKM, BKM>;
+// For launches of 128 tiles that leave compute units empty: a tile there has no neighbour that works while it waits, so it brings
+// two waves per SIMD itself, and a third stage (96 KB) against the latency of memory.
+template <bool SPLIT, bool BF16, bool AKM, bool BKM>
+using Lone128 = TileProduct<128, 128, 2, 4, 3, SPLIT, BF16, AKM, BKM>;
 // waves per SIMD that a kernel with this tile is compiled for
 template <class P>
 constexpr int kWavesPerSimd = P::BM == 256 ? 1 : 2;
