@@ -742,41 +742,43 @@ bool is_narrow(int rows, int cols) {
   return m <= kNarrow && n <= kNarrowLong;
 }
 
-// Tiles and slices of X X': per side the slices that deal the launch's stages evenly to all places, each at least 8 stages long, and
-// the side with the least estimated time; joining costs the slices' way to memory and back.
+// Tiles and slices of X X': per side one slice, or those that deal the launch's stages evenly to all places, each at least 8 stages
+// long; the side and cut with the least estimated time.  Joining costs a launch and the slices' way to memory and back.
 struct GramPlan {
   int side;
+  bool lone;
   float us;
 };
 GramPlan plan_gram(Table& t) {
-  GramPlan best = {64, INFINITY};
+  GramPlan best = {64, false, INFINITY};
   int slices[kMany];
-  for (int side : {256, 128, 64}) {
-    double stages = 0;
-    for (int i = 0; i < t.count; ++i) stages += (double)triangle_tiles(div_up(t.m[i].m, side)) * (up32(t.m[i].n) / 32);
-    double each = stages / tile_places(side);
-    if (each < 8) each = 8;
-    long long tiles = 0;
-    double bytes = 0, longest = 0;
-    int mine[kMany];
-    for (int i = 0; i < t.count; ++i) {
-      const int steps = up32(t.m[i].n) / 32, per = triangle_tiles(div_up(t.m[i].m, side));
-      const double want = steps / each;
-      mine[i] = want < 1.5 ? 1 : want > 32 ? 32 : (int)(want + 0.5);
-      tiles += (long long)per * mine[i];
-      if (mine[i] > 1) bytes += 8.0 * mine[i] * per * side * side;
-      const double len = (double)div_up(steps, mine[i]);
-      longest = len > longest ? len : longest;
+  for (int side : {256, 128, 64})
+    for (bool cut : {false, true}) {
+      double stages = 0;
+      for (int i = 0; i < t.count; ++i) stages += (double)triangle_tiles(div_up(t.m[i].m, side)) * (up32(t.m[i].n) / 32);
+      double each = stages / tile_places(side);
+      if (each < 8) each = 8;
+      long long tiles = 0;
+      double bytes = 0, longest = 0;
+      int mine[kMany];
+      for (int i = 0; i < t.count; ++i) {
+        const int steps = up32(t.m[i].n) / 32, per = triangle_tiles(div_up(t.m[i].m, side));
+        const double want = steps / each;
+        mine[i] = !cut || want < 1.5 ? 1 : want > 32 ? 32 : (int)(want + 0.5);
+        tiles += (long long)per * mine[i];
+        if (mine[i] > 1) bytes += 8.0 * mine[i] * per * side * side;
+        const double len = (double)div_up(steps, mine[i]);
+        longest = len > longest ? len : longest;
+      }
+      const TileTime time = tile_time(side, true);
+      float us = launch_us(side, true, tiles, (float)(stages / tiles));
+      const float least = time.around + (float)longest * time.alone;
+      us = (us > least ? us : least) + (bytes > 0 ? 4.f + (float)(bytes / 8e6) : 0.f);  // joined while the last tiles still run
+      if (us < best.us) {
+        best = {side, tiles <= compute_units(), us};
+        for (int i = 0; i < t.count; ++i) slices[i] = mine[i];
+      }
     }
-    const TileTime time = tile_time(side, true);
-    float us = launch_us(side, true, tiles, (float)(stages / tiles));
-    const float least = time.around + (float)longest * time.alone;
-    us = (us > least ? us : least) + (bytes > 0 ? 4.f + (float)(bytes / 4e6) : 0.f);
-    if (us < best.us) {
-      best = {side, us};
-      for (int i = 0; i < t.count; ++i) slices[i] = mine[i];
-    }
-  }
   for (int i = 0; i < t.count; ++i) t.m[i].slices = slices[i];
   return best;
 }
@@ -844,6 +846,7 @@ Dealt choose(const Table& t, F tiles_of) {
 
 // How many iterations share a pass over the long side (1, 2 or 3): the least estimated time among those whose product of factors C
 // stays within the stored form's range.
+constexpr float kLaunch = 3.f;  // us around the tiles of a launch: start, table and a result that others read
 int iterations_a_pass(int steps, float gram_us, float square_us, float apply_us, const double* growth) {
   int best = 1;
   float least = INFINITY;
@@ -852,7 +855,7 @@ int iterations_a_pass(int steps, float gram_us, float square_us, float apply_us,
     float us = 0.f;
     for (int done = 0; done < steps; done += g) {
       const int now = steps - done < g ? steps - done : g;
-      us += gram_us + apply_us + (4 * now - 3) * square_us;
+      us += gram_us + apply_us + (4 * now - 3) * square_us + (4 * now - 1) * kLaunch;
     }
     if (us < least) least = us, best = g;
   }
@@ -869,8 +872,6 @@ void iterate(const Table& t, const Step& s, const GramPlan& plan, const double* 
   const Tiles squares = deal(t, [](const Mat& q) { return div_up(q.m, 64) * div_up(q.n, 64); });
   normalize<T><<<squares.first[t.count], 256, 0, stream>>>(squares, norm, s, ws);
   const Tiles g = deal(t, [&](const Mat& q) { return triangle_tiles(div_up(q.m, plan.side)) * q.slices; });
-  const int frags = plan.side / 64 * (plan.side / 64);
-  const Tiles joins = deal(t, [&](const Mat& q) { return q.slices > 1 ? triangle_tiles(div_up(q.m, plan.side)) * frags : 0; });
   const Dealt p = choose(t, [](const Mat& q, int side) { return triangle_tiles(div_up(q.m, side)); });
   const Dealt f = choose(t, [](const Mat& q, int side) { return div_up(q.m, side) * div_up(q.n, side); });
   const auto do_square = [&](int left, int right, int out, float f0, float f1, float fi) {
@@ -885,9 +886,10 @@ void iterate(const Table& t, const Step& s, const GramPlan& plan, const double* 
   for (int done = 0; done < s.steps; flip ^= 1) {
     const int now = s.steps - done < a_pass ? s.steps - done : a_pass;
     done += now;
-    with_tile<false>(plan.side, false, [&](auto tile) {
+    with_tile<false>(plan.side, plan.lone, [&](auto tile) {
       using P = decltype(tile);
       launch<P::kThreads>(gram<P>, P::kLds, g.first[t.count], stream, g, ws, flip);
+      const Tiles joins = deal(t, [](const Mat& q) { return q.slices > 1 ? triangle_tiles(div_up(q.m, P::BM)) * P::FM * P::FN : 0; });
       if (joins.first[t.count] > 0) launch<P::kThreads>(join_gram<P>, 0, joins.first[t.count], stream, joins, ws);
     });
     int product = kQ, spare = kT;
