@@ -11,6 +11,7 @@
 // Short side up to 64 (and long side up to 16384): everything happens in the m x m space, in fp64.  A_0 = G G' / |G|^2 (the
 // norm is its trace), Q = product of the C_k with A_k+1 = C_k A_k C_k, result Q G / |G|: three launches, of which the second
 // is one workgroup per matrix with all its matrices in LDS.  A_0 has squared singular values, so float32 would not do.
+// 64 x 256: 8 + 36 + 10 us; the middle one is bound by its chain of 17 products, each 2 us between barriers.
 //
 // Larger: the products run on the matrix cores (tile_product.h) with X, A and C as hi + lo fp16 times a power of two (22
 // bits).  Their magnitudes are known -- |X| is bounded by the polynomial's largest value, which the host checks -- so no pass
@@ -20,6 +21,9 @@
 // long side: A_k+1 = C_k A_k C_k and Q = C_k+1 C_k are m x m products.  A pass in between renews A from X, which keeps the
 // error at that of separate iterations (2.1e-6 to 5.2e-6 of the norm against 2.1e-6 to 4.9e-6 on Gaussian and strongly
 // low-rank 256 x 1024; with all five in one pass 1e-4).
+//
+// Bound by the matrix cores on long matrices (1024 x 12544: Gram 44 + 11 us, C X 90 us, 292 TFLOP/s in float32 terms) and by the
+// latency of the m x m products, which are too small for the chip (1024: 16 us, 2048: 47 to 54 us).
 //
 // Accumulators are float32; the norm is summed in fp64, so no gradient is too small or too large for it.
 // All matrices of a call go through each stage in one launch: a workgroup finds its matrix in the call's table.
@@ -438,7 +442,7 @@ __global__ __launch_bounds__(256) void narrow_apply(Tiles tiles, Step s, char* w
 
 // ---- larger matrices: momentum, norm, X_0 --------------------------------------------------------------------------------
 
-// M <- mu M + G, and the squares of U: one fp64 sum per workgroup.
+// M <- mu M + G, and the squares of U: one fp64 sum per workgroup.  Bound by memory: 20.9 M float32 elements in 44 us (5.7 TB/s).
 template <int T>
 __global__ __launch_bounds__(256) void momentum_and_norm(Table t, Tiles tiles, Step s, char* ws) {
   leave_table(t, ws);
@@ -471,7 +475,7 @@ __global__ __launch_bounds__(256) void momentum_and_norm(Table t, Tiles tiles, S
   if (threadIdx.x == 0) reinterpret_cast<double*>(ws + q.norm_at)[block] = part[0] + part[1] + part[2] + part[3];
 }
 
-// X_0, 64 x 64 of the given matrix per workgroup, turned on the way if it is tall.
+// X_0, 64 x 64 of the given matrix per workgroup, turned on the way if it is tall.  Bound by memory: 20.9 M elements in 48 us (5.2 TB/s).
 template <int T>
 __global__ __launch_bounds__(256) void normalize(Tiles tiles, Tiles norm, Step s, char* ws) {
   const Table& t = table_of(ws);
@@ -631,7 +635,8 @@ __global__ __launch_bounds__(P::kThreads) void join_gram(Tiles tiles, char* ws) 
   }
 }
 
-// out = f0 L R + f1 L + fi I of the m x m matrices, all symmetric and polynomials of one another: one tile of the upper triangle.
+// out = f0 L R + f1 L + fi I of the m x m matrices, all symmetric and polynomials of one another: one tile of the upper triangle, which
+// halves the work.  Its epilogue (L read, both sides written) is 8 of the 54 us at 2048.
 struct Square {
   int left, right, out;
   float f0, f1, fi;
@@ -664,7 +669,8 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void square(Tiles ti
                    });
 }
 
-// X <- C X (or Q X, several iterations at once), or in the last pass the result itself.
+// X <- C X (or Q X, several iterations at once), or in the last pass the result itself, with the optimiser's step: the update never
+// lies in memory (21 matrices, 20.9 M weights: 172 us, a pass that only writes X 101).
 template <class P, int T, bool LAST>
 __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void apply(Tiles tiles, Step s, char* ws, int factor, int flip) {
   extern __shared__ char smem[];

@@ -9,8 +9,8 @@ the log of the sum of exponentials only (reference of the plain form: lib/modeli
     loss, pred = linear_cross_entropy(x, weight, bias, labels, with_pred=True)
 
 x [rows, dim], weight [classes, dim], bias [classes] or None: all float32, all float16 or all bfloat16, on one GPU; labels int32
-or int64 [rows].  Sums, softmax statistics and the loss are float32; float32 products carry 22 bits of each factor,
-relative to the largest magnitude of its tensor.
+or int64 [rows].  Sums, softmax statistics and the loss are float32.  float32 products carry 22 bits of each factor down to 2^-18 of
+the largest finite magnitude of its tensor, and one bit less per halving below that (an infinite factor makes its logits NaN).
 """
 import torch
 from torch.autograd import Function
