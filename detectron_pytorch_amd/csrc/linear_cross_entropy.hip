@@ -952,6 +952,8 @@ int mi_linear_cross_entropy_backward(const float* grad_loss, const void* weight,
                                 mi_linear_cross_entropy_workspace_bytes(rows, dim, classes, dtype, MI_PASS_BACKWARD), &p))
     return rc;
   MI_REQUIRE(grad_loss != nullptr, "linear_cross_entropy: null pointer");
+  MI_REQUIRE((reinterpret_cast<uintptr_t>(grad_x) | reinterpret_cast<uintptr_t>(grad_weight)) % 16 == 0,
+             "linear_cross_entropy: gradients start on 16 bytes");
   begin_call();
   const Call c = {nullptr, weight, bias, nullptr, dim, weight_stride, 0, 0, reduction,
                   static_cast<char*>(saved), static_cast<char*>(workspace), as_stream(stream)};

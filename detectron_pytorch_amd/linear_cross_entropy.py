@@ -19,6 +19,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 
 TYPES = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16}
+MOST_STRIDE = 1 << 22   # rows further apart are brought together first
 REDUCTIONS = {"none": _lib.REDUCTION_NONE, "mean": _lib.REDUCTION_MEAN, "sum": _lib.REDUCTION_SUM}
 
 
@@ -46,9 +47,9 @@ def _check(x, weight, bias, labels, reduction):
 
 
 def _rows(t):
-    """`t` with contiguous rows (any distance between them, as long as they do not overlap) and that distance."""
+    """`t` with contiguous rows that do not overlap, and the distance between them."""
     rows, cols = t.shape
-    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and not cols <= t.stride(0) <= MOST_STRIDE):
         t = t.contiguous()
     return t, (t.stride(0) if rows > 1 else cols)
 

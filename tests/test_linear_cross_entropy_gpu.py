@@ -182,6 +182,14 @@ def test_strides_and_alignment(dtype):
     check(x[:1].detach().expand(100, 64).requires_grad_(True), w, b, y)
 
 
+def test_rows_far_apart():
+    x, w, b, y = make(3, 24, 3, torch.float16, ignored=0.0)
+    far = [torch.zeros(3, (1 << 22) + 8, dtype=torch.float16, device=DEV)[:, :24] for _ in range(2)]
+    far[0].copy_(x.detach())
+    far[1].copy_(w.detach())
+    check(far[0].requires_grad_(True), far[1].requires_grad_(True), b, y)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_ignored_rows_may_hold_anything(dtype):
     x, w, b, y = make(90, 64, 70, dtype, ignored=0.4)

@@ -129,6 +129,9 @@ def test_loss_arguments_at_the_boundary(hip_lib_path):
                                               NULL) == 1
     assert h.mi_linear_cross_entropy_backward(SOME, SOME, 8, NULL, 4, 8, 5, 0, 1, NULL, NULL, NULL, SOME, 1 << 30, SOME, 8,
                                               NULL) == 3
+    for gx, gw in ((ctypes.c_void_p(4104), NULL), (NULL, ctypes.c_void_p(4098))):
+        assert h.mi_linear_cross_entropy_backward(SOME, SOME, 8, NULL, 4, 8, 5, 0, 1, gx, gw, NULL, SOME, 1 << 30, SOME, 1 << 30,
+                                                  NULL) == 1
     assert h.mi_linear_cross_entropy_saved_bytes(0, 8, 5, 0, SOME, 8) == 0
     # 16-bit weights that can be multiplied where they lie are not kept a second time
     in_place = h.mi_linear_cross_entropy_saved_bytes(4, 64, 5000, 2, ctypes.c_void_p(4096), 64)
