@@ -534,34 +534,35 @@ __global__ __launch_bounds__(256) void normalize(Tiles tiles, Tiles norm, Step s
 
 // ---- larger matrices: the products ---------------------------------------------------------------------------------------
 
-// A symmetric result's tile of the upper triangle, on both sides (the padding of a row lies in its upper half).  `finish(row, col,
+// A symmetric result's tile of the upper triangle, on both sides (the padding of a row lies in its upper half; both sides are
+// the same to the last bit off the diagonal's tiles).  `finish(row, col,
 // v, old)` is what is still done to four columns of a row, `before(row, col)` what it wants to know of the place.
 template <class P, class B, class F>
 __device__ __forceinline__ void put_symmetric(f32x16 (&acc)[P::FM][P::FN], lds_bytes lds, uint16_t* out, int m, int ti, int tj,
                                               B before, F finish) {
   const int ld = up32(m);
-  const auto asked = [&](int r, int c, bool turned) {
+  const auto asked = [&](int r, int c) {
     const int row = ti * P::BM + r, col = tj * P::BN + c;
-    if (turned ? col >= m : row >= m || col >= ld) return f32x4{0.f, 0.f, 0.f, 0.f};
-    return turned ? before(col, row) : before(row, col);
+    return row < m && col < ld ? before(row, col) : f32x4{0.f, 0.f, 0.f, 0.f};
   };
   const auto by_row = [&](int r, int c, f32x4 v, f32x4 old) {
     const int row = ti * P::BM + r, col = tj * P::BN + c;
-    if (row >= m || col >= ld) return;
+    if (row >= m || col >= ld) return v;
     v = finish(row, col, v, old);
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (col + k >= m) v[k] = 0.f;
     put_split4(out + split_at(row, col, ld), v);
+    return v;
   };
   if (ti == tj) {
     P::template hand_out<false>(acc, lds, asked, by_row, typename P::Nothing{});
     return;
   }
   // rows of the transposed tile: ti is not the last tile, so its 4 rows are all inside
-  P::template hand_out<true>(acc, lds, asked, by_row, [&](int r, int c, f32x4 v, f32x4 old) {
+  P::template hand_out<true>(acc, lds, asked, by_row, [&](int r, int c, f32x4 v) {
     const int row = ti * P::BM + r, col = tj * P::BN + c;
-    if (col < m) put_split4(out + split_at(col, row, ld), finish(col, row, v, old));
+    if (col < m) put_split4(out + split_at(col, row, ld), v);
   });
 }
 
@@ -656,7 +657,6 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void square(Tiles ti
   f32x16 acc[P::FM][P::FN];
   P::run(acc, {l, (long long)ld * 2, q.m, ld}, {at(s.right), (long long)ld * 2, q.m, ld}, ti * P::BM, tj * P::BN, 0, ld / 32,
          (lds_bytes)smem);
-  // L is symmetric, so the transposed side finds its element of it at its own place
   put_symmetric<P>(acc, (lds_bytes)smem, at(s.out), q.m, ti, tj,
                    [&](int row, int col) {
                      return s.f1 != 0.f ? get_split4(l + split_at(row, col, ld)) : f32x4{0.f, 0.f, 0.f, 0.f};
@@ -697,7 +697,7 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void apply(Tiles til
   if (!q.tall && aligned16(q.out) && q.n % 4 == 0) {
     P::template hand_out<false>(
         acc, (lds_bytes)smem,
-        [&](int r, int c, bool) {
+        [&](int r, int c) {
           const int row = tm * P::BM + r, col = tn * P::BN + c;
           if (!s.update || row >= q.m || col >= q.n) return f32x4{0.f, 0.f, 0.f, 0.f};
           return load_four<T>(q.out, (long long)row * q.n + col, 4, true);

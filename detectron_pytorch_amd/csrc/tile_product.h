@@ -296,10 +296,10 @@ struct TileProduct {
 
   // Hands the wave's part of the tile out in the order of memory: four columns of a row a lane, lanes along the row.  As it lies in
   // the registers, a store would touch 32 rows with 16 or 32 bytes each; through LDS (a strip of 32 rows at a time, a
-  // region per wave) it writes whole rows of the part.  `by_row(row, col, v, old)` gets them; with COLUMNS `by_column(row, col, v,
-  // old)` gets four rows of a column a lane, lanes along the column, for a result that is also stored transposed.  `old` is
-  // what `before` returned for the place: a strip's are all asked for before the first of its stores, behind which the
-  // compiler would not move them.
+  // region per wave) it writes whole rows of the part.  `by_row(row, col, v, old)` gets them; `old` is what `before` returned for the
+  // place: a strip's are all asked for before the first of its stores, behind which the compiler would not move them.  With COLUMNS
+  // `by_row` returns what it made of v, and `by_column(row, col, v)` gets four rows of a column of that a lane, lanes along the
+  // column, for a result that is also stored transposed.
   static constexpr int kPitch = FN * 32 + 4;
   static_assert(kWaves * 32 * kPitch * 4 <= kLds, "the strips fit where the stages were");
   template <bool COLUMNS, class B, class R, class C>
@@ -319,29 +319,30 @@ struct TileProduct {
           *reinterpret_cast<quad_at>(mine + ((lane & 31) * kPitch + j * 32 + g * 8 + (lane >> 5) * 4) * 4) = quad(acc[i][j], g);
       constexpr int kQuads = FN * 8, kRows = 64 / kQuads;
       const int r = lane / kQuads, c = lane % kQuads * 4, rc = (lane & 7) * 4, cc = lane >> 3;
-      f32x4 old[32 / kRows], old_c[COLUMNS ? FN * 4 : 1];
+      f32x4 old[32 / kRows];
 #pragma unroll
-      for (int n = 0; n < 32 / kRows; ++n) old[n] = before(row0 + i * 32 + n * kRows + r, col0 + c, false);
-      if constexpr (COLUMNS) {
+      for (int n = 0; n < 32 / kRows; ++n) old[n] = before(row0 + i * 32 + n * kRows + r, col0 + c);
 #pragma unroll
-        for (int n = 0; n < FN * 4; ++n) old_c[n] = before(row0 + i * 32 + rc, col0 + n * 8 + cc, true);
+      for (int n = 0; n < 32 / kRows; ++n) {
+        const quad_at p = reinterpret_cast<quad_at>(mine + ((n * kRows + r) * kPitch + c) * 4);
+        if constexpr (COLUMNS)
+          *p = by_row(row0 + i * 32 + n * kRows + r, col0 + c, *p, old[n]);
+        else
+          by_row(row0 + i * 32 + n * kRows + r, col0 + c, *p, old[n]);
       }
-#pragma unroll
-      for (int n = 0; n < 32 / kRows; ++n)
-        by_row(row0 + i * 32 + n * kRows + r, col0 + c, *reinterpret_cast<quad_at>(mine + ((n * kRows + r) * kPitch + c) * 4), old[n]);
       if constexpr (COLUMNS) {
 #pragma unroll
         for (int n = 0; n < FN * 4; ++n) {
           const float_at p = reinterpret_cast<float_at>(mine + (rc * kPitch + n * 8 + cc) * 4);
-          by_column(row0 + i * 32 + rc, col0 + n * 8 + cc, f32x4{p[0], p[kPitch], p[2 * kPitch], p[3 * kPitch]}, old_c[n]);
+          by_column(row0 + i * 32 + rc, col0 + n * 8 + cc, f32x4{p[0], p[kPitch], p[2 * kPitch], p[3 * kPitch]});
         }
       }
     }
   }
 
   struct Nothing {  // for results that are only written
-    __device__ __forceinline__ f32x4 operator()(int, int, bool) const { return f32x4{0.f, 0.f, 0.f, 0.f}; }
-    __device__ __forceinline__ void operator()(int, int, f32x4, f32x4) const {}
+    __device__ __forceinline__ f32x4 operator()(int, int) const { return f32x4{0.f, 0.f, 0.f, 0.f}; }
+    __device__ __forceinline__ void operator()(int, int, f32x4) const {}
   };
   template <class R>
   static __device__ __forceinline__ void hand_out(const f32x16 (&acc)[FM][FN], lds_bytes lds, R by_row) {
