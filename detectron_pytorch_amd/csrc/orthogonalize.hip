@@ -22,8 +22,8 @@
 // error at that of separate iterations (2.1e-6 to 5.2e-6 of the norm against 2.1e-6 to 4.9e-6 on Gaussian and strongly
 // low-rank 256 x 1024; with all five in one pass 1e-4).
 //
-// Bound by the matrix cores on long matrices (1024 x 12544: Gram 44 + 11 us, C X 90 us, 292 TFLOP/s in float32 terms) and by the
-// latency of the m x m products, which are too small for the chip (1024: 16 us, 2048: 47 to 54 us).
+// Bound by the matrix cores on long matrices (1024 x 12544: Gram 45 + 9 us, C X 90 us, 292 TFLOP/s in float32 terms) and by the
+// latency of the m x m products, which are too small for the chip (1024: 16 us, 2048: 46 to 51 us).
 //
 // Accumulators are float32; the norm is summed in fp64, so no gradient is too small or too large for it.
 // All matrices of a call go through each stage in one launch: a workgroup finds its matrix in the call's table.
@@ -563,7 +563,8 @@ __device__ __forceinline__ void put_symmetric(f32x16 (&acc)[P::FM][P::FN], lds_b
 
 // A = X X': one tile of the upper triangle and one slice of the sum over n.  With one slice the tile is written as it is; slices leave
 // their float32 sums in the workspace, as they lie in the registers, for join_gram.  (Having the slice that comes last join
-// them saves that launch, but each workgroup then writes its L2 back first: 241 us instead of 70 + 8 at 1024 x 12544.)
+// them saves that launch, but each workgroup then writes its L2 back first: 241 us instead of 70 + 8 at 1024 x 12544, both before
+// the tiles' order of today.)
 template <class P>
 __device__ __forceinline__ f32x4* slice_sums(const Mat& q, char* ws, int per, int tile, int slice, int i, int j, int g) {
   return reinterpret_cast<f32x4*>(ws + q.parts_at) +
@@ -641,7 +642,7 @@ __global__ __launch_bounds__(P::kThreads) void join_gram(Tiles tiles, char* ws) 
 }
 
 // out = f0 L R + f1 L + fi I of the m x m matrices, all symmetric and polynomials of one another: one tile of the upper triangle, which
-// halves the work.  Its epilogue (L read, both sides written) is 8 of the 54 us at 2048.
+// halves the work.  Its epilogue (L read, both sides written) is 6 of the 50 us at 2048.
 struct Square {
   int left, right, out;
   float f0, f1, fi;
