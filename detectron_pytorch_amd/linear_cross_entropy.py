@@ -127,4 +127,6 @@ def linear_cross_entropy(x, weight, bias, labels, ignore_index=-1, reduction="me
     its row's loss NaN.  `with_pred`: also the class of the largest logit per row (int64, lowest index of equal ones, -1
     for ignored rows).  The backward is captured into a graph or run eagerly like the forward: no host synchronisation."""
     _check(x, weight, bias, labels, reduction)
+    if not -2 ** 63 <= ignore_index < 2 ** 63:
+        raise ValueError("ignore_index must be a label's value, got %r" % (ignore_index,))
     return _LinearCrossEntropy.apply(x, weight, bias, labels, int(ignore_index), REDUCTIONS[reduction], bool(with_pred))

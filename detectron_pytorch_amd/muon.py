@@ -8,12 +8,10 @@ Per matrix:  M <- mu M + G,  U = G + mu M (nesterov) or M,
 A convolution's weight [out, in, kh, kw] is the matrix [out, in kh kw].  What is no matrix (biases) takes the momentum SGD step
 of torch.optim.SGD, with its own learning rate.
 """
-import ctypes
-
 import torch
 
 from . import _lib
-from .orthogonalize import COEFFICIENTS, EPS, STEPS, check_matrices, host_arrays, pointers, workspace_for
+from .orthogonalize import COEFFICIENTS, EPS, STEPS, check_matrices, host_arrays, pointers, polynomial, workspace_for
 
 
 def _check_apart(written, read):
@@ -64,7 +62,7 @@ def muon_step_(params, grads, momenta, lr, momentum=0.95, weight_decay=0.0, nest
         workspace = workspace_for(count, rows, cols, dev)
         rc = _lib.lib().mi_muon_step(count, pointers(ps), pointers(gs), pointers(ms), rows, cols, dtype, float(lr),
                                      float(momentum), int(nesterov), float(weight_decay), int(steps),
-                                     (ctypes.c_float * 3)(*coefficients), float(eps), workspace.data_ptr(), workspace.numel(),
+                                     polynomial(coefficients), float(eps), workspace.data_ptr(), workspace.numel(),
                                      _lib.current_stream_handle(dev))
     _lib.check(rc, "mi_muon_step")
 

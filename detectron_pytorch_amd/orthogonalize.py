@@ -40,6 +40,14 @@ def pointers(tensors):
     return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
 
 
+def polynomial(coefficients):
+    """(a, b, c) as the C side takes them."""
+    coefficients = [float(c) for c in coefficients]
+    if len(coefficients) != 3:
+        raise ValueError("coefficients are (a, b, c), got %d numbers" % len(coefficients))
+    return (ctypes.c_float * 3)(*coefficients)
+
+
 def workspace_for(count, rows, cols, device):
     n = _lib.lib().mi_orthogonalize_workspace_bytes(count, rows, cols)
     if n == 0:
@@ -63,7 +71,7 @@ def orthogonalize_many(mats, steps=STEPS, coefficients=COEFFICIENTS, eps=EPS):
     with torch.cuda.device(dev):
         workspace = workspace_for(count, rows, cols, dev)
         rc = _lib.lib().mi_orthogonalize(count, pointers(ins), pointers(results), rows, cols, dtype, int(steps),
-                                         (ctypes.c_float * 3)(*coefficients), float(eps), workspace.data_ptr(), workspace.numel(),
+                                         polynomial(coefficients), float(eps), workspace.data_ptr(), workspace.numel(),
                                          _lib.current_stream_handle(dev))
     _lib.check(rc, "mi_orthogonalize")
     return outs

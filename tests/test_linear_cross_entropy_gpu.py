@@ -182,6 +182,13 @@ def test_strides_and_alignment(dtype):
     check(x[:1].detach().expand(100, 64).requires_grad_(True), w, b, y)
 
 
+def test_ignored_label_outside_of_int64_is_refused():
+    x, w, b, y = make(4, 8, 5, torch.float32)
+    for bad in (2 ** 63, 2 ** 64 - 1, -2 ** 63 - 1):
+        with pytest.raises(ValueError):
+            linear_cross_entropy(x, w, b, y, ignore_index=bad)
+
+
 def test_rows_far_apart():
     x, w, b, y = make(3, 24, 3, torch.float16, ignored=0.0)
     far = [torch.zeros(3, (1 << 22) + 8, dtype=torch.float16, device=DEV)[:, :24] for _ in range(2)]

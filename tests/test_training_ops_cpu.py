@@ -7,7 +7,7 @@ import torch
 from detectron_pytorch_amd import _lib
 from detectron_pytorch_amd.linear_cross_entropy import linear_cross_entropy
 from detectron_pytorch_amd.muon import Muon, _check_apart, as_matrix, muon_step_
-from detectron_pytorch_amd.orthogonalize import orthogonalize, orthogonalize_many
+from detectron_pytorch_amd.orthogonalize import orthogonalize, orthogonalize_many, polynomial
 
 NULL = ctypes.c_void_p(0)
 SOME = ctypes.c_void_p(4096)   # an address that a refused call never touches
@@ -32,6 +32,13 @@ def test_cpu_tensors_are_refused(hip_lib_path):
     assert muon_step_([], [], [], lr=0.1) is None
     with pytest.raises(ValueError):
         muon_step_([torch.zeros(2, 3)], [], [], lr=0.1)
+
+
+def test_coefficients_are_three():
+    assert list(polynomial([1, 2.5, -3])) == [1.0, 2.5, -3.0]
+    for bad in ((), (1.0, 2.0), (1.0, 2.0, 3.0, 4.0)):
+        with pytest.raises(ValueError):
+            polynomial(bad)
 
 
 def test_optimizer_arguments():
