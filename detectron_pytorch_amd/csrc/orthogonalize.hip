@@ -11,7 +11,8 @@
 // Short side up to 64 (and long side up to 16384): everything happens in the m x m space, in fp64.  A_0 = G G' / |G|^2 (the
 // norm is its trace), Q = product of the C_k with A_k+1 = C_k A_k C_k, result Q G / |G|: three launches, of which the second
 // is one workgroup per matrix with all its matrices in LDS.  A_0 has squared singular values, so float32 would not do.
-// 64 x 256: 8 + 36 + 10 us; the middle one is bound by its chain of 17 products, each 2 us between barriers.
+// 64 x 256: 8 + 36 + 10 us; the middle one is bound by the fp64 matrix instructions of one compute unit (17 products, 10 tiles each
+// on 4 SIMDs).
 //
 // Larger: the products run on the matrix cores (tile_product.h) with X, A and C as hi + lo fp16 times a power of two (22
 // bits).  Their magnitudes are known -- |X| is bounded by the polynomial's largest value, which the host checks -- so no pass
