@@ -35,6 +35,7 @@ constexpr float kQScale = 16384.f;    // q is stored times 2^14: fp16 keeps prob
 constexpr int kIgnored = -1, kOutside = -2;
 constexpr int kIsNaN = 1 << 30;       // mark of a predicted class whose logit is NaN
 constexpr int kNoClass = kIsNaN - 1;
+constexpr int kElsewhere = 1 << 28;   // a row's largest logit is not among this lane's columns
 constexpr float kLargest = 3.402823466e38f;
 constexpr size_t kPieceBytes = size_t(1) << 30;  // q of one piece of the vocabulary
 
@@ -299,28 +300,27 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_forward(
     m = fmaxf(m, __shfl_xor(m, 32));
     const float from = m == -INFINITY ? 0.f : m;  // a strip of classes that are all masked sums to zero
     float s = 0.f;
+    int at = kElsewhere;  // from the last column down, so that the lowest one of the largest logit stays
 #pragma unroll
-    for (int j = 0; j < P::FN; ++j)
+    for (int j = P::FN - 1; j >= 0; --j)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s += __expf(acc[i][j][e] - from);
+      for (int e = 15; e >= 0; --e) {
+        if constexpr (PRED) at = acc[i][j][e] == m ? j * 32 + column(e) : at;
+        s += __expf(acc[i][j][e] - from);
+      }
     s += __shfl_xor(s, 32);
     const bool writes = row < rows && (threadIdx.x & 32) == 0;
     if (writes) part[(long long)strip * rows_p + row] = make_float2(m, s);
     if constexpr (PRED) {
-      int at = kNoClass;
-#pragma unroll
-      for (int j = P::FN - 1; j >= 0; --j)
-#pragma unroll
-        for (int e = 15; e >= 0; --e) at = acc[i][j][e] == m ? col0 + j * 32 + column(e) : at;
+      at += col0;
       if (__any(s != s)) {  // the first NaN, where the row has one
-        int first = kNoClass;
+        int first = kNoClass, inside = classes - col0;
+        asm volatile("" : "+v"(inside));  // compared here only: kept for all rows, 64 results would fill the scalar registers
 #pragma unroll
         for (int j = P::FN - 1; j >= 0; --j)
 #pragma unroll
-          for (int e = 15; e >= 0; --e) {
-            const int col = col0 + j * 32 + column(e);
-            first = col < classes && acc[i][j][e] != acc[i][j][e] ? col : first;
-          }
+          for (int e = 15; e >= 0; --e)
+            first = j * 32 + column(e) < inside && acc[i][j][e] != acc[i][j][e] ? col0 + j * 32 + column(e) : first;
         const int other = min(first, __shfl_xor(first, 32));
         if (other != kNoClass) at = other | kIsNaN;
       }
@@ -330,12 +330,13 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_forward(
   }
 }
 
-// Joins the strips of 16 rows, 16 threads a row; the workgroup that comes last sums the rows' losses in their order.
+// Joins the strips of 16 rows, 16 threads a row with eight strips on their way at a time; the workgroup that comes last sums the rows'
+// losses in their order.  Bound by latency: 171 strips of 2000 rows with classes 9.1 us (two to four at a time 12.2).
 __global__ __launch_bounds__(256) void join_strips(const float2* part, const int* best, int strips, const int* lab, int rows,
                                                    int rows_p, const float* target, float* lse, float* losses, int64_t* pred,
                                                    int mean, float* loss, Sum* sums, Scalars* sc) {
-  __shared__ float2 s[16][17];
-  __shared__ Best sb[16][17];
+  __shared__ float2 s[4][16];
+  __shared__ Best sb[4][16];
   __shared__ Sum total[16];
   __shared__ int last;
   const int r = threadIdx.x & 15, p0 = threadIdx.x >> 4, row = blockIdx.x * 16 + r;
@@ -346,24 +347,40 @@ __global__ __launch_bounds__(256) void join_strips(const float2* part, const int
   float2 a = make_float2(-INFINITY, 0.f);
   Best b = {-INFINITY, kNoClass};
   if (row < rows) {
-#pragma unroll 4
-    for (int p = p0; p < strips; p += 16) {
-      const float2 v = part[(long long)p * rows_p + row];
-      merge(a, v);
-      if (best != nullptr) {
-        const int at = best[(long long)p * rows_p + row];
-        const Best o = {at & kIsNaN ? NAN : v.x, at & ~kIsNaN};
+    constexpr int kTogether = 8;
+    for (int from = p0; from < strips; from += 16 * kTogether) {
+      float2 v[kTogether];
+      int at[kTogether];
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) {
+        const int p = from + 16 * u;
+        v[u] = p < strips ? part[(long long)p * rows_p + row] : make_float2(-INFINITY, 0.f);
+        at[u] = best != nullptr && p < strips ? best[(long long)p * rows_p + row] : kNoClass;
+      }
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) {
+        if (from + 16 * u >= strips) continue;
+        merge(a, v[u]);
+        const Best o = {at[u] & kIsNaN ? NAN : v[u].x, at[u] & ~kIsNaN};
         if (beats(o, b)) b = o;
       }
     }
   }
-  s[p0][r] = a;
-  sb[p0][r] = b;
+  // a wave's four threads of a row, then the four waves
+#pragma unroll
+  for (int d = 16; d < 64; d <<= 1) {
+    const float2 v = make_float2(__shfl_xor(a.x, d), __shfl_xor(a.y, d));
+    const Best o = {__shfl_xor(b.v, d), __shfl_xor(b.at, d)};
+    merge(a, v);
+    if (beats(o, b)) b = o;
+  }
+  if ((threadIdx.x & 48) == 0) s[threadIdx.x >> 6][r] = a, sb[threadIdx.x >> 6][r] = b;
   __syncthreads();
   if (p0 == 0) {
-    for (int p = 1; p < 16; ++p) {
+#pragma unroll
+    for (int p = 1; p < 4; ++p) {
       merge(a, s[p][r]);
-      if (best != nullptr && beats(sb[p][r], b)) b = sb[p][r];
+      if (beats(sb[p][r], b)) b = sb[p][r];
     }
     float mine = 0.f;
     int y = kIgnored;
