@@ -72,7 +72,7 @@ struct Plan {
   int rows_p, dim_p;        // padded to kPad
   bool split, copy_w;       // float32; weights laid out anew (float32, or 16-bit ones that the product cannot take in place)
   long long ld;             // words between rows of a laid-out operand
-  size_t x_at, w_at, lab_at, lse_at, scalars_at, saved_bytes;
+  size_t x_at, lab_at, lse_at, scalars_at, w_at, saved_bytes;
 };
 
 size_t up(size_t v) { return (v + 255) & ~size_t(255); }
@@ -87,10 +87,11 @@ Plan make_plan(int rows, int dim, int classes, int dtype, bool w_in_place) {
   p.ld = (long long)p.dim_p * (p.split ? 2 : 1);
   size_t at = 0;
   p.x_at = at, at = up(at + (size_t)p.rows_p * p.ld * 2);
-  p.w_at = at, at = up(at + (p.copy_w ? (size_t)classes * p.ld * 2 : 0));
   p.lab_at = at, at = up(at + (size_t)p.rows_p * 4);
   p.lse_at = at, at = up(at + (size_t)p.rows_p * 4);
   p.scalars_at = at, at = up(at + 64);
+  // the weights come last: a backward whose weight lies on another alignment than the forward's finds the rest where it was left
+  p.w_at = at, at = up(at + (p.copy_w ? (size_t)classes * p.ld * 2 : 0));
   p.saved_bytes = at;
   return p;
 }

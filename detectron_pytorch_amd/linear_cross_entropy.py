@@ -54,6 +54,19 @@ def _rows(t):
     return t, (t.stride(0) if rows > 1 else cols)
 
 
+def _unpacked(ctx, weight, bias, saved):
+    """The saved tensors as the backward reads them, and the distance of the weight's rows.  Hooks on saved tensors
+    (torch.autograd.graph.saved_tensors_hooks, save_on_cpu) may give back others: of other strides, at another address."""
+    weight, stride = _rows(weight)
+    if (weight.data_ptr(), stride) != ctx.weight_at:
+        needed = _lib.lib().mi_linear_cross_entropy_saved_bytes(*ctx.shape, weight.data_ptr(), stride)
+        if needed > saved.numel():   # the forward read it where it lay and kept no copy, which this place does not allow
+            weight, stride = weight.clone(memory_format=torch.contiguous_format), weight.size(1)
+    if saved.data_ptr() % 256 or not saved.is_contiguous():
+        saved = saved.clone(memory_format=torch.contiguous_format)
+    return weight, stride, None if bias is None else bias.contiguous(), saved
+
+
 class _LinearCrossEntropy(Function):
     """`.apply(x, weight, bias_or_None, labels, ignore_index, reduction, with_pred)`; pred is not differentiable."""
 
@@ -64,7 +77,7 @@ class _LinearCrossEntropy(Function):
         rows, dim = x.shape
         classes, dtype, dev = weight.size(0), TYPES[x.dtype], x.device
         lib = _lib.lib()
-        ctx.shape, ctx.reduction, ctx.w_stride = (rows, dim, classes, dtype), reduction, w_stride
+        ctx.shape, ctx.reduction = (rows, dim, classes, dtype), reduction
         if rows == 0:   # nothing to launch
             ctx.save_for_backward(weight, bias, None)
             loss = torch.zeros((0,) if reduction == _lib.REDUCTION_NONE else (), dtype=torch.float32, device=dev)
@@ -85,6 +98,7 @@ class _LinearCrossEntropy(Function):
                 loss.data_ptr(), pred.data_ptr() if with_pred else None, saved.data_ptr(), saved.numel(), workspace.data_ptr(),
                 ws_bytes, _lib.current_stream_handle(dev))
         _lib.check(rc, "mi_linear_cross_entropy_forward")
+        ctx.weight_at = weight.data_ptr(), w_stride
         ctx.save_for_backward(weight, bias, saved)
         if with_pred:
             ctx.mark_non_differentiable(pred)
@@ -104,6 +118,7 @@ class _LinearCrossEntropy(Function):
                     torch.zeros((classes,), dtype=weight.dtype, device=dev) if want_b else None, None, None, None, None)
         lib = _lib.lib()
         with torch.cuda.device(dev):
+            weight, w_stride, bias, saved = _unpacked(ctx, weight, bias, saved)
             grad_loss = grad_loss.contiguous().float()
             grad_x = torch.empty((rows, dim), dtype=weight.dtype, device=dev) if want_x else None
             grad_w = torch.empty((classes, dim), dtype=weight.dtype, device=dev) if want_w else None
@@ -111,7 +126,7 @@ class _LinearCrossEntropy(Function):
             ws_bytes = lib.mi_linear_cross_entropy_workspace_bytes(rows, dim, classes, dtype, _lib.PASS_BACKWARD)
             workspace = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
             rc = lib.mi_linear_cross_entropy_backward(
-                grad_loss.data_ptr(), weight.data_ptr(), ctx.w_stride, None if bias is None else bias.data_ptr(), rows, dim,
+                grad_loss.data_ptr(), weight.data_ptr(), w_stride, None if bias is None else bias.data_ptr(), rows, dim,
                 classes, dtype, ctx.reduction, grad_x.data_ptr() if want_x else None, grad_w.data_ptr() if want_w else None,
                 grad_b.data_ptr() if want_b else None, saved.data_ptr(), saved.numel(), workspace.data_ptr(), ws_bytes,
                 _lib.current_stream_handle(dev))

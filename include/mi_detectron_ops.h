@@ -500,8 +500,9 @@ int mi_keypoint_nms_oks(const float* xy_preds, const float* rois, int num_rois, 
  *   saved         kept by the caller from the forward to the backward; nothing but the forward writes it, so
  *                 several backward passes may follow, each with a workspace of its own
  * The backward takes grad_loss float32 ([1], or [rows] for MI_REDUCTION_NONE) and writes dense gradients [rows, dim],
- * [classes, dim], [classes]; each of the three may be NULL.  `weight` must be the forward's, unchanged.  Results do not depend on the
- * order of execution: every sum has a fixed order.  At most 2^24 rows and classes, 2^20 features, and 2^25 tiles of 64 x 64 of the
+ * [classes, dim], [classes]; each of the three may be NULL.  `weight` must have the forward's elements, unchanged; they may lie elsewhere,
+ * at another distance of rows, but where mi_linear_cross_entropy_saved_bytes asks for more there than for the forward's, the forward
+ * has not kept what the backward needs.  Results do not depend on the order of execution: every sum has a fixed order.  At most 2^24 rows and classes, 2^20 features, and 2^25 tiles of 64 x 64 of the
  * logits (MI_ERR_BAD_ARGUMENT beyond).  `saved` and `workspace` start on 256 bytes, gradients
  * on 16. */
 size_t mi_linear_cross_entropy_saved_bytes(int rows, int dim, int classes, int dtype, const void* weight,
