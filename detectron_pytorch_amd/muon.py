@@ -65,6 +65,8 @@ def muon_step_(params, grads, momenta, lr, momentum=0.95, weight_decay=0.0, nest
                                      polynomial(coefficients), float(eps), workspace.data_ptr(), workspace.numel(),
                                      _lib.current_stream_handle(dev))
     _lib.check(rc, "mi_muon_step")
+    # written through their addresses: a backward over a graph from before the step has to see it, as after torch's own optimisers
+    torch.autograd.graph.increment_version([t for t in ps + ms if not t.is_inference()])
 
 
 def as_matrix(t):
