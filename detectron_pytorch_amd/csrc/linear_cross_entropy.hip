@@ -31,7 +31,8 @@ namespace {
 
 constexpr int kPad = 64;              // rows and classes of the operands' k axes are padded to this
 constexpr int kMaxParts = 1024;       // workgroups of the maximum's pass
-constexpr float kQScale = 16384.f;    // q is stored times 2^14: fp16 keeps probabilities down to 2^-38
+constexpr int kQExponent = 14;        // q is stored times 2^14: fp16 keeps probabilities down to 2^-38
+constexpr float kQScale = 1 << kQExponent;
 constexpr int kIgnored = -1, kOutside = -2;
 constexpr int kIsNaN = 1 << 30;       // mark of a predicted class whose logit is NaN
 constexpr int kNoClass = kIsNaN - 1;
@@ -97,9 +98,9 @@ Plan make_plan(int rows, int dim, int classes, int dtype, bool w_in_place) {
 }
 
 struct Scalars {        // at scalars_at
-  float inv_x, inv_w;   // what undoes the scales of features and weights, powers of two
-  float count;          // rows that count, at least 1
-  int done;             // workgroups of the join that are through
+  int ex, ew;   // features and weights are their stored forms times 2^ex and 2^ew
+  float count;  // rows that count, at least 1
+  int done;     // workgroups of the join that are through
 };
 struct Sum {
   double loss;
@@ -108,11 +109,10 @@ struct Sum {
 
 // ---- laying out --------------------------------------------------------------------------------------------------------
 
-// 2^(14 - floor(log2 m)); 1 for zero and for what is no number
-__device__ __forceinline__ float scale_of(float m) {
-  if (!(m > 0.f) || m > kLargest) return 1.f;
-  const int e = 14 - ilogbf(m);
-  return ldexpf(1.f, min(max(e, -120), 120));
+// 14 - floor(log2 m); 0 for zero and for what is no number
+__device__ __forceinline__ int exponent_of(float m) {
+  if (!(m > 0.f) || m > kLargest) return 0;
+  return min(max(14 - ilogbf(m), -120), 120);
 }
 
 // Four float32 from `p`: one load where the row starts on 16 bytes (`aligned`), else one each; zeros behind `left` elements.
@@ -167,7 +167,7 @@ __global__ __launch_bounds__(256) void lay_out(const void* x, long long x_stride
                                                int dim, int dim_p, uint16_t* xo, uint16_t* wo, int* lab, const float* parts,
                                                int x_parts, int w_parts, Scalars* sc) {
   constexpr bool split = T == MI_TYPE_F32;
-  __shared__ float scales[2];
+  __shared__ int scales[2];  // their exponents
   if constexpr (split) {
     __shared__ float s[2][4];
     float mx = 0.f, mw = 0.f;
@@ -178,12 +178,12 @@ __global__ __launch_bounds__(256) void lay_out(const void* x, long long x_stride
     __syncthreads();
     if (threadIdx.x < 2) {
       const float* v = s[threadIdx.x];
-      scales[threadIdx.x] = scale_of(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
+      scales[threadIdx.x] = exponent_of(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
     }
     __syncthreads();
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) {
-    sc->inv_x = split ? 1.f / scales[0] : 1.f, sc->inv_w = split ? 1.f / scales[1] : 1.f;
+    sc->ex = split ? -scales[0] : 0, sc->ew = split ? -scales[1] : 0;
     sc->done = 0;
   }
   for (int i = blockIdx.x * 256 + threadIdx.x; i < rows_p; i += gridDim.x * 256) {
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(256) void lay_out(const void* x, long long x_stride
     const char* src = static_cast<const char*>(is_x ? x : w) + (long long)row * (is_x ? x_stride : w_stride) * bytes;
     const bool aligned = reinterpret_cast<uintptr_t>(src) % 16 == 0;
     uint16_t* to = (is_x ? xo : wo) + (long long)row * dim_p * (split ? 2 : 1);
-    const float scale = split ? scales[is_x ? 0 : 1] : 1.f;
+    const float scale = split ? ldexpf(1.f, scales[is_x ? 0 : 1]) : 1.f;
 #pragma unroll 2
     for (int c = lane * 8; c < dim_p; c += 512) {
       s16x8 hi = {0, 0, 0, 0, 0, 0, 0, 0}, lo = hi;
@@ -274,7 +274,7 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_forward(
   f32x16 acc[P::FM][P::FN];
   P::run(acc, x, w, tm * P::BM, tn * P::BN, 0, steps, (lds_bytes)smem);
   const int row0 = tm * P::BM + P::lane_row(), col0 = tn * P::BN + P::lane_col();
-  const float ix = P::SPLIT ? sc->inv_x : 1.f, iw = P::SPLIT ? sc->inv_w : 1.f;
+  const int scale = P::SPLIT ? sc->ex + sc->ew : 0;  // one step: neither factor's own scale may leave the range of a float
   float b[P::FN][16];
   load_bias<P, T>(b, bias, 0, col0, classes);
   const int strip = tn * P::WC + uniform((int)(threadIdx.x >> 6)) % P::WC;
@@ -287,7 +287,7 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_forward(
     for (int j = 0; j < P::FN; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        acc[i][j][e] = (P::SPLIT ? acc[i][j][e] * ix * iw : acc[i][j][e]) + b[j][e];
+        acc[i][j][e] = (P::SPLIT ? ldexpf(acc[i][j][e], scale) : acc[i][j][e]) + b[j][e];
         m = fmaxf(m, acc[i][j][e]);
       }
     const int in = y - col0;  // the label's class among the wave's columns, from the lane's first one on
@@ -433,9 +433,18 @@ struct Factor {
   const float* scale;  // [1], behind the rows' factors
   int mean;
 };
-__device__ __forceinline__ float value(const Factor& f) {
-  if (f.grad == nullptr) return *f.scale;
-  return (f.mean ? *f.grad / f.sc->count : *f.grad) * (1.f / kQScale);
+// It and the operands' scales, as one number in [1, 2) and a power of two: their product alone may be no float where the result is one.
+struct Undo {
+  float m;
+  int e;
+  __device__ __forceinline__ float operator()(float v) const { return ldexpf(v * m, e); }
+};
+__device__ __forceinline__ Undo undo(const Factor& f, int e) {
+  const float v = f.grad == nullptr ? *f.scale : f.mean ? *f.grad / f.sc->count : *f.grad;
+  if (f.grad != nullptr) e -= kQExponent;
+  if (!(fabsf(v) > 0.f && fabsf(v) <= kLargest)) return {v, 0};
+  const int k = ilogbf(v);
+  return {ldexpf(v, -k), k + e};
 }
 
 // Gradients of single rows, times a power of two so that the largest of them fills the type.
@@ -450,7 +459,7 @@ __global__ __launch_bounds__(1024) void row_factors(const float* grad, const int
   if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
   __syncthreads();
   for (int i = 0; i < 16; ++i) m = fmaxf(m, sm[i]);
-  const float s = scale_of(m) * 0.5f;
+  const float s = ldexpf(0.5f, exponent_of(m));
   for (int i = threadIdx.x; i < rows_p; i += 1024) factors[i] = (i >= rows || lab[i] == kIgnored) ? 0.f : grad[i] * s;
   if (threadIdx.x == 0) factors[rows_p] = 1.f / s;
 }
@@ -470,7 +479,7 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_backward
   f32x16 acc[P::FM][P::FN];
   P::run(acc, x, w, tm * P::BM, tn * P::BN, 0, steps, (lds_bytes)smem);
   const int row0 = tm * P::BM + P::lane_row(), col0 = tn * P::BN + P::lane_col();
-  const float ix = P::SPLIT ? sc->inv_x : 1.f, iw = P::SPLIT ? sc->inv_w : 1.f;
+  const int scale = P::SPLIT ? sc->ex + sc->ew : 0;  // one step: neither factor's own scale may leave the range of a float
   const long long ld = (long long)classes_p * (P::SPLIT ? 2 : 1);
   float b[P::FN][16], sum[P::FN][16];
   load_bias<P, T>(b, bias, class0, col0, classes);
@@ -490,7 +499,7 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_backward
     for (int j = 0; j < P::FN; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        acc[i][j][e] = __expf((P::SPLIT ? acc[i][j][e] * ix * iw : acc[i][j][e]) + b[j][e] - l) * f;
+        acc[i][j][e] = __expf((P::SPLIT ? ldexpf(acc[i][j][e], scale) : acc[i][j][e]) + b[j][e] - l) * f;
     if (__any(ignored)) {  // rows that do not count, also beside a bias or weight that is no number
 #pragma unroll
       for (int j = 0; j < P::FN; ++j)
@@ -566,7 +575,7 @@ __device__ __forceinline__ void gradient_tile(const Gradient& g, int id, const F
   f32x16 acc[P::FM][P::FN];
   const int step0 = slice * g.per_slice;
   P::run(acc, g.a, g.b, tm * P::BM, tn * P::BN, step0, min(g.per_slice, g.steps - step0), lds);
-  const float f = value(factor) * (P::SPLIT ? (OF_WEIGHT ? factor.sc->inv_x : factor.sc->inv_w) : 1.f);
+  const Undo scaled = undo(factor, P::SPLIT ? (OF_WEIGHT ? factor.sc->ex : factor.sc->ew) : 0);
   const bool whole = (g.cols & 3) == 0;  // then every four columns of a lane are inside or outside together, and aligned
   P::hand_out(acc, lds, [&](int r0, int c0, f32x4 v) {
     const int row = tm * P::BM + r0, col = tn * P::BN + c0;
@@ -582,7 +591,8 @@ __device__ __forceinline__ void gradient_tile(const Gradient& g, int id, const F
       }
       return;
     }
-    v *= f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = scaled(v[r]);
     const long long at = (long long)row * g.cols + col;
     if (whole && T == MI_TYPE_F32) {
       *reinterpret_cast<f32x4*>(static_cast<float*>(g.out) + at) = v;
@@ -619,7 +629,7 @@ __global__ __launch_bounds__(PX::kThreads, kWavesPerSimd<PX>) void gradients(Gra
     __syncthreads();
     if (at != 0 || c >= bias.classes) return;
     for (int s = 1; s < PX::kThreads / 64; ++s) v += part[s * 64 + threadIdx.x];
-    store_from_float<T>(bias.out, c, v * value(factor));
+    store_from_float<T>(bias.out, c, undo(factor, 0)(v));
   }
 }
 
@@ -635,14 +645,14 @@ __global__ __launch_bounds__(256) void join_slices(Joined x, Joined w, int x_blo
   const bool is_x = (int)blockIdx.x < x_blocks;
   const Joined& j = is_x ? x : w;
   const int block = is_x ? blockIdx.x : blockIdx.x - x_blocks, blocks = is_x ? x_blocks : gridDim.x - x_blocks;
-  const float f = value(factor) * (T == MI_TYPE_F32 ? (is_x ? factor.sc->inv_w : factor.sc->inv_x) : 1.f);
+  const Undo scaled = undo(factor, T == MI_TYPE_F32 ? (is_x ? factor.sc->ew : factor.sc->ex) : 0);
   const bool whole = (j.count & 3) == 0;
   for (long long i = (block * 256LL + threadIdx.x) * 4; i < j.count; i += blocks * 1024LL) {
     const int left = j.count - i < 4 ? (int)(j.count - i) : 4;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int s = 0; s < j.n; ++s) v += four(j.slices + s * j.count + i, left, whole);
-    for (int r = 0; r < left; ++r) store_from_float<T>(j.out, i + r, v[r] * f);
+    for (int r = 0; r < left; ++r) store_from_float<T>(j.out, i + r, scaled(v[r]));
   }
 }
 
