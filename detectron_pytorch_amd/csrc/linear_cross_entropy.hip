@@ -16,14 +16,20 @@
 // Types.  16-bit features and weights are multiplied as they are, in place.  float32 ones are laid out as hi + lo fp16 under one
 // power-of-two scale per tensor (its largest finite magnitude lands in [2^14, 2^15), so hi + lo carry 22 bits for
 // everything within 2^18 of it and lose one bit per halving below).  Maximum, sum, lse, loss and all accumulators are float32;
-// the sum over rows is fp64.  q is rounded once, to the features' type: |q| <= 1 and the error of a gradient element
-// is that of a sum of such roundings, below the rounding of the gradient itself; for float32 q is hi + lo again.
+// the sum over rows is fp64.
+// q is stored times 2^14 in 16 bits: in the features' type, for float32 as hi + lo fp16.  Against that, elements of q near 1 (a row's own
+// class) keep 8, 11 or 22 bits, as many as the type of the gradients holds; in fp16 and float32 the smallest step is 2^-38, so a
+// probability keeps all its bits down to 2^-28 (float32: 2^-17, one bit less per halving below) and is zero below 2^-39.  A gradient
+// element whose terms are all that small, a class that no row is near, is off by as much: in float32 by 1e-5 of itself where its
+// probabilities are 2^-28.  Gradients of single rows are kept apart from q as powers of two, so dx has these bits in every row; in dw
+// rows are summed, and there a row's part is rounded at 2^-38 of the largest row gradient (weigh_rows).
 //
 // Rows with the ignored label are laid out as zeros, whatever they hold, and get q = 0.  A label that is neither ignored nor
 // a class makes its row's loss and gradient NaN.
 #include "common.h"
 #include "tile_product.h"
 
+#include <climits>
 #include <cmath>
 
 namespace mi {
@@ -426,11 +432,17 @@ __global__ __launch_bounds__(256) void join_strips(const float2* part, const int
 
 // ---- backward ------------------------------------------------------------------------------------------------------------
 
-// What the finished sums are multiplied with.  A common gradient stays out of q; gradients of single rows are in it already.
+// A single row's gradient as m 2^(E + log2 w): E is the largest exponent of all rows, m in [1, 2), w a power of two up to 1 (0: the row
+// does not count).  q holds m only, so that a row of small gradient keeps its bits; dx gets w when its sums are done.
+struct RowFactor {
+  float m, w;
+};
+// What the finished sums are multiplied with.  A common gradient stays out of q.
 struct Factor {
   const float* grad;  // of the loss; NULL: the rows' factors are in use
   const Scalars* sc;
-  const float* scale;  // [1], behind the rows' factors
+  const RowFactor* rows;
+  const int* exponent;  // E
   int mean;
 };
 // It and the operands' scales, as one number in [1, 2) and a power of two: their product alone may be no float where the result is one.
@@ -440,37 +452,77 @@ struct Undo {
   __device__ __forceinline__ float operator()(float v) const { return ldexpf(v * m, e); }
 };
 __device__ __forceinline__ Undo undo(const Factor& f, int e) {
-  const float v = f.grad == nullptr ? *f.scale : f.mean ? *f.grad / f.sc->count : *f.grad;
-  if (f.grad != nullptr) e -= kQExponent;
+  e -= kQExponent;
+  if (f.grad == nullptr) return {1.f, e + *f.exponent};
+  const float v = f.mean ? *f.grad / f.sc->count : *f.grad;
   if (!(fabsf(v) > 0.f && fabsf(v) <= kLargest)) return {v, 0};
   const int k = ilogbf(v);
   return {ldexpf(v, -k), k + e};
 }
 
-// Gradients of single rows, times a power of two so that the largest of them fills the type.
-__global__ __launch_bounds__(1024) void row_factors(const float* grad, const int* lab, int rows, int rows_p, float* factors) {
-  float m = 0.f;
-  for (int i = threadIdx.x; i < rows; i += 1024) {
-    const float v = fabsf(grad[i]);
-    if (lab[i] != kIgnored && v <= kLargest) m = fmaxf(m, v);
-  }
-  for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-  __shared__ float sm[16];
-  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
+__global__ __launch_bounds__(1024) void row_factors(const float* grad, const int* lab, int rows, int rows_p, RowFactor* factors,
+                                                    int* exponent) {
+  const auto counts = [](float v) { return fabsf(v) > 0.f && fabsf(v) <= kLargest; };
+  int most = INT_MIN;
+  for (int i = threadIdx.x; i < rows; i += 1024)
+    if (lab[i] != kIgnored && counts(grad[i])) most = max(most, ilogbf(grad[i]));
+  for (int d = 32; d; d >>= 1) most = max(most, __shfl_xor(most, d));
+  __shared__ int sm[16];
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = most;
   __syncthreads();
-  for (int i = 0; i < 16; ++i) m = fmaxf(m, sm[i]);
-  const float s = ldexpf(0.5f, exponent_of(m));
-  for (int i = threadIdx.x; i < rows_p; i += 1024) factors[i] = (i >= rows || lab[i] == kIgnored) ? 0.f : grad[i] * s;
-  if (threadIdx.x == 0) factors[rows_p] = 1.f / s;
+  for (int i = 0; i < 16; ++i) most = max(most, sm[i]);
+  if (most == INT_MIN) most = 0;
+  for (int i = threadIdx.x; i < rows_p; i += 1024) {
+    RowFactor f = {0.f, 0.f};
+    if (i < rows && lab[i] != kIgnored) {
+      const float g = grad[i];
+      const int e = counts(g) ? ilogbf(g) : most;
+      f = {counts(g) ? ldexpf(g, -e) : g, ldexpf(1.f, e - most)};
+    }
+    factors[i] = f;
+  }
+  if (threadIdx.x == 0) *exponent = most;
 }
 
-// One tile of logits, again -> q times its row's factor; column sums for the bias gradient, one strip per wave row.  Forming the
+// q times its rows' w, for q' x: there the rows are summed, and only their ratios count.  What falls below 2^-38 of the largest row's
+// gradient is lost.  A wave takes a row; rows of the largest exponent stay as they are.
+template <int T>
+__global__ __launch_bounds__(256) void weigh_rows(const RowFactor* factors, int rows_p, int classes_p, uint16_t* q) {
+  constexpr int words = T == MI_TYPE_F32 ? 2 : 1;
+  for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < rows_p; r += gridDim.x * 4) {
+    const float w = factors[r].w;
+    if (w == 1.f || w == 0.f) continue;  // 0: a row of zeros
+    uint16_t* row = q + (long long)r * classes_p * words;
+    for (int c = (threadIdx.x & 63) * 8; c < classes_p; c += 512) {
+      if constexpr (T == MI_TYPE_F32) {
+        s16x8 *hi = reinterpret_cast<s16x8*>(row + (c >> 5) * 64 + (c & 31)), *lo = hi + 4;
+        s16x8 h = *hi, l = *lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float v = (to_float((uint16_t)h[e], false) + to_float((uint16_t)l[e], false)) * w;
+          const _Float16 f = (_Float16)v;
+          h[e] = __builtin_bit_cast(short, f);
+          l[e] = (short)half_bits(v - (float)f);
+        }
+        *hi = h, *lo = l;
+      } else {
+        s16x8* at = reinterpret_cast<s16x8*>(row + c);
+        s16x8 h = *at;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = (short)round16<T>(to_float((uint16_t)h[e], T == MI_TYPE_BF16) * w);
+        *at = h;
+      }
+    }
+  }
+}
+
+// One tile of logits, again -> q times its row's m (`whole`: and w); column sums for the bias gradient, one strip per wave row.  Forming the
 // logits a second time costs 2 R V D operations; keeping them would cost 8 R V bytes of traffic and 4 R V of memory.
 template <class P, int T>
 __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_backward(Operand x, Operand w, const void* bias,
                                                                                  const int* lab, const float* lse,
-                                                                                 const float* factors, const Scalars* sc,
-                                                                                 int rows_p, int class0, int classes, int classes_p,
+                                                                                 const RowFactor* factors, int whole,
+                                                                                 const Scalars* sc, int rows_p, int class0, int classes, int classes_p,
                                                                                  int tiles_m, int tiles_n, int steps, uint16_t* q,
                                                                                  float* sums) {
   extern __shared__ char smem[];
@@ -494,7 +546,12 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_backward
     const int label = in ? lab[row] : kIgnored, y = label - class0 - col0;
     const bool ignored = label == kIgnored;
     const float l = in ? lse[row] : INFINITY;
-    const float f = factors != nullptr ? (in ? factors[row] : 0.f) : kQScale;
+    RowFactor g = {1.f, 1.f};
+    if (factors != nullptr) {
+      g = in ? factors[row] : RowFactor{0.f, 0.f};
+      if (whole) g = {g.m * g.w, 1.f};
+    }
+    const float f = g.m * kQScale;
 #pragma unroll
     for (int j = 0; j < P::FN; ++j)
 #pragma unroll
@@ -515,7 +572,7 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_backward
 #pragma unroll
     for (int j = 0; j < P::FN; ++j)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sum[j][e] += acc[i][j][e];
+      for (int e = 0; e < 16; ++e) sum[j][e] = fmaf(acc[i][j][e], g.w, sum[j][e]);
   }
   P::hand_out(acc, (lds_bytes)smem, [&](int r, int c, f32x4 v) {
     const int row = tm * P::BM + r, col = tn * P::BN + c;
@@ -580,6 +637,11 @@ __device__ __forceinline__ void gradient_tile(const Gradient& g, int id, const F
   P::hand_out(acc, lds, [&](int r0, int c0, f32x4 v) {
     const int row = tm * P::BM + r0, col = tn * P::BN + c0;
     if (row >= g.rows || col >= g.cols) return;
+    if (!OF_WEIGHT && factor.rows != nullptr) {
+      const float w = factor.rows[row].w;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = w == 0.f ? 0.f : v[r] * w;
+    }
     if (g.slices != nullptr) {
       float* at = g.slices + ((long long)slice * g.rows + row) * g.cols + col;
       if (whole) {
@@ -716,7 +778,7 @@ Pieces make_pieces(const Plan& p) {
   size_t at = 0;
   c.q_at = at, at = up(at + (size_t)p.rows_p * c.width * words * 2);
   c.sums_at = at, at = up(at + (size_t)(ceil_div(p.rows_p, 64) * 2) * c.width * 4);
-  c.factors_at = at, at = up(at + (size_t)(p.rows_p + 1) * 4);
+  c.factors_at = at, at = up(at + (size_t)(p.rows_p + 1) * sizeof(RowFactor));  // E behind them
   c.x_at = at, at = up(at + (c.x_joined ? (size_t)c.cut.x * p.rows * p.dim * 4 : 0));
   c.w_at = at, at = up(at + (c.cut.w > 1 ? (size_t)c.cut.w * c.width * p.dim * 4 : 0));
   c.bytes = at;
@@ -815,7 +877,7 @@ int forward(const Plan& p, const Call& c, float* loss, float* losses, int64_t* p
 }
 
 template <class P, int T>
-int launch_q(const Plan& p, const Call& c, const Pieces& s, int class0, int classes, int classes_p, bool want_bias) {
+int launch_q(const Plan& p, const Call& c, const Pieces& s, int class0, int classes, int classes_p, bool want_bias, bool whole) {
   const Operand x = {reinterpret_cast<uint16_t*>(c.saved + p.x_at), p.ld, p.rows_p, p.dim_p};
   const long long ld = weights_ld(p, c);
   const Operand w = {weights_of(p, c) + (long long)class0 * ld, ld, classes, p.dim_p};
@@ -823,7 +885,7 @@ int launch_q(const Plan& p, const Call& c, const Pieces& s, int class0, int clas
   allow_lds(logits_backward<P, T>, P::kLds);
   logits_backward<P, T><<<tm * tn, P::kThreads, P::kLds, c.stream>>>(
       x, w, c.bias, reinterpret_cast<const int*>(c.saved + p.lab_at), reinterpret_cast<const float*>(c.saved + p.lse_at),
-      c.reduction == MI_REDUCTION_NONE ? reinterpret_cast<const float*>(c.room + s.factors_at) : nullptr,
+      c.reduction == MI_REDUCTION_NONE ? reinterpret_cast<const RowFactor*>(c.room + s.factors_at) : nullptr, whole,
       reinterpret_cast<const Scalars*>(c.saved + p.scalars_at), p.rows_p, class0, classes, classes_p, tm, tn,
       p.dim_p / P::kStep, reinterpret_cast<uint16_t*>(c.room + s.q_at),
       want_bias ? reinterpret_cast<float*>(c.room + s.sums_at) : nullptr);
@@ -849,12 +911,14 @@ int backward(const Plan& p, const Call& c, const float* grad, void* grad_x, void
   constexpr int words = split ? 2 : 1, step = split ? 32 : 64, out_bytes = T == MI_TYPE_F32 ? 4 : 2;
   const Pieces s = make_pieces(p);
   const Scalars* sc = reinterpret_cast<const Scalars*>(c.saved + p.scalars_at);
-  float* factors = reinterpret_cast<float*>(c.room + s.factors_at);
-  const bool by_row = c.reduction == MI_REDUCTION_NONE;
+  RowFactor* factors = reinterpret_cast<RowFactor*>(c.room + s.factors_at);
+  int* exponent = reinterpret_cast<int*>(factors + p.rows_p);
+  const bool by_row = c.reduction == MI_REDUCTION_NONE, apart = by_row && grad_x != nullptr && grad_w != nullptr;
   if (by_row)
-    row_factors<<<1, 1024, 0, c.stream>>>(grad, reinterpret_cast<const int*>(c.saved + p.lab_at), p.rows, p.rows_p, factors);
-  const Factor factor = {by_row ? nullptr : grad, sc, factors + p.rows_p, c.reduction == MI_REDUCTION_MEAN};
-  const uint16_t* q = reinterpret_cast<const uint16_t*>(c.room + s.q_at);
+    row_factors<<<1, 1024, 0, c.stream>>>(grad, reinterpret_cast<const int*>(c.saved + p.lab_at), p.rows, p.rows_p, factors,
+                                          exponent);
+  const Factor factor = {by_row ? nullptr : grad, sc, by_row ? factors : nullptr, exponent, c.reduction == MI_REDUCTION_MEAN};
+  uint16_t* q = reinterpret_cast<uint16_t*>(c.room + s.q_at);
   const long long ldw = weights_ld(p, c);
   float* x_room = s.x_joined ? reinterpret_cast<float*>(c.room + s.x_at) : nullptr;
   float* w_room = s.cut.w > 1 ? reinterpret_cast<float*>(c.room + s.w_at) : nullptr;
@@ -862,11 +926,11 @@ int backward(const Plan& p, const Call& c, const float* grad, void* grad_x, void
     const int class0 = k * s.width, classes = p.classes - class0 < s.width ? p.classes - class0 : s.width;
     const int classes_p = ceil_div(classes, kPad) * kPad;
     const int tile = tile_for(p.rows_p, classes_p, p.dim_p, split);
-    const bool want_b = grad_b != nullptr, ends = k + 1 == s.n;
+    const bool want_b = grad_b != nullptr, ends = k + 1 == s.n, whole = by_row && grad_x == nullptr;
     const int strips =
-        tile == 256   ? launch_q<Tile256<split, bf16, false, false>, T>(p, c, s, class0, classes, classes_p, want_b)
-        : tile == 128 ? launch_q<Tile128<split, bf16, false, false>, T>(p, c, s, class0, classes, classes_p, want_b)
-                      : launch_q<Tile64<split, bf16, false, false>, T>(p, c, s, class0, classes, classes_p, want_b);
+        tile == 256   ? launch_q<Tile256<split, bf16, false, false>, T>(p, c, s, class0, classes, classes_p, want_b, whole)
+        : tile == 128 ? launch_q<Tile128<split, bf16, false, false>, T>(p, c, s, class0, classes, classes_p, want_b, whole)
+                      : launch_q<Tile64<split, bf16, false, false>, T>(p, c, s, class0, classes, classes_p, want_b, whole);
     // every piece has the same slices of q W: a last, shorter piece leaves some of them empty
     const Gradient x = {{q, (long long)classes_p * words, p.rows_p, classes_p},
                         {weights_of(p, c) + class0 * ldw, ldw, p.dim, classes},
@@ -877,12 +941,22 @@ int backward(const Plan& p, const Call& c, const float* grad, void* grad_x, void
                         classes, p.dim, 0, 0, p.rows_p / step, 0, w_out, w_room, 0};
     const BiasGradient b = {reinterpret_cast<const float*>(c.room + s.sums_at), strips, classes, classes_p,
                             want_b ? static_cast<char*>(grad_b) + (size_t)class0 * out_bytes : nullptr};
-    if (s.cut.tile == 256)
-      launch_gradients<Tile256<split, bf16, false, true>, Tile256<split, bf16, true, true>, T>(x, w, b, s.cut, factor, c.stream);
-    else if (s.cut.tile == 128)
-      launch_gradients<Tile128<split, bf16, false, true>, Tile128<split, bf16, true, true>, T>(x, w, b, s.cut, factor, c.stream);
-    else
-      launch_gradients<Tile64<split, bf16, false, true>, Tile64<split, bf16, true, true>, T>(x, w, b, s.cut, factor, c.stream);
+    const auto multiply = [&](const Gradient& x, const Gradient& w, const BiasGradient& b) {
+      if (s.cut.tile == 256)
+        launch_gradients<Tile256<split, bf16, false, true>, Tile256<split, bf16, true, true>, T>(x, w, b, s.cut, factor, c.stream);
+      else if (s.cut.tile == 128)
+        launch_gradients<Tile128<split, bf16, false, true>, Tile128<split, bf16, true, true>, T>(x, w, b, s.cut, factor, c.stream);
+      else
+        launch_gradients<Tile64<split, bf16, false, true>, Tile64<split, bf16, true, true>, T>(x, w, b, s.cut, factor, c.stream);
+    };
+    if (apart) {
+      multiply(x, Gradient{}, b);
+      const int most = 8 * compute_units(), grid = ceil_div(p.rows_p, 4);
+      weigh_rows<T><<<grid < most ? grid : most, 256, 0, c.stream>>>(factors, p.rows_p, classes_p, q);
+      multiply(Gradient{}, w, BiasGradient{});
+    } else {
+      multiply(x, w, b);
+    }
     const Joined jx = {x_room, s.cut.x, (long long)p.rows * p.dim, grad_x};
     const Joined jw = {w_room, s.cut.w, (long long)classes * p.dim, w_out};
     const int bx = ends && grad_x != nullptr && x_room != nullptr ? grid_for(jx.count / 4, 256) : 0;

@@ -11,6 +11,8 @@ the log of the sum of exponentials only (reference of the plain form: lib/modeli
 x [rows, dim], weight [classes, dim], bias [classes] or None: all float32, all float16 or all bfloat16, on one GPU; labels int32
 or int64 [rows].  Sums, softmax statistics and the loss are float32.  float32 products carry 22 bits of each factor down to 2^-18 of
 the largest finite magnitude of its tensor, and one bit less per halving below that (an infinite factor makes its logits NaN).
+Gradients take probabilities with the bits of their type (float32: 22) and as zero below 2^-39 (float32, float16).  With
+reduction='none' that holds for each row of x's gradient by itself; in the weight's gradient, parts below 2^-38 of the largest row's are lost.
 """
 import torch
 from torch.autograd import Function

@@ -502,9 +502,11 @@ int mi_keypoint_nms_oks(const float* xy_preds, const float* rois, int num_rois, 
  * The backward takes grad_loss float32 ([1], or [rows] for MI_REDUCTION_NONE) and writes dense gradients [rows, dim],
  * [classes, dim], [classes]; each of the three may be NULL.  `weight` must have the forward's elements, unchanged; they may lie elsewhere,
  * at another distance of rows, but where mi_linear_cross_entropy_saved_bytes asks for more there than for the forward's, the forward
- * has not kept what the backward needs.  Results do not depend on the order of execution: every sum has a fixed order.  At most 2^24 rows and classes, 2^20 features, and 2^25 tiles of 64 x 64 of the
- * logits (MI_ERR_BAD_ARGUMENT beyond).  `saved` and `workspace` start on 256 bytes, gradients
- * on 16. */
+ * has not kept what the backward needs.  Gradients are formed from probabilities of `dtype`'s bits (float32: 22); in float32 and
+ * float16 those below 2^-39 count as zero, for MI_REDUCTION_NONE relative to the row's own gradient in grad_x, to the largest row's
+ * in grad_weight.  Results do not depend on the order of execution: every sum has a fixed order.  At most 2^24 rows and classes, 2^20
+ * features, and 2^25 tiles of 64 x 64 of the logits (MI_ERR_BAD_ARGUMENT beyond).  `saved` and `workspace` start on 256 bytes,
+ * gradients on 16. */
 size_t mi_linear_cross_entropy_saved_bytes(int rows, int dim, int classes, int dtype, const void* weight,
                                            long long weight_stride);
 size_t mi_linear_cross_entropy_workspace_bytes(int rows, int dim, int classes, int dtype, int pass);
