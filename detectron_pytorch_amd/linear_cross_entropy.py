@@ -37,6 +37,9 @@ def _check(x, weight, bias, labels, reduction):
                          % (tuple(x.shape), tuple(weight.shape)))
     if weight.numel() == 0:
         raise ValueError("linear_cross_entropy needs at least one class and one feature, got weight %s" % (tuple(weight.shape),))
+    if max(x.size(0), weight.size(0)) > 1 << 24 or x.size(1) > 1 << 20:   # (checked here too: a C int takes sizes modulo 2^32)
+        raise ValueError("linear_cross_entropy takes up to 2^24 rows and classes and 2^20 features, got x %s and weight %s"
+                         % (tuple(x.shape), tuple(weight.shape)))
     if dtype not in TYPES or weight.dtype != dtype:
         raise ValueError("linear_cross_entropy takes float32, float16 or bfloat16 x and weight of one type, got %s and %s"
                          % (dtype, weight.dtype))

@@ -33,6 +33,9 @@ def check_matrices(mats, what):
 def host_arrays(mats):
     """(count, rows, cols) of non-empty matrices as the C side takes them."""
     n = len(mats)
+    for t in mats:
+        if max(t.shape) > 1 << 22:   # (checked here too: a C int takes sizes modulo 2^32)
+            raise ValueError("matrices have sides of up to 2^22, got %s" % (tuple(t.shape),))
     return n, (ctypes.c_int * n)(*[t.size(0) for t in mats]), (ctypes.c_int * n)(*[t.size(1) for t in mats])
 
 
