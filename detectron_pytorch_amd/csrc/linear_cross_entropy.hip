@@ -5,8 +5,8 @@
 //   q_iv = exp(z_iv - lse_i) - [v = y_i],   dx_i = g_i sum_v q_iv w_v,   dw_v = sum_i g_i q_iv x_i,   db_v = sum_i g_i q_iv
 // The [rows, classes] logits are formed tile by tile on the matrix cores (tile_product.h) and die in registers: the forward
 // keeps, per row and strip of columns, the running maximum and the sum of exponentials, and a second kernel joins the
-// strips.  The backward forms the same tiles again, piece of the vocabulary by piece, turns them into q (16 bits, bounded
-// workspace) and multiplies q by the weights and by the features.
+// strips.  The backward forms the same tiles again, piece of the vocabulary by piece, turns them into q (16 bits or 2 x 16, up to 256 MB
+// of it at a time: make_pieces) and multiplies q by the weights and by the features.
 //
 // Work: 2 R V D operations forward, 6 R V D backward (one third of it the logits' second time).  Bound by the matrix cores
 // wherever R and V fill the chip: at 8192 x 4096 and 50021 classes in bf16 the forward's logits take 2.72 ms (1233 TFLOP/s), the
@@ -44,7 +44,12 @@ constexpr int kIsNaN = 1 << 30;       // mark of a predicted class whose logit i
 constexpr int kNoClass = kIsNaN - 1;
 constexpr int kElsewhere = 1 << 28;   // a row's largest logit is not among this lane's columns
 constexpr float kLargest = 3.402823466e38f;
-constexpr size_t kPieceBytes = size_t(1) << 30;  // q of one piece of the vocabulary
+// What a call may hold, so that it stays below the logits that it does without (make_pieces)
+constexpr size_t kMB = size_t(1) << 20;
+constexpr size_t kWeightBytes = 128 * kMB;  // laid-out weights: up to this they are kept from the forward to the backward, more of
+                                            // them are laid out in pieces of this, in either pass
+constexpr size_t kQBytes = 64 * kMB, kMostQBytes = 256 * kMB;  // q of a piece: half of the float32 logits between these
+constexpr size_t kSliceBytes = 32 * kMB;    // sums of the slices of one product, where it has several
 
 __device__ __forceinline__ float to_float(uint16_t v, bool bf16) {
   return bf16 ? __uint_as_float((unsigned)v << 16) : (float)__builtin_bit_cast(_Float16, v);
@@ -78,6 +83,7 @@ struct Plan {
   int rows, dim, classes;
   int rows_p, dim_p;        // padded to kPad
   bool split, copy_w;       // float32; weights laid out anew (float32, or 16-bit ones that the product cannot take in place)
+  bool keep_w;              // the whole of them lies in `saved`; otherwise a piece at a time in the workspace, in both passes
   long long ld;             // words between rows of a laid-out operand
   size_t x_at, lab_at, lse_at, scalars_at, w_at, saved_bytes;
 };
@@ -92,13 +98,15 @@ Plan make_plan(int rows, int dim, int classes, int dtype, bool w_in_place) {
   p.split = dtype == MI_TYPE_F32;
   p.copy_w = p.split || !w_in_place;
   p.ld = (long long)p.dim_p * (p.split ? 2 : 1);
+  // 16-bit weights of padded dim that lie off 16 bytes are kept whatever their size: the workspace's size does not know where they lie
+  p.keep_w = p.copy_w && ((size_t)classes * p.ld * 2 <= kWeightBytes || (!p.split && dim % kPad == 0));
   size_t at = 0;
   p.x_at = at, at = up(at + (size_t)p.rows_p * p.ld * 2);
   p.lab_at = at, at = up(at + (size_t)p.rows_p * 4);
   p.lse_at = at, at = up(at + (size_t)p.rows_p * 4);
   p.scalars_at = at, at = up(at + 64);
   // the weights come last: a backward whose weight lies on another alignment than the forward's finds the rest where it was left
-  p.w_at = at, at = up(at + (p.copy_w ? (size_t)classes * p.ld * 2 : 0));
+  p.w_at = at, at = up(at + (p.keep_w ? (size_t)classes * p.ld * 2 : 0));
   p.saved_bytes = at;
   return p;
 }
@@ -165,6 +173,42 @@ __global__ __launch_bounds__(256) void largest(const float* x, long long x_strid
   if (threadIdx.x == 0) parts[blockIdx.x] = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
 }
 
+// One row in the product's form by one wave, a lane eight elements at a time.
+template <bool SPLIT>
+__device__ __forceinline__ void lay_out_row(const char* src, uint16_t* to, int dim, int dim_p, bool zero, float scale, int lane) {
+  const bool aligned = reinterpret_cast<uintptr_t>(src) % 16 == 0;
+#pragma unroll 2
+  for (int c = lane * 8; c < dim_p; c += 512) {
+    s16x8 hi = {0, 0, 0, 0, 0, 0, 0, 0}, lo = hi;
+    if constexpr (SPLIT) {
+      if (!zero) {
+        const float* p = reinterpret_cast<const float*>(src) + c;
+        const f32x4 v0 = four(p, dim - c, aligned), v1 = four(p + 4, dim - c - 4, aligned);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float v = (e < 4 ? v0[e & 3] : v1[e & 3]) * scale;
+          const _Float16 h = (_Float16)v;
+          hi[e] = __builtin_bit_cast(short, h);
+          lo[e] = (short)half_bits(v - (float)h);
+        }
+      }
+      uint16_t* at = to + (c >> 5) * 64 + (c & 31);
+      *reinterpret_cast<s16x8*>(at) = hi;
+      *reinterpret_cast<s16x8*>(at + 32) = lo;
+    } else {
+      const short* p = reinterpret_cast<const short*>(src) + c;
+      if (!zero && aligned && c + 8 <= dim) {
+        hi = *reinterpret_cast<const s16x8*>(p);
+      } else if (!zero) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < dim) hi[e] = p[e];
+      }
+      *reinterpret_cast<s16x8*>(to + c) = hi;
+    }
+  }
+}
+
 // Features (rows_p rows; ignored ones and the padding are zeros), weights and labels in the product's form.  A wave takes one
 // row at a time, a lane eight elements of it.  Bound by memory: 8192 x 4096 bf16 features in 25 us (5.3 TB/s).
 template <int T, class LABEL>
@@ -203,40 +247,20 @@ __global__ __launch_bounds__(256) void lay_out(const void* x, long long x_stride
     const int row = is_x ? r : r - rows_p;
     const bool zero = is_x && (row >= rows || (long long)labels[row] == ignore);
     const char* src = static_cast<const char*>(is_x ? x : w) + (long long)row * (is_x ? x_stride : w_stride) * bytes;
-    const bool aligned = reinterpret_cast<uintptr_t>(src) % 16 == 0;
-    uint16_t* to = (is_x ? xo : wo) + (long long)row * dim_p * (split ? 2 : 1);
-    const float scale = split ? ldexpf(1.f, scales[is_x ? 0 : 1]) : 1.f;
-#pragma unroll 2
-    for (int c = lane * 8; c < dim_p; c += 512) {
-      s16x8 hi = {0, 0, 0, 0, 0, 0, 0, 0}, lo = hi;
-      if constexpr (split) {
-        if (!zero) {
-          const float* p = reinterpret_cast<const float*>(src) + c;
-          const f32x4 v0 = four(p, dim - c, aligned), v1 = four(p + 4, dim - c - 4, aligned);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float v = (e < 4 ? v0[e & 3] : v1[e & 3]) * scale;
-            const _Float16 h = (_Float16)v;
-            hi[e] = __builtin_bit_cast(short, h);
-            lo[e] = (short)half_bits(v - (float)h);
-          }
-        }
-        uint16_t* at = to + (c >> 5) * 64 + (c & 31);
-        *reinterpret_cast<s16x8*>(at) = hi;
-        *reinterpret_cast<s16x8*>(at + 32) = lo;
-      } else {
-        const short* p = reinterpret_cast<const short*>(src) + c;
-        if (!zero && aligned && c + 8 <= dim) {
-          hi = *reinterpret_cast<const s16x8*>(p);
-        } else if (!zero) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (c + e < dim) hi[e] = p[e];
-        }
-        *reinterpret_cast<s16x8*>(to + c) = hi;
-      }
-    }
+    lay_out_row<split>(src, (is_x ? xo : wo) + (long long)row * dim_p * (split ? 2 : 1), dim, dim_p, zero,
+                       split ? ldexpf(1.f, scales[is_x ? 0 : 1]) : 1.f, lane);
   }
+}
+
+// A piece of the weights, under the scale that `lay_out` found.
+template <int T>
+__global__ __launch_bounds__(256) void lay_out_weights(const void* w, long long w_stride, int classes, int dim, int dim_p, uint16_t* wo,
+                                                       const Scalars* sc) {
+  constexpr bool split = T == MI_TYPE_F32;
+  const float scale = split ? ldexpf(1.f, -sc->ew) : 1.f;
+  for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < classes; r += gridDim.x * 4)
+    lay_out_row<split>(static_cast<const char*>(w) + (long long)r * w_stride * (split ? 4 : 2),
+                       wo + (long long)r * dim_p * (split ? 2 : 1), dim, dim_p, false, scale, threadIdx.x & 63);
 }
 
 // ---- forward -------------------------------------------------------------------------------------------------------------
@@ -272,8 +296,9 @@ __device__ __forceinline__ void load_bias(float (&b)[P::FN][16], const void* bia
 template <class P, int T, bool PRED>
 __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_forward(Operand x, Operand w, const void* bias,
                                                                                 const int* lab, const Scalars* sc, int rows,
-                                                                                int rows_p, int classes, int tiles_m, int tiles_n,
-                                                                                int steps, float2* part, int* best, float* target) {
+                                                                                int rows_p, int class0, int classes, int tiles_m,
+                                                                                int tiles_n, int steps, float2* part, int* best,
+                                                                                float* target) {
   extern __shared__ char smem[];
   int tm, tn;
   tile_of(blockIdx.x, tiles_m, tiles_n, 4, tm, tn);
@@ -282,7 +307,7 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_forward(
   const int row0 = tm * P::BM + P::lane_row(), col0 = tn * P::BN + P::lane_col();
   const int scale = P::SPLIT ? sc->ex + sc->ew : 0;  // one step: neither factor's own scale may leave the range of a float
   float b[P::FN][16];
-  load_bias<P, T>(b, bias, 0, col0, classes);
+  load_bias<P, T>(b, bias, class0, col0, classes);
   const int strip = tn * P::WC + uniform((int)(threadIdx.x >> 6)) % P::WC;
 #pragma unroll
   for (int i = 0; i < P::FM; ++i) {
@@ -296,7 +321,7 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_forward(
         acc[i][j][e] = (P::SPLIT ? ldexpf(acc[i][j][e], scale) : acc[i][j][e]) + b[j][e];
         m = fmaxf(m, acc[i][j][e]);
       }
-    const int in = y - col0;  // the label's class among the wave's columns, from the lane's first one on
+    const int in = y - class0 - col0;  // the label's class among the wave's columns, from the lane's first one on
     if (__any(in >= 0 && in < P::FN * 32)) {
 #pragma unroll
       for (int j = 0; j < P::FN; ++j)
@@ -319,7 +344,7 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_forward(
     const bool writes = row < rows && (threadIdx.x & 32) == 0;
     if (writes) part[(long long)strip * rows_p + row] = make_float2(m, s);
     if constexpr (PRED) {
-      at += col0;
+      at += class0 + col0;
       if (__any(s != s)) {  // the first NaN, where the row has one
         int first = kNoClass, inside = classes - col0;
         asm volatile("" : "+v"(inside));  // compared here only: kept for all rows, 64 results would fill the scalar registers
@@ -327,7 +352,7 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_forward(
         for (int j = P::FN - 1; j >= 0; --j)
 #pragma unroll
           for (int e = 15; e >= 0; --e)
-            first = j * 32 + column(e) < inside && acc[i][j][e] != acc[i][j][e] ? col0 + j * 32 + column(e) : first;
+            first = j * 32 + column(e) < inside && acc[i][j][e] != acc[i][j][e] ? class0 + col0 + j * 32 + column(e) : first;
         const int other = min(first, __shfl_xor(first, 32));
         if (other != kNoClass) at = other | kIsNaN;
       }
@@ -727,21 +752,22 @@ int tile_for(long long m, long long n, int k, bool split) {
 }
 
 // Tile of both gradients' products and the slices of their k axes: the least estimated time.  A slice is at least 8 stages long;
-// a join costs a launch and its slices' way to memory and back (8 bytes an element at 4 TB/s).
+// a join costs a launch and its slices' way to memory and back (8 bytes an element at 4 TB/s), and slices stay within kSliceBytes.
 struct Cut {
   int tile, x, w;
+  float us;
 };
 Cut cut_for(const Plan& p, int width, bool x_joined) {
   const int step = p.split ? 32 : 64;
   const long long xs = width / step, ws = p.rows_p / step;
-  Cut best = {64, 1, 1};
-  float least = INFINITY;
+  Cut best = {64, 1, 1, INFINITY};
   for (int tile : {256, 128, 64}) {
     const long long xt = (long long)ceil_div(p.rows, tile) * ceil_div(p.dim, tile), wt = (long long)ceil_div(width, tile) * ceil_div(p.dim, tile);
     const TileTime t = tile_time(tile, p.split);
     const long long places = tile_places(tile);
-    for (long long a = 1; a == 1 || (a <= 64 && xs / a >= 8); a *= 2)
-      for (long long b = 1; b == 1 || (b <= 64 && ws / b >= 8); b *= 2) {
+    const long long x_bytes = 4LL * p.rows * p.dim, w_bytes = 4LL * width * p.dim, most = kSliceBytes;
+    for (long long a = 1; a == 1 || (a <= 64 && xs / a >= 8 && a * x_bytes <= most); a *= 2)
+      for (long long b = 1; b == 1 || (b <= 64 && ws / b >= 8 && b * w_bytes <= most); b *= 2) {
         const long long blocks = xt * a + wt * b, longest = xs / a > ws / b ? xs / a : ws / b;
         float us = t.around + longest * t.alone;
         if (blocks > places / 2) {  // the longest tile may begin when the others are half through
@@ -752,7 +778,7 @@ Cut cut_for(const Plan& p, int width, bool x_joined) {
         if (xj || wj) us += 4.f;
         if (xj) us += 2e-6f * p.rows * p.dim * (a + 1);
         if (wj) us += 2e-6f * width * p.dim * (b + 1);
-        if (us < least) least = us, best = {tile, (int)a, (int)b};
+        if (us < best.us) best = {tile, (int)a, (int)b, us};
       }
   }
   return best;
@@ -762,18 +788,59 @@ struct Pieces {
   int n, width;  // of the vocabulary; width is a multiple of kPad
   Cut cut;
   bool x_joined;
-  size_t q_at, sums_at, factors_at, x_at, w_at, bytes;
+  size_t q_at, sums_at, factors_at, x_at, w_at, weights_at, bytes;
 };
 
+// Classes of one piece of laid-out weights.
+int weights_width(const Plan& p) {
+  const long long most = (long long)(kWeightBytes / ((size_t)p.ld * 2)) / kPad * kPad;
+  return most < kPad ? kPad : most < p.classes ? (int)most : ceil_div(p.classes, kPad) * kPad;
+}
+// Whether they come in pieces; the same for weights that turn out to be read in place.
+bool weights_in_pieces(const Plan& p) {
+  return (size_t)p.classes * p.ld * 2 > kWeightBytes && (p.split || p.dim % kPad != 0);
+}
+
+// The backward's workspace.  q of a piece takes at most half of what float32 logits of all classes would, and at most 256 MB (64 MB
+// where half is less: smaller pieces would leave compute units empty); beside it lie at most an eighth of that in sums for the
+// bias, 32 MB in slices of each product, dx in float32 where there are several pieces, and 128 MB of weights that are not kept (or 64
+// of them).  Several pieces cost the adding up of dx and a launch's last, half-empty round each: 8192 x 4096 and 50021 classes in
+// bf16 take the 11.1 ms that one piece of 0.82 GB takes; pieces of 55 MB cost 8192 x 1024 and 10000 classes 12 %, weights laid out
+// twice 512 x 4096 and 50000 classes in float32 15 %.  Of the widths that are allowed, the one with the least estimated time.
 Pieces make_pieces(const Plan& p) {
   Pieces c;
-  const size_t words = p.split ? 2 : 1;
-  long long most = (long long)(kPieceBytes / ((size_t)p.rows_p * words * 2)) / kPad * kPad;
+  const size_t words = p.split ? 2 : 1, logits = (size_t)p.rows_p * p.classes * 4;
+  const size_t room = logits / 2 < kQBytes ? kQBytes : logits / 2 > kMostQBytes ? kMostQBytes : logits / 2;
+  const long long all = ceil_div(p.classes, kPad) * kPad;
+  long long most = (long long)(room / ((size_t)p.rows_p * words * 2)) / kPad * kPad;
+  // nothing is gained where dx in float32, which several pieces need, is as large as what they save
+  if ((size_t)p.rows_p * all * words * 2 <= room + (size_t)p.rows * p.dim * 4) most = all;
+  if (weights_in_pieces(p) && most > weights_width(p)) most = weights_width(p);
   if (most < kPad) most = kPad;
-  c.n = ceil_div(p.classes, most);
-  c.width = ceil_div(ceil_div(p.classes, c.n), kPad) * kPad;
+  if (most >= p.classes) {
+    c.width = (int)all;
+    c.cut = cut_for(p, c.width, false);
+  } else {
+    const int fewest = ceil_div(p.classes, most);
+    float least = INFINITY;
+    for (int k = 0; k < 8; ++k) {  // equal pieces, and widths of whole tiles with what is left over
+      const long long unit = most >= 1024 ? 256 : kPad, some = (most - most * (k - 4) / 8) / unit * unit;
+      const long long width = k < 4 ? (long long)ceil_div(ceil_div(p.classes, fewest + k), kPad) * kPad : some < unit ? unit : some;
+      const long long whole = p.classes / width, rest = p.classes - whole * width;
+      const Cut cut = cut_for(p, (int)width, true);
+      float us = 0.f;
+      for (const long long n : {width, rest}) {
+        if (n == 0) continue;
+        const int tile = tile_for(p.rows_p, n, p.dim_p, p.split);
+        const float steps = (float)p.dim_p / (p.split ? 32 : 64);
+        const float one = launch_us(tile, p.split, (long long)ceil_div(p.rows_p, tile) * ceil_div(n, tile), steps) + 8.f +
+                          (n == width ? cut.us : cut_for(p, ceil_div(n, kPad) * kPad, true).us);
+        us += n == width ? one * whole : one;
+      }
+      if (us < least) least = us, c.width = (int)width, c.cut = cut;
+    }
+  }
   c.n = ceil_div(p.classes, c.width);
-  c.cut = cut_for(p, c.width, c.n > 1);
   c.x_joined = c.n > 1 || c.cut.x > 1;
   size_t at = 0;
   c.q_at = at, at = up(at + (size_t)p.rows_p * c.width * words * 2);
@@ -781,22 +848,28 @@ Pieces make_pieces(const Plan& p) {
   c.factors_at = at, at = up(at + (size_t)(p.rows_p + 1) * sizeof(RowFactor));  // E behind them
   c.x_at = at, at = up(at + (c.x_joined ? (size_t)c.cut.x * p.rows * p.dim * 4 : 0));
   c.w_at = at, at = up(at + (c.cut.w > 1 ? (size_t)c.cut.w * c.width * p.dim * 4 : 0));
+  c.weights_at = at, at = up(at + (weights_in_pieces(p) ? (size_t)c.width * p.ld * 2 : 0));
   c.bytes = at;
   return c;
 }
 
 struct ForwardRoom {
-  size_t parts_at, best_at, target_at, sums_at, max_at, bytes;
+  int width, tile, strips;  // classes, tile side and strips of a piece (of the weights where these are laid out in pieces)
+  size_t parts_at, best_at, target_at, sums_at, max_at, weights_at, bytes;
 };
 ForwardRoom make_room(const Plan& p, bool with_pred) {
   ForwardRoom f;
-  const size_t strips = (size_t)ceil_div(p.classes, tile_for(p.rows, p.classes, p.dim_p, p.split)) * 2;
+  f.width = weights_in_pieces(p) ? weights_width(p) : p.classes;
+  f.tile = tile_for(p.rows, f.width, p.dim_p, p.split);
+  f.strips = ceil_div(f.width, f.tile) * 2;
+  const size_t strips = (size_t)f.strips * ceil_div(p.classes, f.width);
   size_t at = 0;
   f.parts_at = at, at = up(at + strips * p.rows_p * sizeof(float2));
   f.best_at = at, at = up(at + (with_pred ? strips * p.rows_p * sizeof(int) : 0));
   f.target_at = at, at = up(at + (size_t)p.rows_p * 4);
   f.sums_at = at, at = up(at + (size_t)(p.rows_p / 16) * sizeof(Sum));
   f.max_at = at, at = up(at + (size_t)2 * kMaxParts * 4);
+  f.weights_at = at, at = up(at + (weights_in_pieces(p) ? (size_t)f.width * p.ld * 2 : 0));
   f.bytes = at;
   return f;
 }
@@ -815,11 +888,20 @@ struct Call {
   hipStream_t stream;
 };
 
-uint16_t* weights_of(const Plan& p, const Call& c) {
-  return p.copy_w ? reinterpret_cast<uint16_t*>(c.saved + p.w_at)
-                  : const_cast<uint16_t*>(static_cast<const uint16_t*>(c.weight));
+// The weights of the classes from class0 on as an operand of the products reads them: kept, a piece of them laid out here
+// (at `room`), or where the caller has them.
+template <int T>
+Operand weights_of(const Plan& p, const Call& c, int class0, int classes, char* room) {
+  if (p.keep_w) return {reinterpret_cast<uint16_t*>(c.saved + p.w_at) + (long long)class0 * p.ld, p.ld, classes, p.dim_p};
+  constexpr int bytes = T == MI_TYPE_F32 ? 4 : 2;
+  const char* w = static_cast<const char*>(c.weight) + (long long)class0 * c.w_stride * bytes;
+  if (!p.copy_w) return {reinterpret_cast<const uint16_t*>(w), c.w_stride, classes, p.dim_p};
+  const int most = 8 * compute_units(), grid = ceil_div(classes, 4) < most ? ceil_div(classes, 4) : most;
+  uint16_t* to = reinterpret_cast<uint16_t*>(room);
+  lay_out_weights<T><<<grid, 256, 0, c.stream>>>(w, c.w_stride, classes, p.dim, p.dim_p, to,
+                                                reinterpret_cast<const Scalars*>(c.saved + p.scalars_at));
+  return {to, p.ld, classes, p.dim_p};
 }
-long long weights_ld(const Plan& p, const Call& c) { return p.copy_w ? p.ld : c.w_stride; }
 
 template <int T, class LABEL>
 void lay_out_all(const Plan& p, const Call& c, float* maxima) {
@@ -832,25 +914,25 @@ void lay_out_all(const Plan& p, const Call& c, float* maxima) {
                                                   static_cast<const float*>(c.weight), c.w_stride, labels, c.ignore, p.rows,
                                                   p.classes, p.dim, xb, maxima);
   }
-  const int rows = p.rows_p + (p.copy_w ? p.classes : 0), most = 8 * compute_units();
+  const int rows = p.rows_p + (p.keep_w ? p.classes : 0), most = 8 * compute_units();
   const int grid = ceil_div(rows, 4) < most ? ceil_div(rows, 4) : most;
   lay_out<T, LABEL><<<grid, 256, 0, c.stream>>>(
       c.x, c.x_stride, c.weight, c.w_stride, labels, c.ignore, p.rows, p.rows_p, p.classes, p.dim, p.dim_p,
-      reinterpret_cast<uint16_t*>(c.saved + p.x_at), p.copy_w ? reinterpret_cast<uint16_t*>(c.saved + p.w_at) : nullptr,
+      reinterpret_cast<uint16_t*>(c.saved + p.x_at), p.keep_w ? reinterpret_cast<uint16_t*>(c.saved + p.w_at) : nullptr,
       reinterpret_cast<int*>(c.saved + p.lab_at), maxima, xb, wb, reinterpret_cast<Scalars*>(c.saved + p.scalars_at));
 }
 
 template <class P, int T>
-int launch_logits(const Plan& p, const Call& c, const ForwardRoom& f, bool with_pred) {
+int launch_logits(const Plan& p, const Call& c, const ForwardRoom& f, bool with_pred, int class0, const Operand& w, int strip0) {
   const Operand x = {reinterpret_cast<uint16_t*>(c.saved + p.x_at), p.ld, p.rows_p, p.dim_p};
-  const Operand w = {weights_of(p, c), weights_ld(p, c), p.classes, p.dim_p};
-  const int tm = ceil_div(p.rows, P::BM), tn = ceil_div(p.classes, P::BN);
+  const int tm = ceil_div(p.rows, P::BM), tn = ceil_div(w.rows, P::BN);
+  const long long part0 = (long long)strip0 * p.rows_p;
   const auto kernel = with_pred ? logits_forward<P, T, true> : logits_forward<P, T, false>;
   allow_lds(kernel, P::kLds);
   kernel<<<tm * tn, P::kThreads, P::kLds, c.stream>>>(
       x, w, c.bias, reinterpret_cast<const int*>(c.saved + p.lab_at), reinterpret_cast<const Scalars*>(c.saved + p.scalars_at),
-      p.rows, p.rows_p, p.classes, tm, tn, p.dim_p / P::kStep, reinterpret_cast<float2*>(c.room + f.parts_at),
-      reinterpret_cast<int*>(c.room + f.best_at), reinterpret_cast<float*>(c.room + f.target_at));
+      p.rows, p.rows_p, class0, w.rows, tm, tn, p.dim_p / P::kStep, reinterpret_cast<float2*>(c.room + f.parts_at) + part0,
+      with_pred ? reinterpret_cast<int*>(c.room + f.best_at) + part0 : nullptr, reinterpret_cast<float*>(c.room + f.target_at));
   return tn * P::WC;
 }
 
@@ -863,10 +945,15 @@ int forward(const Plan& p, const Call& c, float* loss, float* losses, int64_t* p
     lay_out_all<T, int64_t>(p, c, maxima);
   else
     lay_out_all<T, int32_t>(p, c, maxima);
-  const int tile = tile_for(p.rows, p.classes, p.dim_p, split);
-  const int strips = tile == 256   ? launch_logits<Tile256<split, bf16, false, false>, T>(p, c, f, pred != nullptr)
-                     : tile == 128 ? launch_logits<Tile128<split, bf16, false, false>, T>(p, c, f, pred != nullptr)
-                                   : launch_logits<Tile64<split, bf16, false, false>, T>(p, c, f, pred != nullptr);
+  int strips = 0;
+  for (int class0 = 0; class0 < p.classes; class0 += f.width) {
+    const int classes = p.classes - class0 < f.width ? p.classes - class0 : f.width;
+    const Operand w = weights_of<T>(p, c, class0, classes, c.room + f.weights_at);
+    const bool with = pred != nullptr;
+    strips += f.tile == 256   ? launch_logits<Tile256<split, bf16, false, false>, T>(p, c, f, with, class0, w, strips)
+              : f.tile == 128 ? launch_logits<Tile128<split, bf16, false, false>, T>(p, c, f, with, class0, w, strips)
+                              : launch_logits<Tile64<split, bf16, false, false>, T>(p, c, f, with, class0, w, strips);
+  }
   join_strips<<<p.rows_p / 16, 256, 0, c.stream>>>(
       reinterpret_cast<const float2*>(c.room + f.parts_at), pred ? reinterpret_cast<const int*>(c.room + f.best_at) : nullptr,
       strips, reinterpret_cast<const int*>(c.saved + p.lab_at), p.rows, p.rows_p,
@@ -877,16 +964,14 @@ int forward(const Plan& p, const Call& c, float* loss, float* losses, int64_t* p
 }
 
 template <class P, int T>
-int launch_q(const Plan& p, const Call& c, const Pieces& s, int class0, int classes, int classes_p, bool want_bias, bool whole) {
+int launch_q(const Plan& p, const Call& c, const Pieces& s, int class0, const Operand& w, int classes_p, bool want_bias, bool whole) {
   const Operand x = {reinterpret_cast<uint16_t*>(c.saved + p.x_at), p.ld, p.rows_p, p.dim_p};
-  const long long ld = weights_ld(p, c);
-  const Operand w = {weights_of(p, c) + (long long)class0 * ld, ld, classes, p.dim_p};
   const int tm = ceil_div(p.rows_p, P::BM), tn = ceil_div(classes_p, P::BN);
   allow_lds(logits_backward<P, T>, P::kLds);
   logits_backward<P, T><<<tm * tn, P::kThreads, P::kLds, c.stream>>>(
       x, w, c.bias, reinterpret_cast<const int*>(c.saved + p.lab_at), reinterpret_cast<const float*>(c.saved + p.lse_at),
       c.reduction == MI_REDUCTION_NONE ? reinterpret_cast<const RowFactor*>(c.room + s.factors_at) : nullptr, whole,
-      reinterpret_cast<const Scalars*>(c.saved + p.scalars_at), p.rows_p, class0, classes, classes_p, tm, tn,
+      reinterpret_cast<const Scalars*>(c.saved + p.scalars_at), p.rows_p, class0, w.rows, classes_p, tm, tn,
       p.dim_p / P::kStep, reinterpret_cast<uint16_t*>(c.room + s.q_at),
       want_bias ? reinterpret_cast<float*>(c.room + s.sums_at) : nullptr);
   return tm * P::WR;
@@ -919,21 +1004,21 @@ int backward(const Plan& p, const Call& c, const float* grad, void* grad_x, void
                                           exponent);
   const Factor factor = {by_row ? nullptr : grad, sc, by_row ? factors : nullptr, exponent, c.reduction == MI_REDUCTION_MEAN};
   uint16_t* q = reinterpret_cast<uint16_t*>(c.room + s.q_at);
-  const long long ldw = weights_ld(p, c);
   float* x_room = s.x_joined ? reinterpret_cast<float*>(c.room + s.x_at) : nullptr;
   float* w_room = s.cut.w > 1 ? reinterpret_cast<float*>(c.room + s.w_at) : nullptr;
   for (int k = 0; k < s.n; ++k) {
     const int class0 = k * s.width, classes = p.classes - class0 < s.width ? p.classes - class0 : s.width;
     const int classes_p = ceil_div(classes, kPad) * kPad;
     const int tile = tile_for(p.rows_p, classes_p, p.dim_p, split);
+    const Operand weights = weights_of<T>(p, c, class0, classes, c.room + s.weights_at);
     const bool want_b = grad_b != nullptr, ends = k + 1 == s.n, whole = by_row && grad_x == nullptr;
     const int strips =
-        tile == 256   ? launch_q<Tile256<split, bf16, false, false>, T>(p, c, s, class0, classes, classes_p, want_b, whole)
-        : tile == 128 ? launch_q<Tile128<split, bf16, false, false>, T>(p, c, s, class0, classes, classes_p, want_b, whole)
-                      : launch_q<Tile64<split, bf16, false, false>, T>(p, c, s, class0, classes, classes_p, want_b, whole);
+        tile == 256   ? launch_q<Tile256<split, bf16, false, false>, T>(p, c, s, class0, weights, classes_p, want_b, whole)
+        : tile == 128 ? launch_q<Tile128<split, bf16, false, false>, T>(p, c, s, class0, weights, classes_p, want_b, whole)
+                      : launch_q<Tile64<split, bf16, false, false>, T>(p, c, s, class0, weights, classes_p, want_b, whole);
     // every piece has the same slices of q W: a last, shorter piece leaves some of them empty
     const Gradient x = {{q, (long long)classes_p * words, p.rows_p, classes_p},
-                        {weights_of(p, c) + class0 * ldw, ldw, p.dim, classes},
+                        {weights.base, weights.ld, p.dim, classes},
                         p.rows, p.dim, 0, 0, classes_p / step, 0, grad_x, x_room, k > 0};
     void* w_out = grad_w == nullptr ? nullptr : static_cast<char*>(grad_w) + (size_t)class0 * p.dim * out_bytes;
     const Gradient w = {{q, (long long)classes_p * words, classes_p, p.rows_p},
