@@ -469,6 +469,7 @@ struct Factor {
   const RowFactor* rows;
   const int* exponent;  // E
   int mean;
+  const int* lab;
 };
 // It and the operands' scales, as one number in [1, 2) and a power of two: their product alone may be no float where the result is one.
 struct Undo {
@@ -662,11 +663,8 @@ __device__ __forceinline__ void gradient_tile(const Gradient& g, int id, const F
   P::hand_out(acc, lds, [&](int r0, int c0, f32x4 v) {
     const int row = tm * P::BM + r0, col = tn * P::BN + c0;
     if (row >= g.rows || col >= g.cols) return;
-    if (!OF_WEIGHT && factor.rows != nullptr) {
-      const float w = factor.rows[row].w;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = w == 0.f ? 0.f : v[r] * w;
-    }
+    if (!OF_WEIGHT && factor.rows != nullptr) v *= factor.rows[row].w;
+    if (!OF_WEIGHT && factor.lab[row] == kIgnored) v = f32x4{0.f, 0.f, 0.f, 0.f};  // q is 0 there, but 0 times a weight may be NaN
     if (g.slices != nullptr) {
       float* at = g.slices + ((long long)slice * g.rows + row) * g.cols + col;
       if (whole) {
@@ -1002,7 +1000,8 @@ int backward(const Plan& p, const Call& c, const float* grad, void* grad_x, void
   if (by_row)
     row_factors<<<1, 1024, 0, c.stream>>>(grad, reinterpret_cast<const int*>(c.saved + p.lab_at), p.rows, p.rows_p, factors,
                                           exponent);
-  const Factor factor = {by_row ? nullptr : grad, sc, by_row ? factors : nullptr, exponent, c.reduction == MI_REDUCTION_MEAN};
+  const Factor factor = {by_row ? nullptr : grad, sc, by_row ? factors : nullptr, exponent, c.reduction == MI_REDUCTION_MEAN,
+                         reinterpret_cast<const int*>(c.saved + p.lab_at)};
   uint16_t* q = reinterpret_cast<uint16_t*>(c.room + s.q_at);
   float* x_room = s.x_joined ? reinterpret_cast<float*>(c.room + s.x_at) : nullptr;
   float* w_room = s.cut.w > 1 ? reinterpret_cast<float*>(c.room + s.w_at) : nullptr;

@@ -146,7 +146,7 @@ def linear_cross_entropy(x, weight, bias, labels, ignore_index=-1, reduction="me
     """Cross entropy of softmax(x weight^T + bias) against `labels`, float32.
 
     Rows with label `ignore_index` (the framework's padding rows: -1) count nowhere and get a zero gradient, whatever x holds
-    there; 'mean' runs over the other rows and is 0 when there are none.  A label that is neither ignored nor a class makes
+    there and the weight anywhere; 'mean' runs over the other rows and is 0 when there are none.  A label that is neither ignored nor a class makes
     its row's loss NaN.  `with_pred`: also the class of the largest logit per row (int64, lowest index of equal ones, -1
     for ignored rows).  The backward is captured into a graph or run eagerly like the forward: no host synchronisation."""
     _check(x, weight, bias, labels, reduction)

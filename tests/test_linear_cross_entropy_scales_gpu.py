@@ -109,3 +109,23 @@ def test_weighted_rows_over_several_pieces(dtype):
         want += torch.autograd.grad(linear_cross_entropy(x, w, b, mine, reduction="sum"), (w,))[0].double() * p.double()
     u = 2 * HALF_STEP[dtype] if dtype != torch.float32 else 2.0 ** -18
     assert float((got[1].double() - want).norm() / want.norm()) <= u
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("classes", [70, 3001])
+def test_ignored_rows_beside_a_weight_that_is_no_number(classes, reduction, dtype):
+    """A row that does not count has a gradient of zero, whatever the other operand holds; the others show it."""
+    for value in (float("nan"), float("inf")):
+        x, w, b, y = make(200, 64, classes, dtype, ignored=0.4)
+        bad = w.detach().clone()
+        bad[classes // 2, 11] = value
+        bad.requires_grad_(True)
+        loss = linear_cross_entropy(x, bad, b, y, reduction=reduction).sum()
+        gx, gw, gb = torch.autograd.grad(loss, (x, bad, b))
+        rows = y == -1
+        # (a row of that class itself, at a logit of -inf: q = -1, -1 times inf)
+        assert bool((gx[rows] == 0).all()) and not bool(torch.isfinite(gx[~rows]).all(dim=1).any())
+        none = torch.full_like(y, -1)
+        for t in torch.autograd.grad(linear_cross_entropy(x, bad, b, none, reduction=reduction).sum(), (x, bad, b)):
+            assert bool((t == 0).all())
