@@ -18,6 +18,7 @@ Flags that matter:
 import os
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -52,6 +53,33 @@ def flags():
     return out
 
 
+# what the host pass says of a feature that only the device has
+HOST_LINE = "'-packed-fp32-ops' is not a recognized feature for this target (ignoring feature)"
+
+
+def worth_saying(output):
+    """The compiler's lines without the expected one."""
+    return [line for line in output.splitlines() if line.strip() and line.strip() != HOST_LINE]
+
+
+def check_no_packed_fp32(options):
+    """Raises unless `options` keep packed float32 instructions out of device code that would have them otherwise: a device pass that
+    ignores the feature says the same line as the host pass does, so a probe is compiled."""
+    with tempfile.TemporaryDirectory() as folder:
+        source = os.path.join(folder, "probe.hip")
+        with open(source, "w") as f:
+            f.write("#include <hip/hip_runtime.h>\n__global__ void probe(float2* a, const float2* b) {\n"
+                    "  a[threadIdx.x].x = a[threadIdx.x].x * b[threadIdx.x].x;\n"
+                    "  a[threadIdx.x].y = a[threadIdx.x].y * b[threadIdx.x].y;\n}\n")
+        p = subprocess.run([hipcc()] + options + ["--cuda-device-only", "-S", source, "-o", "-"], stdout=subprocess.PIPE,
+                           stderr=subprocess.PIPE)
+    if p.returncode != 0:
+        raise RuntimeError("hipcc failed on the probe:\n%s" % p.stderr.decode(errors="replace"))
+    code = p.stdout.decode(errors="replace")
+    if "v_mul_f32" not in code or any("v_pk_%s_f32" % op in code for op in ("add", "mul", "fma")):
+        raise RuntimeError("the compiler makes packed float32 instructions in spite of the build's options")
+
+
 def stale():
     if not os.path.exists(LIB_PATH):
         return True
@@ -67,6 +95,7 @@ def build(force=False, verbose=True):
         return LIB_PATH
     obj_dir = os.path.join(HERE, "build")
     os.makedirs(obj_dir, exist_ok=True)
+    check_no_packed_fp32(flags())
     procs = []
     for src in SOURCES:
         obj = os.path.join(obj_dir, src.replace(".hip", ".o"))
@@ -77,8 +106,8 @@ def build(force=False, verbose=True):
         out, _ = p.communicate()
         if p.returncode != 0:
             raise RuntimeError("hipcc failed on %s:\n%s" % (src, out.decode(errors="replace")))
-        said = [line for line in out.decode(errors="replace").splitlines() if "not a recognized feature" not in line]
-        if verbose and any(line.strip() for line in said):   # (the host pass does not know the device's feature names)
+        said = worth_saying(out.decode(errors="replace"))
+        if verbose and said:
             sys.stderr.write("\n".join(said) + "\n")
         objs.append(obj)
     tmp = LIB_PATH + ".tmp"
