@@ -300,6 +300,11 @@ struct TileProduct {
   // place: a strip's are all asked for before the first of its stores, behind which the compiler would not move them.  With COLUMNS
   // `by_row` returns what it made of v, and `by_column(row, col, v)` gets four rows of a column of that a lane, lanes along the
   // column, for a result that is also stored transposed.
+  // Lanes read there what other lanes of their wave wrote: LDS takes a wave's operations in order, lanes_meet() keeps the compiler to it.
+  static __device__ __forceinline__ void lanes_meet() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+  }
   static constexpr int kPitch = FN * 32 + 4;
   static_assert(kWaves * 32 * kPitch * 4 <= kLds, "the strips fit where the stages were");
   template <bool COLUMNS, class B, class R, class C>
@@ -317,6 +322,7 @@ struct TileProduct {
 #pragma unroll
         for (int g = 0; g < 4; ++g)
           *reinterpret_cast<quad_at>(mine + ((lane & 31) * kPitch + j * 32 + g * 8 + (lane >> 5) * 4) * 4) = quad(acc[i][j], g);
+      lanes_meet();
       constexpr int kQuads = FN * 8, kRows = 64 / kQuads;
       const int r = lane / kQuads, c = lane % kQuads * 4, rc = (lane & 7) * 4, cc = lane >> 3;
       f32x4 old[32 / kRows];
@@ -330,12 +336,14 @@ struct TileProduct {
         else
           by_row(row0 + i * 32 + n * kRows + r, col0 + c, *p, old[n]);
       }
+      lanes_meet();
       if constexpr (COLUMNS) {
 #pragma unroll
         for (int n = 0; n < FN * 4; ++n) {
           const float_at p = reinterpret_cast<float_at>(mine + (rc * kPitch + n * 8 + cc) * 4);
           by_column(row0 + i * 32 + rc, col0 + n * 8 + cc, f32x4{p[0], p[kPitch], p[2 * kPitch], p[3 * kPitch]});
         }
+        lanes_meet();
       }
     }
   }
