@@ -170,12 +170,15 @@ __device__ __forceinline__ void put_results(const Mat& q, const Step& s, A at, I
   }
 #pragma unroll
   for (int e = 0; e < 16; ++e)
-    if (inside(e)) store_float<T>(q.out, at(e), s.update ? w[e] * s.decay - s.lr * q.shape * o[e] : o[e]);
+    if (inside(e)) store_float<T>(q.out, at(e), s.update ? fmaf(w[e], s.decay, -(s.lr * q.shape) * o[e]) : o[e]);
 }
 // Four of them on their alignment, with the old weights.
 template <int T>
 __device__ __forceinline__ void put_result4(const Mat& q, const Step& s, long long i, f32x4 o, f32x4 w) {
-  if (s.update) o = w * s.decay - (s.lr * q.shape) * o;
+  if (s.update) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = fmaf(w[r], s.decay, -(s.lr * q.shape) * o[r]);  // one rounding of a weight's size, not three
+  }
   if constexpr (T == MI_TYPE_F32) {
     *reinterpret_cast<f32x4*>(static_cast<float*>(q.out) + i) = o;
   } else {
@@ -1094,7 +1097,7 @@ int mi_muon_step(int count, void* const* params, const void* const* grads, float
   if (const int rc = check_matrices(count, rows, cols)) return rc;
   if (const int rc = check_coefficients(coefficients, steps, eps, growth)) return rc;
   MI_REQUIRE(momenta != nullptr, "mi_muon_step: null pointer");
-  const Step s = {coefficients[0], coefficients[1], coefficients[2], eps, momentum, lr, 1.f - lr * weight_decay, nesterov, 1, steps};
+  const Step s = {coefficients[0], coefficients[1], coefficients[2], eps, momentum, lr, (float)(1.0 - (double)lr * weight_decay), nesterov, 1, steps};
   return run_all(count, grads, params, momenta, rows, cols, dtype, s, growth, workspace, workspace_bytes, as_stream(stream),
                  "mi_muon_step");
 }

@@ -156,3 +156,14 @@ def test_singular_values_near_the_largest_that_is_stored(coefficients, steps, m,
     g = gradient(m, 1, torch.float32) @ gradient(1, n, torch.float32)
     close(orthogonalize(g, steps=steps, coefficients=coefficients), formula(g, steps, coefficients), torch.float32, "rank one",
           max(ITERATION, noise(coefficients, steps)))
+
+
+@pytest.mark.parametrize("m,n", SIDES)
+def test_a_weight_is_rounded_once(m, n):
+    """Half a step of the new weight, and the decay's own rounding (half a step of a number in [0.5, 1)); what the iteration is off by is
+    small beside that for weights around 100 and a rate of 2e-4."""
+    p, g, mom = 100 * gradient(m, n, torch.float32, 1) / 1e-2, gradient(m, n, torch.float32, 2), torch.zeros(m, n, device=DEV)
+    want, _ = reference_step(p, g, mom, 2e-4, 0.95, 0.5, True)
+    muon_step_([p], [g], [mom], lr=2e-4, weight_decay=0.5)
+    bound = (2.0 ** -24 + 1.01 * 2.0 ** -25) * want.abs() + 2e-4 * max(1.0, m / n) ** 0.5 * 4 * ITERATION
+    assert bool(((p.double() - want).abs() <= bound).all())
