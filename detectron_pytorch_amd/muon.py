@@ -153,13 +153,13 @@ class Muon(torch.optim.Optimizer):
 
 
 def _sgd_step_(params, grads, momenta, lr, momentum, weight_decay):
-    """torch.optim.SGD's momentum step (coupled weight decay, no dampening) of a list, in float32."""
+    """torch.optim.SGD's momentum step (coupled weight decay, no dampening) of a list, with float32 momenta."""
     grads = [g.float() for g in grads]
     torch._foreach_mul_(momenta, momentum)
     torch._foreach_add_(momenta, grads)
     if weight_decay:
         torch._foreach_add_(momenta, [p.float() for p in params], alpha=weight_decay)
-    if params[0].dtype == torch.float32:
+    if params[0].dtype in (torch.float32, torch.float64):
         torch._foreach_add_(params, momenta, alpha=-lr)
     else:   # rounded once
         for p, m in zip(params, momenta):
