@@ -87,10 +87,15 @@ def _same_order(t, like):
     return (t.is_contiguous() and like.is_contiguous()) or t.stride() == like.stride()
 
 
+def _is_captured(p):
+    return p.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 class Muon(torch.optim.Optimizer):
     """Parameters of two or more dimensions take the orthogonalised step with `lr`, the others momentum SGD with `sgd_lr`
     (lr when None) and `sgd_momentum`.  Per group as usual: {"params": ..., "lr": ..., "sgd_lr": ..., "weight_decay": ...};
-    "orthogonalize": False keeps a group's matrices on SGD too.  Momenta are float32, whatever the parameter's type."""
+    "orthogonalize": False keeps a group's matrices on SGD too.  Momenta are float32, whatever the parameter's type.  A step can be
+    captured into a graph after one that ran (which made the momenta)."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, sgd_lr=None, sgd_momentum=0.9,
                  steps=STEPS, coefficients=COEFFICIENTS, eps=EPS, orthogonalize=True):
@@ -103,10 +108,15 @@ class Muon(torch.optim.Optimizer):
     def _momentum(self, p):
         state = self.state[p]
         buf = state.get("momentum_buffer")
+        if buf is not None and _same_order(buf, p):
+            return buf
+        if _is_captured(p):   # every replay would make it anew
+            raise RuntimeError("a step of Muon is captured after one that ran: momenta are made outside of a graph")
         if buf is None:
-            buf = state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
-        elif not _same_order(buf, p):   # the parameter was given another memory format
-            buf = state["momentum_buffer"] = torch.empty_like(p, dtype=torch.float32).copy_(buf)
+            buf = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+        else:   # the parameter was given another memory format
+            buf = torch.empty_like(p, dtype=torch.float32).copy_(buf)
+        state["momentum_buffer"] = buf
         return buf
 
     def load_state_dict(self, state_dict):

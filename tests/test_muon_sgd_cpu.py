@@ -1,6 +1,8 @@
 """The parameters of an optimiser with orthogonalised updates that take the momentum SGD step."""
+import pytest
 import torch
 
+from detectron_pytorch_amd import muon
 from detectron_pytorch_amd.muon import Muon
 
 
@@ -31,3 +33,21 @@ def test_16_bit_biases_are_rounded_once():
             assert float((p.detach().double() - (w.double() - 0.1 * m.double())).abs().max()) <= \
                 torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -8) * float(p.detach().abs().max().double() + 1)
             w = p.detach().clone()
+
+
+def test_momenta_are_not_made_inside_a_graph(monkeypatch):
+    """They would be cleared, or taken from a tensor that is gone, at every replay."""
+    w = torch.nn.Parameter(torch.randn(4, 3, 2, 2))
+    opt = Muon([w], orthogonalize=False)
+    w.grad = torch.randn(4, 3, 2, 2)
+    monkeypatch.setattr(muon, "_is_captured", lambda p: True)
+    with pytest.raises(RuntimeError, match="captured"):
+        opt.step()
+    assert len(opt.state) == 0 or "momentum_buffer" not in opt.state[w]
+    monkeypatch.setattr(muon, "_is_captured", lambda p: False)
+    opt.step()
+    monkeypatch.setattr(muon, "_is_captured", lambda p: True)
+    opt.step()
+    w.data = w.data.contiguous(memory_format=torch.channels_last)
+    with pytest.raises(RuntimeError, match="captured"):
+        opt.step()
