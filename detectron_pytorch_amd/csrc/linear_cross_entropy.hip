@@ -9,9 +9,9 @@
 // of it at a time: make_pieces) and multiplies q by the weights and by the features.
 //
 // Work: 2 R V D operations forward, 6 R V D backward (one third of it the logits' second time).  Bound by the matrix cores
-// wherever R and V fill the chip: at 8192 x 4096 and 50021 classes in bf16 the forward's logits take 2.72 ms (1233 TFLOP/s), the
-// backward's with q 3.12 ms, both gradients 5.28 ms (1273 TFLOP/s).  By launches and the latency of a K loop where they do
-// not: 1024 x 1024 and 81 classes in float32 take 58 us in seven launches.
+// wherever R and V fill the chip: at 8192 x 4096 and 50021 classes in bf16 the forward's logits take 2.73 ms (1230 TFLOP/s), the
+// backward's with q 3.20 ms, both gradients 5.67 ms (1183 TFLOP/s), these in four pieces.  By launches and the latency of a K loop where they do
+// not: 1024 x 1024 and 81 classes in float32 take 59 us in seven launches.
 //
 // Types.  16-bit features and weights are multiplied as they are, in place.  float32 ones are laid out as hi + lo fp16 under one
 // power-of-two scale per tensor (its largest finite magnitude lands in [2^14, 2^15), so hi + lo carry 22 bits for
@@ -693,7 +693,8 @@ __device__ __forceinline__ void gradient_tile(const Gradient& g, int id, const F
 }
 
 // All gradients of a piece in one launch: the tiles of q W, those of q' x, and the bias' columns, 64 a workgroup.  Where each
-// product alone would leave compute units empty, they fill up together (1024 x 1024 and 1204 classes in float32: 29 us).
+// product alone would leave compute units empty, they fill up together (1024 x 1024 and 1204 classes in float32: 31 us).  With a gradient
+// per row they go out in two, q being weighed in between.
 template <class PX, class PW, int T>
 __global__ __launch_bounds__(PX::kThreads, kWavesPerSimd<PX>) void gradients(Gradient x, Gradient w, BiasGradient bias, int x_blocks,
                                                                              int w_blocks, Factor factor) {

@@ -23,8 +23,9 @@
 // error at that of separate iterations (2.1e-6 to 5.2e-6 of the norm against 2.1e-6 to 4.9e-6 on Gaussian and strongly
 // low-rank 256 x 1024; with all five in one pass 1e-4).
 //
-// Bound by the matrix cores on long matrices (1024 x 12544: Gram 45 + 9 us, C X 90 us, 292 TFLOP/s in float32 terms) and by the
-// latency of the m x m products, which are too small for the chip (1024: 16 us, 2048: 46 to 51 us).
+// Bound by the matrix cores on long matrices (1024 x 12544: Gram 45 + 9 us, C X 92 us, 285 TFLOP/s in float32 terms) and by the m x m
+// products, which are too small for the chip: their 136 tiles leave nearly half of the compute units without one (1024: 16 us, 2048: 49
+// to 52 us).
 //
 // Accumulators are float32; the norm is summed in fp64, so no gradient is too small or too large for it.
 // All matrices of a call go through each stage in one launch: a workgroup finds its matrix in the call's table.
@@ -679,7 +680,7 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void square(Tiles ti
 }
 
 // X <- C X (or Q X, several iterations at once), or in the last pass the result itself, with the optimiser's step: the update never
-// lies in memory (21 matrices, 20.9 M weights: 172 us, a pass that only writes X 101).
+// lies in memory (21 matrices, 20.9 M weights: 174 us, a pass that only writes X 103).
 template <class P, int T, bool LAST>
 __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void apply(Tiles tiles, Step s, char* ws, int factor, int flip) {
   extern __shared__ char smem[];
