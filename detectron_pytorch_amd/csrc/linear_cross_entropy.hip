@@ -457,8 +457,8 @@ __global__ __launch_bounds__(256) void join_strips(const float2* part, const int
 
 // ---- backward ------------------------------------------------------------------------------------------------------------
 
-// A single row's gradient as m 2^(E + log2 w): E is the largest exponent of all rows, m in [1, 2), w a power of two up to 1 (0: the row
-// does not count).  q holds m only, so that a row of small gradient keeps its bits; dx gets w when its sums are done.
+// A single row's gradient as m 2^(E + log2 w): E is the largest exponent of all rows, m in [1, 2), w a power of two up to 1 (0: the row's
+// gradient is below 2^-149 of the largest).  q holds m only, so that a row of small gradient keeps its bits; dx gets w when its sums are done.
 struct RowFactor {
   float m, w;
 };
@@ -499,7 +499,7 @@ __global__ __launch_bounds__(1024) void row_factors(const float* grad, const int
   for (int i = 0; i < 16; ++i) most = max(most, sm[i]);
   if (most == INT_MIN) most = 0;
   for (int i = threadIdx.x; i < rows_p; i += 1024) {
-    RowFactor f = {0.f, 0.f};
+    RowFactor f = {0.f, 1.f};  // a row that does not count: zeros in q
     if (i < rows && lab[i] != kIgnored) {
       const float g = grad[i];
       const int e = counts(g) ? ilogbf(g) : most;
@@ -517,7 +517,7 @@ __global__ __launch_bounds__(256) void weigh_rows(const RowFactor* factors, int 
   constexpr int words = T == MI_TYPE_F32 ? 2 : 1;
   for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < rows_p; r += gridDim.x * 4) {
     const float w = factors[r].w;
-    if (w == 1.f || w == 0.f) continue;  // 0: a row of zeros
+    if (w == 1.f) continue;
     uint16_t* row = q + (long long)r * classes_p * words;
     for (int c = (threadIdx.x & 63) * 8; c < classes_p; c += 512) {
       if constexpr (T == MI_TYPE_F32) {
@@ -574,7 +574,7 @@ __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_backward
     const float l = in ? lse[row] : INFINITY;
     RowFactor g = {1.f, 1.f};
     if (factors != nullptr) {
-      g = in ? factors[row] : RowFactor{0.f, 0.f};
+      g = in ? factors[row] : RowFactor{0.f, 1.f};
       if (whole) g = {g.m * g.w, 1.f};
     }
     const float f = g.m * kQScale;

@@ -129,3 +129,19 @@ def test_ignored_rows_beside_a_weight_that_is_no_number(classes, reduction, dtyp
         none = torch.full_like(y, -1)
         for t in torch.autograd.grad(linear_cross_entropy(x, bad, b, none, reduction=reduction).sum(), (x, bad, b)):
             assert bool((t == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_row_gradients_at_the_two_ends_of_a_float(dtype):
+    """A row whose gradient is nothing beside the others' leaves no trace in the sum over rows."""
+    x, w, b, y = make(130, 64, 300, dtype, ignored=0.0)
+    g = torch.full((130,), 2.0 ** 20, device=DEV)
+    g[40], g[41], g[42] = 2.0 ** -145, 2.0 ** -120, -2.0 ** -100
+    want = formulas(x, w, b, y, reduction="none", grad=g)
+    losses = linear_cross_entropy(x, w, b, y, reduction="none")
+    for wanted in ((0, 1, 2), (1,), (1, 2), (0,)):
+        got = torch.autograd.grad(losses, [(x, w, b)[k] for k in wanted], g, retain_graph=True)
+        for k, t in zip(wanted, got):
+            close(t, want[2 + k], "%s of %s" % (k, wanted))
+        if 0 in wanted:
+            assert float(got[0][40:43].abs().max()) < 2.0 ** -90
