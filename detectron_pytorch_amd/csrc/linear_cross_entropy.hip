@@ -548,9 +548,9 @@ template <class P, int T>
 __global__ __launch_bounds__(P::kThreads, kWavesPerSimd<P>) void logits_backward(Operand x, Operand w, const void* bias,
                                                                                  const int* lab, const float* lse,
                                                                                  const RowFactor* factors, int whole,
-                                                                                 const Scalars* sc, int rows_p, int class0, int classes, int classes_p,
-                                                                                 int tiles_m, int tiles_n, int steps, uint16_t* q,
-                                                                                 float* sums) {
+                                                                                 const Scalars* sc, int rows_p, int class0,
+                                                                                 int classes, int classes_p, int tiles_m, int tiles_n,
+                                                                                 int steps, uint16_t* q, float* sums) {
   extern __shared__ char smem[];
   int tm, tn;
   tile_of(blockIdx.x, tiles_m, tiles_n, 4, tm, tn);

@@ -505,10 +505,11 @@ int mi_keypoint_nms_oks(const float* xy_preds, const float* rois, int num_rois, 
  * has not kept what the backward needs.  Gradients are formed from probabilities of `dtype`'s bits (float32: 22); in float32 and
  * float16 those below 2^-39 count as zero, for MI_REDUCTION_NONE relative to the row's own gradient in grad_x, to the largest row's
  * in grad_weight.  Results do not depend on the order of execution: every sum has a fixed order.  At most 2^24 rows and classes, 2^20
- * features, and 2^25 tiles of 64 x 64 of the logits (MI_ERR_BAD_ARGUMENT beyond).  Kept are the features as the products read them and
- * up to 128 MB of weights laid out anew; a backward works in at most 256 MB of softmax, 64 MB of partial sums, 128 MB of weights and
- * grad_x in float32: less than float32 logits of 200 MB and more, but for few rows of many features.  `saved` and `workspace` start on 256 bytes,
- * gradients on 16. */
+ * features, and 2^25 tiles of 64 x 64 of the logits (MI_ERR_BAD_ARGUMENT beyond).
+ * Memory: kept are the features as the products read them and up to 128 MB of weights laid out anew (16-bit ones of a multiple of 64
+ * features that do not lie on 16 bytes: all of them).  A backward works in at most 256 MB of softmax, 64 MB of partial sums,
+ * 128 MB of weights and grad_x in float32, a piece being 64 classes at least: less than float32 logits of 200 MB and more, but for
+ * few rows of many features.  `saved` and `workspace` start on 256 bytes, gradients on 16. */
 size_t mi_linear_cross_entropy_saved_bytes(int rows, int dim, int classes, int dtype, const void* weight,
                                            long long weight_stride);
 size_t mi_linear_cross_entropy_workspace_bytes(int rows, int dim, int classes, int dtype, int pass);
