@@ -804,7 +804,7 @@ bool weights_in_pieces(const Plan& p) {
 // where half is less: smaller pieces would leave compute units empty); beside it lie at most an eighth of that in sums for the
 // bias, 32 MB in slices of each product, dx in float32 where there are several pieces, and 128 MB of weights that are not kept (or 64
 // of them).  Several pieces cost the adding up of dx and a launch's last, half-empty round each: 8192 x 4096 and 50021 classes in
-// bf16 take the 11.1 ms that one piece of 0.82 GB takes; pieces of 55 MB cost 8192 x 1024 and 10000 classes 12 %, weights laid out
+// bf16 take 11.1 to 11.4 ms, 0.5 to 2 % more than in one piece of 0.82 GB; pieces of 55 MB cost 8192 x 1024 and 10000 classes 12 %, weights laid out
 // twice 512 x 4096 and 50000 classes in float32 15 %.  Of the widths that are allowed, the one with the least estimated time.
 Pieces make_pieces(const Plan& p) {
   Pieces c;

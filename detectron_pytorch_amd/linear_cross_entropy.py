@@ -65,11 +65,12 @@ def _rows(t):
 def _unpacked(ctx, weight, bias, saved):
     """The saved tensors as the backward reads them, and the distance of the weight's rows.  Hooks on saved tensors
     (torch.autograd.graph.saved_tensors_hooks, save_on_cpu) may give back others: of other strides, at another address."""
+    if (weight.data_ptr(), weight.stride(), saved.data_ptr()) == ctx.places and (bias is None or bias.is_contiguous()):
+        return weight, ctx.w_stride, bias, saved
     weight, stride = _rows(weight)
-    if (weight.data_ptr(), stride) != ctx.weight_at:
-        needed = _lib.lib().mi_linear_cross_entropy_saved_bytes(*ctx.shape, weight.data_ptr(), stride)
-        if needed > saved.numel():   # the forward read it where it lay and kept no copy, which this place does not allow
-            weight, stride = weight.clone(memory_format=torch.contiguous_format), weight.size(1)
+    needed = _lib.lib().mi_linear_cross_entropy_saved_bytes(*ctx.shape, weight.data_ptr(), stride)
+    if needed > saved.numel():   # the forward read it where it lay and kept no copy, which this place does not allow
+        weight, stride = weight.clone(memory_format=torch.contiguous_format), weight.size(1)
     if saved.data_ptr() % 256 or not saved.is_contiguous():
         saved = saved.clone(memory_format=torch.contiguous_format)
     return weight, stride, None if bias is None else bias.contiguous(), saved
@@ -106,7 +107,7 @@ class _LinearCrossEntropy(Function):
                 loss.data_ptr(), pred.data_ptr() if with_pred else None, saved.data_ptr(), saved.numel(), workspace.data_ptr(),
                 ws_bytes, _lib.current_stream_handle(dev))
         _lib.check(rc, "mi_linear_cross_entropy_forward")
-        ctx.weight_at = weight.data_ptr(), w_stride
+        ctx.places, ctx.w_stride = (weight.data_ptr(), weight.stride(), saved.data_ptr()), w_stride
         ctx.save_for_backward(weight, bias, saved)
         if with_pred:
             ctx.mark_non_differentiable(pred)
